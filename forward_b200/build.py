@@ -5,7 +5,7 @@
     python -m forward_b200.build --verbose  # also print ptxas resource usage
 
 Outputs (git-ignored, next to the sources so they travel with the tree):
-    forward_b200/lib/libfwd_eb.so          kernels + C ABI (include/fwd_eb.h)
+    forward_b200/lib/libfwd_eb.so          kernels + C ABI (include/*.h)
     forward_b200/lib/libfwd_eb_plugin.so   EmbeddingBag_TRT plugin, creators and
                                            the host driver used by the tests
 """
@@ -63,7 +63,8 @@ def _run(cmd: list[str], verbose: bool) -> None:
         sys.stdout.write(proc.stdout + proc.stderr)
 
 
-CORE_SOURCES = ("eb_api.cu", "eb_session.cu", "eb_noalloc.cu", "eb_shard.cu")
+CORE_SOURCES = ("eb_api.cu", "eb_session.cu", "eb_noalloc.cu", "eb_shard.cu",
+                "eb_backward.cu", "eb_layer_norm.cu", "eb_adamw.cu")
 
 
 def build_core(force: bool = False, verbose: bool = False) -> str:

@@ -162,6 +162,18 @@ static int validate(const fwd_eb_params* p) {
   return 0;
 }
 
+int check_lookup(const fwd_eb_params* p) {
+  if (!p) return fail(FWD_EB_EINVAL, "params is null");
+  fwd_eb_params q = *p;
+  // these belong to the forward call's result: any valid value passes
+  q.out = &q;
+  q.out_dtype = FWD_EB_F32;
+  q.out_stride = 0;
+  q.strategy = FWD_EB_STRATEGY_AUTO;
+  if (!q.table) q.table = &q;   // not every gradient reads the table
+  return validate(&q);
+}
+
 static int pick_strategy(const fwd_eb_params* p) {
   if (p->strategy != FWD_EB_STRATEGY_AUTO) return p->strategy;
   if (p->num_bags <= 0) return FWD_EB_STRATEGY_GROUP;

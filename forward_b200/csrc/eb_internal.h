@@ -45,5 +45,8 @@ struct PoolArgs;
 // then set), 2 for the lean kernel (eb_lite.cuh), 0 for eb_pool_group_kernel.
 int plan_group(const struct ::fwd_eb_params* p, PoolArgs* args, int* vec, int* cpl, int* tiles, int* stream);
 int sm_count();
+// The argument checks of fwd_eb_forward on a call whose out, out_dtype, out_stride, strategy and
+// workspace do not matter (the gradient of the call).
+int check_lookup(const struct ::fwd_eb_params* p);
 
 }  // namespace fwd_eb

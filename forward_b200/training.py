@@ -1,0 +1,494 @@
+"""Training operators around the pooled lookup (include/fwd_eb_train.h): the gradient of an
+EmbeddingBag call, layer norm with its gradients, and AdamW over many tensors at once.
+
+Like capi, the functions take torch CUDA tensors, launch on the current stream of the tensors'
+device and return without synchronising; outputs and scratch come from torch's allocator.
+Every result is deterministic.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import capi
+
+BF16 = 3
+BACKWARD_ACCUMULATE = 1
+ADAMW_BLOCK = 256
+
+_p, _i32, _i64 = C.c_void_p, C.c_int32, C.c_int64
+
+
+class BackwardParams(C.Structure):
+    """Mirror of struct fwd_eb_backward_params."""
+    _fields_ = [
+        ("fwd", capi.Params), ("grad_out", _p), ("grad_out_dtype", _i32), ("grad_table_dtype", _i32),
+        ("grad_out_stride", _i64), ("grad_table", _p), ("grad_table_stride", _i64), ("grad_weights", _p),
+        ("winners", _p), ("winners_stride", _i64), ("workspace", _p), ("workspace_bytes", C.c_size_t),
+        ("flags", C.c_uint32), ("reserved", _i32),
+    ]
+
+
+class LayerNormParams(C.Structure):
+    """Mirror of struct fwd_eb_layer_norm_params."""
+    _fields_ = [
+        ("x", _p), ("dtype", _i32), ("weight_dtype", _i32), ("rows", _i64), ("cols", _i64), ("x_stride", _i64),
+        ("weight", _p), ("bias", _p), ("eps", C.c_double), ("mean", _p), ("rstd", _p), ("y", _p),
+        ("y_stride", _i64), ("grad_y", _p), ("grad_y_stride", _i64), ("grad_x", _p), ("grad_x_stride", _i64),
+        ("grad_weight", _p), ("grad_bias", _p), ("workspace", _p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class AdamWTensor(C.Structure):
+    """Mirror of struct fwd_eb_adamw_tensor."""
+    _fields_ = [
+        ("param", _p), ("grad", _p), ("master", _p), ("exp_avg", _p), ("exp_avg_sq", _p), ("exp_avg_scale", _p),
+        ("exp_avg_sq_scale", _p), ("n", _i64), ("param_dtype", _i32), ("grad_dtype", _i32), ("state_bits", _i32),
+        ("weight_decay", C.c_float),
+    ]
+
+
+class AdamWConfig(C.Structure):
+    """Mirror of struct fwd_eb_adamw_config."""
+    _fields_ = [
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+        ("grad_scale", C.c_double), ("step", _i64), ("d_lr", _p), ("d_grad_scale", _p), ("d_step", _p),
+        ("d_skip", _p),
+    ]
+
+
+SIGNATURES = {
+    "fwd_eb_backward_params_size": (C.c_size_t, []),
+    "fwd_eb_backward_workspace_size": (C.c_size_t, [C.POINTER(BackwardParams)]),
+    "fwd_eb_backward": (C.c_int, [C.POINTER(BackwardParams), _p]),
+    "fwd_eb_layer_norm_params_size": (C.c_size_t, []),
+    "fwd_eb_layer_norm_workspace_size": (C.c_size_t, [C.POINTER(LayerNormParams)]),
+    "fwd_eb_layer_norm_forward": (C.c_int, [C.POINTER(LayerNormParams), _p]),
+    "fwd_eb_layer_norm_backward": (C.c_int, [C.POINTER(LayerNormParams), _p]),
+    "fwd_eb_adamw_tensor_size": (C.c_size_t, []),
+    "fwd_eb_adamw_config_size": (C.c_size_t, []),
+    "fwd_eb_adamw_step": (C.c_int, [C.POINTER(AdamWTensor), _i32, C.POINTER(AdamWConfig), _p]),
+}
+
+_bound = None
+
+
+def _lib() -> C.CDLL:
+    global _bound
+    if _bound is None:
+        lib = capi.lib()
+        for name, (res, args) in SIGNATURES.items():
+            fn = getattr(lib, name)
+            fn.restype = res
+            fn.argtypes = args
+        for size, mirror in ((lib.fwd_eb_backward_params_size, BackwardParams),
+                             (lib.fwd_eb_layer_norm_params_size, LayerNormParams),
+                             (lib.fwd_eb_adamw_tensor_size, AdamWTensor),
+                             (lib.fwd_eb_adamw_config_size, AdamWConfig)):
+            if size() != C.sizeof(mirror):
+                raise RuntimeError(f"ctypes mirror {mirror.__name__} is out of step with the library")
+        _bound = lib
+    return _bound
+
+
+_DTYPES = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: BF16}
+
+
+def _dtype(t, what: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: unsupported dtype {t.dtype}")
+    return code
+
+
+def _device_of(tensors) -> torch.device:
+    """The one CUDA device of the (name, tensor) pairs; None tensors are skipped."""
+    device = None
+    for name, t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor; there is no CPU path")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    return device
+
+
+class _On:
+    """Makes a device current for the launch, when it is not already."""
+
+    def __init__(self, device):
+        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+        return _p(torch.cuda.current_stream().cuda_stream)
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _scratch(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _rows(t, name: str, cols: int, rows: int | None = None) -> int:
+    """Row stride of a 2-D tensor with unit column stride (0, that is `cols`, when it has at most
+    one row); raises unless it is [rows, cols]."""
+    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {cols}], got {list(t.shape)}")
+    if cols > 1 and t.shape[0] > 0 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have unit column stride")
+    if t.shape[0] <= 1:
+        return 0
+    if t.stride(0) < cols:
+        raise ValueError(f"{name}: rows overlap (row stride {t.stride(0)}, {cols} columns)")
+    return t.stride(0)
+
+
+# ---- gradient of the pooled lookup ----------------------------------------------------
+
+
+def embedding_bag_winners(table, indices, offsets=None, *, fixed_len=0, include_last_offset=False, padding_idx=-1,
+                          row_lo=0):
+    """A max-pooled call that keeps what its gradient needs: fp32 pairs [num_bags, dim, 2] of the value and, as
+    int32 bits, the position in the bag of the index that supplied it (FWD_EB_F32_POS).  The pooled
+    rows are pairs[..., 0]; the whole tensor is embedding_bag_backward's `winners`."""
+    device = _device_of([("table", table), ("indices", indices), ("offsets", offsets)])
+    if fixed_len == 0 and offsets is None:
+        raise ValueError("offsets is None and fixed_len is 0")
+    bags = indices.numel() // fixed_len if fixed_len else offsets.numel() - int(include_last_offset)
+    with _On(device) as stream:
+        pairs = torch.empty((max(bags, 0), table.shape[1], 2), dtype=torch.float32, device=device)
+        p = capi.make_params(table, indices, offsets, out=pairs, mode=capi.MODE_MAX, fixed_len=fixed_len,
+                             include_last_offset=include_last_offset, padding_idx=padding_idx, row_lo=row_lo)
+        p.out_dtype, p.out_stride = capi.F32_POS, 0
+        capi.check(_lib().fwd_eb_forward(C.byref(p), stream))
+    return pairs
+
+
+def embedding_bag_backward(grad_out, table, indices, offsets=None, *, mode=capi.MODE_SUM, fixed_len=0,
+                           per_sample_weights=None, include_last_offset=False, padding_idx=-1, row_lo=0, flags=0,
+                           winners=None, grad_table=None, grad_dtype=None, accumulate=False, need_table=True,
+                           need_weights=False):
+    """Gradients of capi.embedding_bag(table, indices, offsets, ...) for grad_out = d loss / d out.
+
+    Returns (grad_table, grad_weights).  grad_table is dense, [num_rows, dim] over the table's rows, in
+    `grad_dtype` (default: the table's) or the tensor given as `grad_table`; with accumulate=True
+    the gradient is added to what that tensor holds, at a cost that goes by the lookups and not by the
+    table.  grad_weights is fp32, [num_indices].  What is not asked for is None.  MODE_MAX takes
+    `winners` from embedding_bag_winners.
+    """
+    device = _device_of([("grad_out", grad_out), ("table", table), ("indices", indices), ("offsets", offsets),
+                         ("per_sample_weights", per_sample_weights), ("winners", winners),
+                         ("grad_table", grad_table)])
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table must be 2-D with unit column stride")
+    rows, dim = table.shape
+    if not indices.is_contiguous():
+        raise ValueError("indices must be contiguous")
+    n = indices.numel()
+    gather = mode == capi.MODE_GATHER
+    if gather:
+        bags, offsets = n, None
+    elif fixed_len > 0:
+        bags, offsets = n // fixed_len, None
+    else:
+        if offsets is None:
+            raise ValueError("offsets is None and fixed_len is 0")
+        if offsets.dtype != indices.dtype or not offsets.is_contiguous():
+            raise ValueError("offsets must be a contiguous tensor of the indices' dtype")
+        bags = offsets.numel() - int(include_last_offset)
+    if bags < 0:
+        raise ValueError("offsets is empty, include_last_offset wants an entry")
+    if accumulate and grad_table is None:
+        raise ValueError("accumulate=True adds to a grad_table that the caller gives")
+    if not need_table and not need_weights:
+        raise ValueError("neither gradient is asked for")
+    if grad_table is not None and not need_table:
+        raise ValueError("grad_table is given but need_table is False")
+    if grad_out.dtype not in (torch.float32, torch.float16):
+        raise TypeError(f"grad_out: unsupported dtype {grad_out.dtype}")
+    if per_sample_weights is not None and (per_sample_weights.dtype != torch.float32
+                                           or not per_sample_weights.is_contiguous()
+                                           or per_sample_weights.numel() != n):
+        raise ValueError("per_sample_weights must be contiguous fp32, one per index")
+    win_stride = 0
+    if winners is not None:
+        if winners.dtype != torch.float32 or tuple(winners.shape) != (bags, dim, 2):
+            raise ValueError(f"winners must be fp32 [{bags}, {dim}, 2]")
+        if bags > 0 and (winners.stride(2) != 1 or (dim > 1 and winners.stride(1) != 2)
+                         or (bags > 1 and (winners.stride(0) % 2 or winners.stride(0) < 2 * dim))):
+            raise ValueError("winners must be rows of adjacent pairs")
+        win_stride = winners.stride(0) // 2 if bags > 1 else 0
+    go_stride = _rows(grad_out, "grad_out", dim, bags)
+    lib = _lib()
+    with _On(device) as stream:
+        if need_table:
+            if grad_table is None:
+                grad_table = torch.empty((rows, dim), dtype=grad_dtype or table.dtype, device=device)
+            if grad_table.dtype not in (torch.float32, torch.float16):
+                raise TypeError(f"grad_table: unsupported dtype {grad_table.dtype}")
+            gt_stride = _rows(grad_table, "grad_table", dim, rows)
+        grad_weights = torch.empty(n, dtype=torch.float32, device=device) if need_weights else None
+        if (rows == 0 or not need_table) and (n == 0 or not need_weights):
+            return grad_table, grad_weights   # nothing to compute; torch gives empty tensors no address
+        psw = per_sample_weights
+        p = BackwardParams(
+            capi.Params(
+                table.data_ptr(), capi._torch_dtype_code(table), dim, rows, row_lo,
+                table.stride(0) if rows > 1 else 0, indices.data_ptr(),
+                None if offsets is None else offsets.data_ptr(), capi._index_code(indices),
+                0 if gather else fixed_len, n, 0 if gather else bags, None if psw is None else psw.data_ptr(), mode,
+                int(include_last_offset), padding_idx, None, 0, 0, 0, None, 0, flags, 0),
+            grad_out.data_ptr(), _DTYPES[grad_out.dtype], _DTYPES[grad_table.dtype] if need_table else 0, go_stride,
+            grad_table.data_ptr() if need_table else None, gt_stride if need_table else 0,
+            grad_weights.data_ptr() if need_weights else None, None if winners is None else winners.data_ptr(),
+            win_stride, None, 0, BACKWARD_ACCUMULATE if accumulate else 0, 0)
+        need = lib.fwd_eb_backward_workspace_size(C.byref(p))
+        if need:
+            ws = _scratch(need, device)
+            p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        capi.check(lib.fwd_eb_backward(C.byref(p), stream))
+    return grad_table, grad_weights
+
+
+# ---- layer norm -------------------------------------------------------------------------
+
+
+def _vector(t, name: str, cols: int, like=None):
+    if t.dim() != 1 or t.shape[0] != cols or (cols > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be contiguous [{cols}]")
+    if like is not None and t.dtype != like.dtype:
+        raise TypeError(f"{name} must have the weight's dtype")
+
+
+def _stats(t, name: str, rows: int):
+    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous fp32 [{rows}]")
+
+
+def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=False):
+    """Layer norm of the rows of x [rows, cols] (fp32, fp16 or bf16; any row stride).
+
+    Returns y of x's dtype (`out`, which may be x, or a new tensor), or (y, mean, rstd) with
+    return_stats=True: the fp32 statistics that layer_norm_backward takes."""
+    device = _device_of([("x", x), ("weight", weight), ("bias", bias), ("out", out)])
+    if x.dim() != 2:
+        raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
+    rows, cols = x.shape
+    code = _dtype(x, "x")
+    x_stride = _rows(x, "x", cols)
+    wtype = 0
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _vector(t, name, cols, weight)
+            wtype = _dtype(t, name)
+    if out is not None and out.dtype != x.dtype:
+        raise TypeError("out must have x's dtype")
+    with _On(device) as stream:
+        y = torch.empty((rows, cols), dtype=x.dtype, device=device) if out is None else out
+        y_stride = _rows(y, "out", cols, rows)
+        mean = rstd = None
+        if return_stats:
+            mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=device)
+        p = LayerNormParams(
+            x.data_ptr(), code, wtype, rows, cols, x_stride, None if weight is None else weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), eps, mean.data_ptr() if return_stats else None,
+            rstd.data_ptr() if return_stats else None, y.data_ptr(), y_stride)
+        capi.check(_lib().fwd_eb_layer_norm_forward(C.byref(p), stream))
+    return (y, mean, rstd) if return_stats else y
+
+
+def layer_norm_backward(grad_y, x, mean, rstd, weight=None, *, grad_x=None, need_x=True, need_params=True,
+                        param_dtype=None):
+    """Gradients of layer_norm: (grad_x, grad_weight, grad_bias).
+
+    mean and rstd are the forward call's.  grad_x (x's dtype) may be given, and may be grad_y or x
+    itself.  grad_weight and grad_bias have the weight's dtype, or `param_dtype` (default fp32)
+    where there is no weight.  What is not asked for is None."""
+    device = _device_of([("x", x), ("grad_y", grad_y), ("mean", mean), ("rstd", rstd), ("weight", weight),
+                         ("grad_x", grad_x)])
+    if x.dim() != 2:
+        raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
+    rows, cols = x.shape
+    code = _dtype(x, "x")
+    if grad_y.dtype != x.dtype or (grad_x is not None and grad_x.dtype != x.dtype):
+        raise TypeError("grad_y and grad_x must have x's dtype")
+    if grad_x is not None and not need_x:
+        raise ValueError("grad_x is given but need_x is False")
+    x_stride, gy_stride = _rows(x, "x", cols), _rows(grad_y, "grad_y", cols, rows)
+    _stats(mean, "mean", rows)
+    _stats(rstd, "rstd", rows)
+    if weight is not None:
+        _vector(weight, "weight", cols)
+        param_dtype = weight.dtype
+    param_dtype = param_dtype or torch.float32
+    if param_dtype not in _DTYPES:
+        raise TypeError(f"param_dtype: unsupported dtype {param_dtype}")
+    lib = _lib()
+    with _On(device) as stream:
+        gx_stride = 0
+        if need_x:
+            if grad_x is None:
+                grad_x = torch.empty((rows, cols), dtype=x.dtype, device=device)
+            gx_stride = _rows(grad_x, "grad_x", cols, rows)
+        gw = gb = None
+        if need_params:
+            gw = torch.empty(cols, dtype=param_dtype, device=device)
+            gb = torch.empty(cols, dtype=param_dtype, device=device)
+        p = LayerNormParams(
+            x.data_ptr(), code, _DTYPES[param_dtype], rows, cols, x_stride,
+            None if weight is None else weight.data_ptr(), None, 0.0, mean.data_ptr(), rstd.data_ptr(), None, 0,
+            grad_y.data_ptr(), gy_stride, grad_x.data_ptr() if need_x else None, gx_stride,
+            gw.data_ptr() if need_params else None, gb.data_ptr() if need_params else None, None, 0)
+        if need_params:
+            need = lib.fwd_eb_layer_norm_workspace_size(C.byref(p))
+            if need:
+                ws = _scratch(need, device)
+                p.workspace, p.workspace_bytes = ws.data_ptr(), need
+        capi.check(lib.fwd_eb_layer_norm_backward(C.byref(p), stream))
+    return grad_x, gw, gb
+
+
+# ---- AdamW ------------------------------------------------------------------------------
+
+
+class AdamW:
+    """AdamW over a list of contiguous CUDA tensors of one device, one launch a step (per 256 tensors).
+
+    state_bits=32 keeps exp_avg and exp_avg_sq in fp32; 8 keeps exp_avg and the square root of
+    exp_avg_sq as float8_e4m3fn with one fp32 scale per 256 elements (exp_avg_scale,
+    exp_avg_sq_scale): the value of element i is float(code[i]) * scale[i // 256].  masters[i], fp32, is
+    the copy that the step works on where parameter i is fp16 or bf16; the parameter is then
+    its rounded image.  The state tensors may be given (to resume); otherwise they start at zero.
+    weight_decay is a number, or one per tensor.
+
+    capturable=True keeps the step count and lr on the device (step_tensor, lr_tensor): a step
+    captured into a graph then counts on with every replay, and lr may be changed in between.
+    """
+
+    def __init__(self, params, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32,
+                 masters=None, exp_avg=None, exp_avg_sq=None, exp_avg_scale=None, exp_avg_sq_scale=None, step=0,
+                 capturable=False):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("AdamW needs at least one parameter")
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits is 32 or 8 (got {state_bits})")
+        self.device = _device_of([(f"params[{i}]", p) for i, p in enumerate(self.params)])
+        self.state_bits = state_bits
+        self.step_count = int(step)
+        n = len(self.params)
+        decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(d) for d in weight_decay]
+        if len(decay) != n:
+            raise ValueError("weight_decay: one number, or one per parameter")
+        state = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        blocks = [-(-p.numel() // ADAMW_BLOCK) for p in self.params]
+        if state_bits == 32 and (exp_avg_scale is not None or exp_avg_sq_scale is not None):
+            raise ValueError("states of 32 bits have no scales")
+
+        def states(given, name, dtype, sizes):
+            if given is None:
+                return [torch.zeros(k, dtype=dtype, device=self.device) for k in sizes]
+            given = list(given)
+            if len(given) != n:
+                raise ValueError(f"{name}: one tensor per parameter")
+            for i, t in enumerate(given):
+                self._check(t, f"{name}[{i}]", sizes[i])
+                if t.dtype != dtype:
+                    raise TypeError(f"{name}[{i}] must be {dtype}")
+            return given
+
+        for i, p in enumerate(self.params):
+            self._check(p, f"params[{i}]", p.numel())
+            _dtype(p, f"params[{i}]")
+        sizes = [p.numel() for p in self.params]
+        self.masters = [None] * n if masters is None else list(masters)
+        if len(self.masters) != n:
+            raise ValueError("masters: one tensor (or None) per parameter")
+        for i, t in enumerate(self.masters):
+            if t is not None:
+                self._check(t, f"masters[{i}]", sizes[i])
+                if t.dtype != torch.float32:
+                    raise TypeError(f"masters[{i}] must be fp32")
+        self.exp_avg = states(exp_avg, "exp_avg", state, sizes)
+        self.exp_avg_sq = states(exp_avg_sq, "exp_avg_sq", state, sizes)
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        if state_bits == 8:
+            self.exp_avg_scale = states(exp_avg_scale, "exp_avg_scale", torch.float32, blocks)
+            self.exp_avg_sq_scale = states(exp_avg_sq_scale, "exp_avg_sq_scale", torch.float32, blocks)
+        self._table = (AdamWTensor * n)()
+        for i, p in enumerate(self.params):
+            t = self._table[i]
+            t.param, t.n, t.param_dtype = p.data_ptr(), p.numel(), _DTYPES[p.dtype]
+            t.master = None if self.masters[i] is None else self.masters[i].data_ptr()
+            t.exp_avg, t.exp_avg_sq = self.exp_avg[i].data_ptr(), self.exp_avg_sq[i].data_ptr()
+            if state_bits == 8:
+                t.exp_avg_scale = self.exp_avg_scale[i].data_ptr()
+                t.exp_avg_sq_scale = self.exp_avg_sq_scale[i].data_ptr()
+            t.state_bits, t.weight_decay = state_bits, decay[i]
+        self._config = AdamWConfig(lr, betas[0], betas[1], eps, 1.0, 0, None, None, None, None)
+        self.step_tensor = self.lr_tensor = None
+        if capturable:
+            self.step_tensor = torch.full((1,), self.step_count, dtype=torch.int64, device=self.device)
+            self.lr_tensor = torch.full((1,), lr, dtype=torch.float32, device=self.device)
+            self._config.d_step, self._config.d_lr = self.step_tensor.data_ptr(), self.lr_tensor.data_ptr()
+            self._config.step = 1
+        self._grads = None
+        self._lib = _lib()
+
+    def _check(self, t, name, numel):
+        if not t.is_cuda or t.device != self.device:
+            raise ValueError(f"{name} must be on {self.device}")
+        if t.numel() != numel or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous, {numel} elements")
+
+    def bind(self, grads) -> None:
+        """Gradients of the steps to come, one per parameter: buffers that the caller refills between steps.
+        They are kept alive until the next bind."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError("one gradient per parameter")
+        for i, g in enumerate(grads):
+            self._check(g, f"grads[{i}]", self._table[i].n)
+            _dtype(g, f"grads[{i}]")
+        for t, g in zip(self._table, grads):
+            t.grad, t.grad_dtype = g.data_ptr(), _DTYPES[g.dtype]
+        self._grads = grads
+
+    def step(self, grads=None, *, lr=None, grad_scale=1.0, skip=None) -> None:
+        """One step with `grads` (bound first) or the bound gradients.  lr, where given, holds from this step
+        on.  grad_scale: a number, or an fp32 device tensor of one element.  skip: an int32
+        device tensor of one element; where it is not 0 the step changes nothing (it still counts)."""
+        if grads is not None:
+            self.bind(grads)
+        if self._grads is None:
+            raise ValueError("no gradients: give them here or call bind()")
+        cfg = self._config
+        for name, t, dtype in (("grad_scale", grad_scale, torch.float32), ("skip", skip, torch.int32)):
+            if isinstance(t, torch.Tensor):
+                self._check(t, name, 1)
+                if t.dtype != dtype:
+                    raise TypeError(f"{name} must be {dtype}")
+        if isinstance(grad_scale, torch.Tensor):
+            cfg.d_grad_scale = grad_scale.data_ptr()
+        else:
+            cfg.d_grad_scale, cfg.grad_scale = None, grad_scale
+        cfg.d_skip = None if skip is None else skip.data_ptr()
+        with _On(self.device) as stream:
+            if self.step_tensor is not None:
+                if lr is not None:
+                    self.lr_tensor.fill_(lr)
+                self.step_tensor.add_(1)
+            else:
+                if lr is not None:
+                    cfg.lr = lr
+                cfg.step = self.step_count + 1
+            capi.check(self._lib.fwd_eb_adamw_step(self._table, len(self._table), C.byref(cfg), stream))
+        self.step_count += 1
