@@ -6,6 +6,10 @@
 // lane handles 8 consecutive elements, so a warp's 256 are exactly one block of an 8-bit
 // state: the block's largest value is one integer reduction over the warp (positive floats order
 // as integers), and no value is read or written twice.
+//
+// States of 32 bits are bound by memory whatever the code does.  With states of 8 bits the bytes
+// shrink to a third and the instructions grow, so both count there: whole chunks run
+// a loop without bounds checks in which the next turn's loads are under way.
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -18,11 +22,10 @@ namespace {
 
 constexpr int kAdamThreads = 256;
 constexpr int kLane = 8;                                // elements a lane handles at a time
-constexpr int kTurns = 2;                               // times a CTA goes over its chunk
-constexpr int kChunk = kAdamThreads * kLane * kTurns;   // elements of a chunk
+constexpr int kTurn = kAdamThreads * kLane;              // elements a CTA handles at a time
+constexpr int kMostTurns = 8;                           // turns of a chunk, at most
 constexpr int kMost = 256;                              // tensors of a launch
 static_assert(32 * kLane == FWD_EB_ADAMW_BLOCK, "a warp's elements are one block of an 8-bit state");
-static_assert(kChunk % FWD_EB_ADAMW_BLOCK == 0, "blocks do not cross chunks");
 
 struct AdamTensor {
   void* param;
@@ -46,6 +49,7 @@ struct AdamScalars {
   float step_size;     // lr / (1 - beta1^t)
   float root_scale;    // 1 / sqrt(1 - beta2^t)
   float log1, log2;    // log(beta), for a step that lies on the device
+  int eps_normal;      // eps is far enough from zero that a subnormal v may count as zero
   long long step;
   const float* d_lr;
   const float* d_grad_scale;
@@ -57,6 +61,7 @@ template <int CAP>
 struct AdamArgs {
   AdamScalars s;
   int count;
+  int turns;           // of a chunk
   AdamTensor t[CAP];
 };
 
@@ -119,47 +124,129 @@ __device__ __forceinline__ void store_codes(void* p, long long at, int n, bool w
     if (i < n) q[i] = c[i];
   }
 }
-__device__ __forceinline__ void decode(uint2 r, float scale, float (&f)[kLane]) {
+__device__ __forceinline__ void decode(uint2 r, float (&f)[kLane]) {
   const unsigned w[2] = {r.x, r.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i / 2] >> (16 * (i & 1))), __NV_E4M3);
     const float2 t = __half22float2(__half2(h));
-    f[2 * i] = t.x * scale;
-    f[2 * i + 1] = t.y * scale;
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
   }
 }
 
+// Root and reciprocal within an ulp or two, in one or a few instructions where the correctly rounded ones
+// take ten: the update is lr times smaller than the parameter it is added to, and a code or
+// scale of an 8-bit state is far coarser.  FTZ: a subnormal v counts as zero.  Without it the
+// reciprocal's argument is zero only where sqrt(v) + eps is.
+template <bool FTZ>
+__device__ __forceinline__ float quick_root(float x) {
+  float y;
+  if (FTZ) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  else asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float quick_reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Codes of a block's values and its scale, the same in every lane: x ~ scale * e4m3(x / scale) with
-// scale = max|x| / 448.  Every lane of the warp calls it; `least` is the smallest code that a
-// value above zero may get.  A scale below the normal range counts as zero: its reciprocal
-// would not be finite.  A block that holds a NaN or an infinity gets a scale that is neither
-// finite nor zero, so the whole block reads back as NaN.
-__device__ __forceinline__ uint2 encode(const float (&x)[kLane], float least, float& scale) {
-  unsigned top = 0;
+// scale = max|x| / 448.  Every lane of the warp calls it.  UP: x >= 0, and a value above zero
+// gets the smallest code at least.  A scale below the normal range counts as zero: its reciprocal
+// would not be finite.  A NaN gets the code of a NaN and does not touch the scale; an infinity makes
+// the scale infinite, and the whole block reads back as NaN.
+template <bool UP>
+__device__ __forceinline__ uint2 encode(const float (&x)[kLane], float& scale) {
+  float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kLane; ++i) {
-    const unsigned b = __float_as_uint(x[i]) & 0x7fffffffu;
-    top = b > top ? b : top;
-  }
-  scale = __uint_as_float(__reduce_max_sync(0xffffffffu, top)) * (float)(1.0 / 448.0);
+  for (int i = 0; i < kLane; ++i) top = fmaxf(top, UP ? x[i] : fabsf(x[i]));
+  // floats that are not negative order as integers
+  scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))) * (float)(1.0 / 448.0);
   if (scale < FLT_MIN) scale = 0.0f;
-  const float inverse = scale > 0.0f ? __frcp_rn(scale) : 0.0f;
+  const float inverse = scale > 0.0f ? quick_reciprocal(scale) : 0.0f;
   unsigned w[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 t = make_float2(x[2 * i] * inverse, x[2 * i + 1] * inverse);
-    if (least > 0.0f) {
-      if (x[2 * i] > 0.0f && t.x < least) t.x = least;
-      if (x[2 * i + 1] > 0.0f && t.y < least) t.y = least;
-    }
+    const float2 t = mul2(make_float2(x[2 * i], x[2 * i + 1]), both(inverse));
     w[i / 2] |= (unsigned)__nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
+  }
+  if (UP) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (((w[k] - 0x01010101u) & ~w[k] & 0x80808080u) == 0) continue;   // no byte of it is zero
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (x[4 * k + i] > 0.0f && (w[k] & (0xffu << (8 * i))) == 0) w[k] |= 1u << (8 * i);
+      }
+    }
   }
   return make_uint2(w[0], w[1]);
 }
 
-template <int CAP>
-__global__ void __launch_bounds__(kAdamThreads)
+// What a step multiplies by, once device scalars are read.
+struct Rates {
+  float beta1, rest1, beta2, rest2, eps, grad_scale, step_size, root_scale, keep;
+};
+
+// One lane's 8 elements: m and v come as loaded, to be multiplied by keep1 and keep2.
+template <bool FTZ>
+__device__ __forceinline__ void update(const Rates& r, float keep1, float keep2, float (&p)[kLane], const float (&g)[kLane],
+                                       float (&m)[kLane], float (&v)[kLane], float (&root)[kLane]) {
+#pragma unroll
+  for (int i = 0; i < kLane; i += 2) {
+    const float2 gi = mul2(make_float2(g[i], g[i + 1]), both(r.grad_scale));
+    const float2 mi = fma2(make_float2(m[i], m[i + 1]), both(keep1), mul2(gi, both(r.rest1)));
+    const float2 vi = fma2(make_float2(v[i], v[i + 1]), both(keep2), mul2(mul2(gi, gi), both(r.rest2)));
+    const float2 ri = make_float2(quick_root<FTZ>(vi.x), quick_root<FTZ>(vi.y));
+    const float2 den = fma2(ri, both(r.root_scale), both(r.eps));
+    const float2 upd = mul2(mi, make_float2(quick_reciprocal(den.x), quick_reciprocal(den.y)));
+    const float2 pi = fma2(make_float2(p[i], p[i + 1]), both(r.keep), mul2(upd, both(-r.step_size)));
+    m[i] = mi.x, m[i + 1] = mi.y;
+    v[i] = vi.x, v[i + 1] = vi.y;
+    root[i] = ri.x, root[i + 1] = ri.y;
+    p[i] = pi.x, p[i + 1] = pi.y;
+  }
+}
+__device__ __forceinline__ void square(float (&v)[kLane]) {   // of codes: exact
+#pragma unroll
+  for (int i = 0; i < kLane; i += 2) {
+    const float2 c = make_float2(v[i], v[i + 1]), c2 = mul2(c, c);
+    v[i] = c2.x, v[i + 1] = c2.y;
+  }
+}
+
+// 8 elements of any type as they lie in memory: 16-bit types fill half of it.
+struct Raw {
+  uint4 lo, hi;
+  __device__ __forceinline__ void load(const void* p, bool wide, int at) {
+    if (wide) {
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at);
+      lo = q[0];
+      hi = q[1];
+    } else {
+      lo = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + at);
+    }
+  }
+  __device__ __forceinline__ void get(int dtype, float (&f)[kLane]) const {
+    if (dtype == FWD_EB_F32) {
+      memcpy(f, &lo, 16);
+      memcpy(f + 4, &hi, 16);
+    } else if (dtype == FWD_EB_F16) {
+      Pack<__half, kLane> r;
+      r.w[0] = lo;
+      r.get(f);
+    } else {
+      Pack<__nv_bfloat16, kLane> r;
+      r.w[0] = lo;
+      r.get(f);
+    }
+  }
+};
+
+template <int CAP, bool BITS8>
+__global__ void __launch_bounds__(kAdamThreads, BITS8 ? 3 : 4)
 adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   pdl_enter();
   if (a.s.d_skip && *a.s.d_skip != 0) return;
@@ -168,69 +255,107 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
     const int mid = (lo + hi) / 2;
     if (a.t[mid].first <= blockIdx.x) lo = mid; else hi = mid;
   }
-  const AdamTensor& t = a.t[lo];
-  const long long chunk = (long long)(blockIdx.x - t.first) * kChunk;
-
-  float lr = a.s.lr, step_size = a.s.step_size, root_scale = a.s.root_scale, grad_scale = a.s.grad_scale;
-  if (a.s.d_lr) lr = *a.s.d_lr;
-  if (a.s.d_grad_scale) grad_scale = *a.s.d_grad_scale;
+  AdamTensor t = a.t[lo];
+  Rates r = {a.s.beta1, a.s.rest1, a.s.beta2, a.s.rest2, a.s.eps, a.s.grad_scale, a.s.step_size, a.s.root_scale, t.keep};
+  if (a.s.d_grad_scale) r.grad_scale = *a.s.d_grad_scale;
   if (a.s.d_lr || a.s.d_step) {
     // 1 - beta^t = -expm1(t log beta): no cancellation, in fp32
+    const float lr = a.s.d_lr ? *a.s.d_lr : a.s.lr;
     const float at = (float)(a.s.d_step ? *a.s.d_step : a.s.step);
-    step_size = lr / -expm1f(at * a.s.log1);
-    root_scale = 1.0f / sqrtf(-expm1f(at * a.s.log2));
+    r.step_size = lr / -expm1f(at * a.s.log1);
+    r.root_scale = 1.0f / sqrtf(-expm1f(at * a.s.log2));
+    if (a.s.d_lr) r.keep = 1.0f - lr * t.weight_decay;
   }
-  const float keep = a.s.d_lr ? 1.0f - lr * t.weight_decay : t.keep;
-  const bool bits8 = t.m_scale != nullptr;
+  // this chunk's part of the tensor
+  const int chunk = a.turns * kTurn;
+  const long long begin = (long long)(blockIdx.x - t.first) * chunk;
+  const int left = t.n - begin < chunk ? (int)(t.n - begin) : chunk;
+  const int psize = t.ptype == FWD_EB_F32 ? 4 : 2, gsize = t.gtype == FWD_EB_F32 ? 4 : 2;
+  t.param = static_cast<char*>(t.param) + begin * psize;
+  t.grad = static_cast<const char*>(t.grad) + begin * gsize;
+  if (t.master) t.master += begin;
+  t.m = static_cast<char*>(t.m) + begin * (BITS8 ? 1 : 4);
+  t.v = static_cast<char*>(t.v) + begin * (BITS8 ? 1 : 4);
+  if (BITS8) {
+    t.m_scale += begin / FWD_EB_ADAMW_BLOCK;
+    t.v_scale += begin / FWD_EB_ADAMW_BLOCK;
+  }
+  const void* from = t.master ? t.master : t.param;      // what the step works on, and its type
+  const int ftype = t.master ? FWD_EB_F32 : t.ptype;
 
-#pragma unroll
-  for (int turn = 0; turn < kTurns; ++turn) {
-    const long long at = chunk + (turn * kAdamThreads + (int)threadIdx.x) * kLane;
-    if (t.n <= at - (int)(threadIdx.x & 31) * kLane) continue;   // the warp's first element: all its lanes go on together
-    const long long left = t.n - at;
-    const int n = left < 0 ? 0 : (left < kLane ? (int)left : kLane);
-    const bool whole = n == kLane && t.aligned;
-    float p[kLane], g[kLane], m[kLane], v[kLane];
-    load_lane(t.grad, t.gtype, at, n, whole, g);
-    if (t.master) {
-      load_lane(t.master, FWD_EB_F32, at, n, whole, p);
-    } else {
-      load_lane(t.param, t.ptype, at, n, whole, p);
+  if (BITS8 && left == chunk && t.aligned && a.s.eps_normal) {
+    Raw p0, g0;
+    uint2 m0, v0;
+    float ms0, vs0;
+    auto fetch = [&](int at) {
+      p0.load(from, ftype == FWD_EB_F32, at);
+      g0.load(t.grad, gsize == 4, at);
+      m0 = *reinterpret_cast<const uint2*>(static_cast<const char*>(t.m) + at);
+      v0 = *reinterpret_cast<const uint2*>(static_cast<const char*>(t.v) + at);
+      ms0 = t.m_scale[at / FWD_EB_ADAMW_BLOCK];
+      vs0 = t.v_scale[at / FWD_EB_ADAMW_BLOCK];
+    };
+    int at = threadIdx.x * kLane;
+    fetch(at);
+    for (int turn = 0; turn < a.turns; ++turn, at += kTurn) {
+      float p[kLane], g[kLane], m[kLane], v[kLane], root[kLane];
+      p0.get(ftype, p);
+      g0.get(t.gtype, g);
+      decode(m0, m);
+      decode(v0, v);
+      const float keep1 = ms0 * r.beta1, keep2 = vs0 * vs0 * r.beta2;
+      if (turn + 1 < a.turns) fetch(at + kTurn);
+      square(v);
+      update<true>(r, keep1, keep2, p, g, m, v, root);
+      float ms, vs;
+      const uint2 cm = encode<false>(m, ms), cv = encode<true>(root, vs);
+      if (t.master) store_any<kLane>(t.master, FWD_EB_F32, at, p);
+      store_any<kLane>(t.param, t.ptype, at, p);
+      *reinterpret_cast<uint2*>(static_cast<char*>(t.m) + at) = cm;
+      *reinterpret_cast<uint2*>(static_cast<char*>(t.v) + at) = cv;
+      if ((threadIdx.x & 31) == 0) {
+        t.m_scale[at / FWD_EB_ADAMW_BLOCK] = ms;
+        t.v_scale[at / FWD_EB_ADAMW_BLOCK] = vs;
+      }
     }
-    const long long block = at / FWD_EB_ADAMW_BLOCK;
-    const bool has_block = block * FWD_EB_ADAMW_BLOCK < t.n;
-    if (bits8) {
+    return;
+  }
+
+  for (int turn = 0; turn < a.turns; ++turn) {
+    const int at = (turn * kAdamThreads + (int)threadIdx.x) * kLane;
+    if (left <= at - (int)(threadIdx.x & 31) * kLane) return;   // the warp's first element: all its lanes go on together
+    const int n = left - at < 0 ? 0 : (left - at < kLane ? left - at : kLane);
+    const bool whole = n == kLane && t.aligned;
+    float p[kLane], g[kLane], m[kLane], v[kLane], root[kLane];
+    load_lane(t.grad, t.gtype, at, n, whole, g);
+    load_lane(from, ftype, at, n, whole, p);
+    const int block = at / FWD_EB_ADAMW_BLOCK;
+    float keep1 = r.beta1, keep2 = r.beta2;
+    if (BITS8) {
       const uint2 cm = load_codes(t.m, at, n, whole), cv = load_codes(t.v, at, n, whole);
-      decode(cm, has_block ? t.m_scale[block] : 0.0f, m);
-      decode(cv, has_block ? t.v_scale[block] : 0.0f, v);
-#pragma unroll
-      for (int i = 0; i < kLane; ++i) v[i] = __fmul_rn(v[i], v[i]);
+      keep1 *= t.m_scale[block];
+      const float vs = t.v_scale[block];
+      keep2 *= vs * vs;
+      decode(cm, m);
+      decode(cv, v);
+      square(v);
     } else {
       load_lane(t.m, FWD_EB_F32, at, n, whole, m);
       load_lane(t.v, FWD_EB_F32, at, n, whole, v);
     }
-    float root[kLane];
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      // each product and sum rounds by itself: an 8-bit code must not depend on how they are fused
-      const float gi = __fmul_rn(g[i], grad_scale);
-      m[i] = __fadd_rn(__fmul_rn(m[i], a.s.beta1), __fmul_rn(gi, a.s.rest1));
-      v[i] = __fadd_rn(__fmul_rn(v[i], a.s.beta2), __fmul_rn(__fmul_rn(gi, gi), a.s.rest2));
-      root[i] = __fsqrt_rn(v[i]);
-      p[i] = p[i] * keep - step_size * (m[i] / fmaf(root[i], root_scale, a.s.eps));
-    }
+    update<false>(r, keep1, keep2, p, g, m, v, root);
     if (t.master) store_lane(t.master, FWD_EB_F32, at, n, whole, p);
     store_lane(t.param, t.ptype, at, n, whole, p);
-    if (bits8) {
+    if (BITS8) {
 #pragma unroll
       for (int i = 0; i < kLane; ++i) {   // what lies behind the tensor's end takes no part in its last scale
         if (i >= n) m[i] = root[i] = 0.0f;
       }
       float ms, vs;
-      const uint2 cm = encode(m, 0.0f, ms), cv = encode(root, 0.001953125f, vs);   // 2^-9: the smallest code
+      const uint2 cm = encode<false>(m, ms), cv = encode<true>(root, vs);
       store_codes(t.m, at, n, whole, cm);
       store_codes(t.v, at, n, whole, cv);
-      if ((threadIdx.x & 31) == 0 && has_block) {
+      if ((threadIdx.x & 31) == 0) {
         t.m_scale[block] = ms;
         t.v_scale[block] = vs;
       }
@@ -294,6 +419,7 @@ AdamScalars scalars_of(const fwd_eb_adamw_config* c) {
   s.log1 = (float)std::log(c->beta1);
   s.log2 = (float)std::log(c->beta2);
   s.step = c->step;
+  s.eps_normal = c->eps >= 1e-30;
   s.d_lr = c->d_lr;
   s.d_grad_scale = c->d_grad_scale;
   s.d_step = reinterpret_cast<const long long*>(c->d_step);
@@ -322,23 +448,47 @@ AdamTensor tensor_of(const fwd_eb_adamw_tensor& t, unsigned first, double lr) {
   return r;
 }
 
-// Fills one launch from the tensors at *next on, moves *next behind them, launches.
-template <int CAP>
+// Fills one launch with the tensors of one state width from *next on, moves *next behind them, launches.
+template <int CAP, bool BITS8>
 cudaError_t launch_some(const fwd_eb_adamw_tensor* ts, int count, int* next, const AdamScalars& s, double lr,
                         cudaStream_t st) {
   AdamArgs<CAP> a = {};
   a.s = s;
+  int end = *next;
+  long long total = 0;     // turns, at one turn a chunk
+  for (int found = 0; end < count && found < CAP; ++end) {
+    const fwd_eb_adamw_tensor& t = ts[end];
+    if (t.n == 0 || (t.state_bits == 8) != BITS8) continue;
+    total += (t.n + kTurn - 1) / kTurn;
+    ++found;
+  }
+  // 8-bit chunks: longer ones where a few waves of CTAs are left even so (100 M elements: 1 turn 293 us, 4 turns 273)
+  const long long wave = 3LL * sm_count();
+  a.turns = 1;
+  while (BITS8 && a.turns < kMostTurns && total / (2 * a.turns) >= 4 * wave) a.turns *= 2;
   long long chunks = 0;
-  while (*next < count && a.count < CAP) {
+  for (; *next < end; ++*next) {
     const fwd_eb_adamw_tensor& t = ts[*next];
-    const long long c = (t.n + kChunk - 1) / kChunk;
-    if (chunks + c > INT_MAX) break;
-    if (c > 0) a.t[a.count++] = tensor_of(t, (unsigned)chunks, lr);
+    if (t.n == 0 || (t.state_bits == 8) != BITS8) continue;
+    const long long c = (t.n + (long long)a.turns * kTurn - 1) / ((long long)a.turns * kTurn);
+    if (chunks + c > INT_MAX) break;     // the rest in a launch of its own
+    a.t[a.count++] = tensor_of(t, (unsigned)chunks, lr);
     chunks += c;
-    ++*next;
   }
   if (chunks == 0) return cudaSuccess;
-  return launch_pdl(adamw_kernel<CAP>, dim3((unsigned)chunks), kAdamThreads, 0, st, a);
+  return launch_pdl(adamw_kernel<CAP, BITS8>, dim3((unsigned)chunks), kAdamThreads, 0, st, a);
+}
+
+template <bool BITS8>
+cudaError_t launch_all(const fwd_eb_adamw_tensor* ts, int count, const AdamScalars& s, double lr, cudaStream_t st) {
+  for (int next = 0; next < count;) {
+    const int left = count - next;
+    cudaError_t e = left <= 8    ? launch_some<8, BITS8>(ts, count, &next, s, lr, st)
+                    : left <= 64 ? launch_some<64, BITS8>(ts, count, &next, s, lr, st)
+                                 : launch_some<kMost, BITS8>(ts, count, &next, s, lr, st);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace
@@ -356,13 +506,10 @@ extern "C" int fwd_eb_adamw_step(const fwd_eb_adamw_tensor* tensors, int32_t cou
   if (rc) return rc;
   clear_error();
   const AdamScalars s = scalars_of(cfg);
-  for (int next = 0; next < count;) {
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int left = count - next;
-    cudaError_t e = left <= 8    ? launch_some<8>(tensors, count, &next, s, cfg->lr, st)
-                    : left <= 64 ? launch_some<64>(tensors, count, &next, s, cfg->lr, st)
-                                 : launch_some<kMost>(tensors, count, &next, s, cfg->lr, st);
-    if (e != cudaSuccess) return cuda_fail(e, "kernel launch");
-  }
-  return 0;
+  bool any8 = false, any32 = false;
+  for (int i = 0; i < count; ++i) (tensors[i].state_bits == 8 ? any8 : any32) = true;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = any32 ? launch_all<false>(tensors, count, s, cfg->lr, st) : cudaSuccess;
+  if (e == cudaSuccess && any8) e = launch_all<true>(tensors, count, s, cfg->lr, st);
+  return e == cudaSuccess ? 0 : cuda_fail(e, "kernel launch");
 }

@@ -2,12 +2,16 @@
 //
 // grad_table[r] is the sum of the grad_out rows of all lookups of r: a reduction by key whose keys
 // are the indices.  Adding with atomics would take them in any order, so the lookups are
-// sorted by row first: a stable radix sort of (row, lookup) pairs, digits of up to 8 bits, two
-// kernels a digit (histogram of every tile, then scatter).  A warp then takes 32 sorted lookups, keeps
-// its columns' running sum in registers, and stores a row's sum where the row's lookups end.  A row
-// whose lookups cross from one run of 32 into the next leaves partial sums, which a last kernel adds in
-// run order; a popular row's thousands of runs are first added 32 at a time.  Every sum has
-// one order, whatever the schedule.
+// sorted by row first: a stable radix sort of (row, payload) pairs, digits of 8 bits, two kernels
+// a digit (histogram of every tile, then scatter; up to 4096 lookups: one kernel in one CTA).  The
+// sort is bound by latency and leaves the memory idle, so the same launches carry CTAs that fill
+// the dense gradient with zeros.
+//
+// A warp then takes a run of 32 sorted lookups, keeps its columns' running sum in registers,
+// and stores a row's sum where the row's lookups end.  The weights' gradient falls out of the same
+// pass: the table row is read once for all its lookups.  A row whose lookups cross from one run into
+// the next leaves partial sums, which a last kernel adds in run order; a popular row's thousands
+// of runs are first added 32 at a time.  Every sum has one order, whatever the schedule.
 #include <climits>
 
 #include "eb_train.cuh"
@@ -17,11 +21,22 @@ namespace {
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kItems = 4;                          // keys a thread handles at a time
+constexpr int kItems = 5;                          // pairs a thread ranks at a time
 constexpr int kSubTile = kSortThreads * kItems;
+constexpr int kSmallItems = 7;                     // ... in the kernel that sorts all of a small call
+constexpr int kSmall = kSortThreads * kSmallItems;
 constexpr int kDigits = 256;
+constexpr int kStarts = 2048;                      // bag starts a tile keeps in shared memory
 constexpr int kRun = 32;                           // sorted lookups of a run, runs of a block of runs
 constexpr unsigned kNone = 0xffffffffu;
+
+struct ZeroSpan {          // words of grad_table that a launch fills with zeros
+  char* base;
+  long long stride;        // bytes between rows
+  long long per_row;       // words a row
+  long long begin, end;
+  int word;                // bytes: 16, 4 or 2
+};
 
 struct BackArgs {
   // the lookups
@@ -45,13 +60,15 @@ struct BackArgs {
   long long gt_stride;
   const int2* winners;
   long long win_stride;   // pairs
+  unsigned char* won;     // [num_bags][pstride]: the low byte of each winner's position
   float* grad_weights;
   int dim;
   int table_f16, gt_f16, square, accumulate;
   // scratch
   int* bag_of;            // [n]
   int* counted;           // [num_bags]: non-padding lookups (mean with a padding index)
-  uint2* pairs[2];        // [n] {row, lookup}
+  uint2* pairs[2];        // [n] {row, payload}
+  int by_bag;             // the payload is the bag (-1 with a row of num_rows), else the lookup
   unsigned* hist;         // [tiles][kDigits]
   float* partial;         // [runs][2][pstride]: sums of a run's first row, when it began before the run,
                           // and of its last, when it began in the run and goes on
@@ -87,14 +104,45 @@ __device__ __forceinline__ void bag_range(const BackArgs& a, int bag, long long&
   if (end < start) end = start;
 }
 
-// The bag that holds lookup j: the last one that starts at or before it; -1 where there is none.
-__device__ __forceinline__ int find_bag(const BackArgs& a, int j, int lo, int hi) {
-  // the number of starts <= j lies in [lo, hi]
+// The number of starts (ascending) in [lo, hi) that are <= j, plus lo.
+template <typename Start>
+__device__ __forceinline__ int upper_bound(Start start, long long j, int lo, int hi) {
   while (lo < hi) {
     const int mid = lo + (hi - lo) / 2;
-    if (index_at(a.offsets, a.idx64, mid) <= j) lo = mid + 1; else hi = mid;
+    if (start(mid) <= j) lo = mid + 1; else hi = mid;
   }
-  return lo - 1;
+  return lo;
+}
+// The same over all starts by a whole CTA: every thread tests one start a round.
+template <int THREADS>
+__device__ __forceinline__ int upper_bound_cta(const BackArgs& a, long long j, int n) {
+  int lo = 0, len = n;
+  while (len > 0) {
+    const int step = (len + THREADS - 1) / THREADS;
+    const long long at = lo + (long long)(threadIdx.x + 1) * step - 1;
+    const int c = __syncthreads_count(at < lo + len && index_at(a.offsets, a.idx64, at) <= j);
+    const int next = lo + c * step;
+    len = min(step - 1, lo + len - next);
+    lo = next;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void zero_span(const ZeroSpan& z, int part, int parts) {
+  const long long total = z.end - z.begin;
+  const bool dense = z.per_row * z.word == z.stride;
+  for (long long k = (long long)part * blockDim.x + threadIdx.x; k < total; k += (long long)parts * blockDim.x) {
+    const long long i = z.begin + k;
+    char* q = dense ? z.base + i * z.word : z.base + (i / z.per_row) * z.stride + (i % z.per_row) * z.word;
+    if (z.word == 16) *reinterpret_cast<uint4*>(q) = make_uint4(0, 0, 0, 0);
+    else if (z.word == 4) *reinterpret_cast<unsigned*>(q) = 0;
+    else *reinterpret_cast<unsigned short*>(q) = 0;
+  }
+}
+
+__global__ void __launch_bounds__(kSortThreads) zero_kernel(const ZeroSpan z) {
+  pdl_enter();
+  zero_span(z, blockIdx.x, gridDim.x);
 }
 
 // counted[b] = length of bag b; the histogram kernel takes the padding off.
@@ -107,141 +155,288 @@ __global__ void __launch_bounds__(256) bag_length_kernel(const BackArgs a) {
   a.counted[b] = (int)(e - s);
 }
 
-__global__ void __launch_bounds__(256) zero_rows_kernel(char* p, long long row_bytes, long long stride, long long rows,
-                                                        int word) {
-  pdl_enter();
-  const long long per_row = row_bytes / word;
-  const long long total = per_row * rows;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    char* q = per_row * word == stride ? p + i * word : p + (i / per_row) * stride + (i % per_row) * word;
-    if (word == 16) *reinterpret_cast<uint4*>(q) = make_uint4(0, 0, 0, 0);
-    else if (word == 4) *reinterpret_cast<unsigned*>(q) = 0;
-    else *reinterpret_cast<unsigned short*>(q) = 0;
+// The bag starts that the lookups [begin, end) of a tile can lie behind.
+struct TileStarts {
+  int lo, hi;        // the number of starts <= a lookup lies in [lo, hi]
+  bool in_shared;    // starts [lo, hi) are in shared memory
+};
+__device__ __forceinline__ TileStarts find_starts(const BackArgs& a, int begin, int end, long long* shared) {
+  TileStarts t = {0, 0, false};
+  if (a.fixed_len > 0 || begin >= end) return t;
+  const int n = a.num_bags > 0 ? a.num_bags + (a.include_last ? 1 : 0) : 0;
+  t.lo = upper_bound_cta<kSortThreads>(a, begin, n);
+  t.hi = max(t.lo, upper_bound_cta<kSortThreads>(a, end - 1, n));
+  t.in_shared = t.hi - t.lo <= kStarts;
+  if (t.in_shared) {
+    for (int i = t.lo + threadIdx.x; i < t.hi; i += kSortThreads) shared[i - t.lo] = index_at(a.offsets, a.idx64, i);
+    __syncthreads();
   }
+  return t;
+}
+// The bag that holds lookup j: the last one that starts at or before it; -1 where there is none.
+__device__ __forceinline__ int bag_of(const BackArgs& a, int j, const TileStarts& t, const long long* shared) {
+  if (a.fixed_len > 0) {
+    const int bag = j / a.fixed_len;
+    return bag < a.num_bags ? bag : -1;
+  }
+  const int bag = (t.in_shared ? upper_bound([&](int i) { return shared[i - t.lo]; }, j, t.lo, t.hi)
+                               : upper_bound([&](int i) { return index_at(a.offsets, a.idx64, i); }, j, t.lo, t.hi)) - 1;
+  return bag < a.num_bags ? bag : -1;     // behind the last offset of include_last_offset
+}
+// Padding is not counted for a mean: one subtraction a warp and bag.  All lanes of the warp call it.
+__device__ __forceinline__ void uncount_padding(const BackArgs& a, int j, bool in, int bag) {
+  const bool pad = in && bag >= 0 && index_at(a.indices, a.idx64, j) == a.padding_idx;
+  const unsigned same = __match_any_sync(0xffffffffu, pad ? bag : -1);
+  if (pad && (threadIdx.x & 31) == __ffs(same) - 1) atomicSub(a.counted + bag, __popc(same));
 }
 
 // hist[tile][d] = keys of the tile whose digit is d.  FIRST: the keys are made from the indices, and
-// bag_of is written.
+// bag_of is written.  CTAs from `tiles` on fill their span with zeros.
 template <bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const BackArgs a, const uint2* from, int shift) {
+__global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const BackArgs a, const uint2* from, int shift,
+                                                                      const ZeroSpan z) {
   pdl_enter();
+  if ((int)blockIdx.x >= a.tiles) {
+    zero_span(z, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+    return;
+  }
   __shared__ unsigned count[kDigits];
+  __shared__ long long starts[FIRST ? kStarts : 1];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
-  __syncthreads();
   const int begin = blockIdx.x * a.tile;
   const int end = min(a.n, begin + a.tile);
-  const int starts = a.num_bags > 0 ? a.num_bags + (a.include_last ? 1 : 0) : 0;
-  int lo = 0, hi = starts;
-  if (FIRST && a.fixed_len == 0) {   // the starts that this tile's lookups can lie behind
-    lo = find_bag(a, begin, 0, starts) + 1;
-    hi = find_bag(a, end - 1, lo, starts) + 1;
-  }
-  for (int base = begin; base < end; base += kSortThreads) {
-    const int j = base + threadIdx.x;
-    const bool in = j < end;
-    unsigned key = 0;
-    if (FIRST) {
-      int bag = -1;
-      if (in) {
-        bag = a.fixed_len > 0 ? j / a.fixed_len : find_bag(a, j, lo, hi);
-        if (bag >= a.num_bags) bag = -1;      // behind the last offset of include_last_offset
-        a.bag_of[j] = bag;
-        key = row_of(a, j, bag);
+  TileStarts t = {};
+  if (FIRST) t = find_starts(a, begin, end, starts);
+  __syncthreads();
+  for (int base = begin; base < end; base += kSubTile) {
+    unsigned key[kItems];
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int j = base + i * kSortThreads + threadIdx.x;
+      key[i] = 0;
+      if (FIRST) {
+        int bag = -1;
+        if (j < end) {
+          bag = bag_of(a, j, t, starts);
+          a.bag_of[j] = bag;
+          key[i] = row_of(a, j, bag);
+        }
+        if (a.counted) uncount_padding(a, j, j < end, bag);
+      } else if (j < end) {
+        key[i] = from[j].x;
       }
-      if (a.counted) {   // padding is not counted: one subtraction a warp and bag
-        const bool pad = in && bag >= 0 && index_at(a.indices, a.idx64, j) == a.padding_idx;
-        const unsigned same = __match_any_sync(0xffffffffu, pad ? bag : -1);
-        if (pad && (threadIdx.x & 31) == __ffs(same) - 1) atomicSub(a.counted + bag, __popc(same));
-      }
-    } else if (in) {
-      key = from[j].x;
     }
-    if (in) atomicAdd(&count[(key >> shift) & (kDigits - 1)], 1u);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (base + i * kSortThreads + (int)threadIdx.x < end) atomicAdd(&count[(key[i] >> shift) & (kDigits - 1)], 1u);
+    }
   }
   __syncthreads();
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) a.hist[blockIdx.x * kDigits + d] = count[d];
 }
 
+// Ranks of a CTA's items among those of the same digit, in the order of (warp, item, lane): in the warp here, and
+// in_warp[w][d] becomes the number of warp w's items with digit d.  kNone is no digit.
+template <int ITEMS>
+__device__ __forceinline__ void rank_items(const unsigned (&digit)[ITEMS], unsigned (&rank)[ITEMS],
+                                           unsigned (*in_warp)[kDigits]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&in_warp[0][0])[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const unsigned same = __match_any_sync(0xffffffffu, digit[i]);
+    const bool in = digit[i] != kNone;
+    rank[i] = in ? in_warp[warp][digit[i]] + __popc(same & ((1u << lane) - 1u)) : 0;
+    __syncwarp();
+    if (in && lane == __ffs(same) - 1) in_warp[warp][digit[i]] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+}
+// in_warp[w][d] becomes the place of warp w's first item with digit d; place[d] moves behind all of them.
+__device__ __forceinline__ void place_warps(unsigned (*in_warp)[kDigits], unsigned* place) {
+  if (threadIdx.x < kDigits) {
+    unsigned count[kSortWarps];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) count[w] = in_warp[w][threadIdx.x];
+    unsigned at = place[threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      in_warp[w][threadIdx.x] = at;
+      at += count[w];
+    }
+    place[threadIdx.x] = at;
+  }
+  __syncthreads();
+}
+// Exclusive sums over the digits of `mine` (threads below kDigits); `total` is scratch.  All threads call it.
+__device__ __forceinline__ unsigned digits_below(unsigned mine, unsigned* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += x;
+  }
+  if (lane == 31 && warp < kDigits / 32) total[warp] = sum;
+  __syncthreads();
+  for (int w = 0; w < warp && w < kDigits / 32; ++w) sum += total[w];
+  __syncthreads();
+  return sum - mine;
+}
+
 // Moves a tile's pairs to their place in the order of the digit, ties in the order they came.
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const BackArgs a, const uint2* from, uint2* to,
-                                                                    int shift) {
+                                                                    int shift, const ZeroSpan z) {
   pdl_enter();
+  if ((int)blockIdx.x >= a.tiles) {
+    zero_span(z, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+    return;
+  }
   __shared__ unsigned place[kDigits];                    // next free place of a digit
   __shared__ unsigned in_warp[kSortWarps][kDigits];
-  __shared__ unsigned scan[kSortThreads];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // place[d] = keys with a lower digit + keys with digit d in earlier tiles
-  {
-    const int d = threadIdx.x & (kDigits - 1), half = threadIdx.x / kDigits;
-    unsigned before = 0, all = 0;
-    for (int t = half; t < a.tiles; t += kSortThreads / kDigits) {
-      const unsigned c = a.hist[t * kDigits + d];
-      all += c;
-      before += t < (int)blockIdx.x ? c : 0;
-    }
-    in_warp[half][d] = before;
-    scan[threadIdx.x] = all;
-    __syncthreads();
-    unsigned mine = 0;
-    if (threadIdx.x < kDigits) {
-      before = in_warp[0][d] + in_warp[1][d];
-      all = scan[d] + scan[d + kDigits];
-      mine = all;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned x = __shfl_up_sync(0xffffffffu, mine, o);
-        if (lane >= o) mine += x;
-      }
-      if (lane == 31) place[warp] = mine;    // 8 warps' totals, for a moment
-    }
-    __syncthreads();
-    unsigned lower = 0;
-    if (threadIdx.x < kDigits) {
-      for (int w = 0; w < warp; ++w) lower += place[w];
-    }
-    __syncthreads();
-    if (threadIdx.x < kDigits) place[d] = lower + mine - all + before;
-  }
-  static_assert(kSortThreads == 2 * kDigits, "two threads a digit above");
-
   const int begin = blockIdx.x * a.tile;
   const int end = min(a.n, begin + a.tile);
-  for (int base = begin; base < end; base += kSubTile) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&in_warp[0][0])[i] = 0;
-    __syncthreads();
-    uint2 pair[kItems];
-    unsigned rank[kItems];
+  uint2 pair[kItems];
+  auto fetch = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int j = base + (warp * kItems + i) * 32 + lane;
-      const bool in = j < end;
       pair[i] = make_uint2(0, 0);
-      if (in) pair[i] = FIRST ? make_uint2(row_of(a, j, a.bag_of[j]), (unsigned)j) : from[j];
-      const unsigned d = in ? (pair[i].x >> shift) & (kDigits - 1) : kNone;
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      rank[i] = in ? in_warp[warp][d] + __popc(same & ((1u << lane) - 1u)) : 0;
-      __syncwarp();
-      if (in && lane == __ffs(same) - 1) in_warp[warp][d] += __popc(same);
-      __syncwarp();
-    }
-    __syncthreads();
-    if (threadIdx.x < kDigits) {
-      unsigned at = place[threadIdx.x];
-      for (int w = 0; w < kSortWarps; ++w) {
-        const unsigned c = in_warp[w][threadIdx.x];
-        in_warp[w][threadIdx.x] = at;
-        at += c;
+      if (j >= end) continue;
+      if (FIRST) {
+        const int bag = a.bag_of[j];
+        pair[i] = make_uint2(row_of(a, j, bag), a.by_bag ? (unsigned)bag : (unsigned)j);
+      } else {
+        pair[i] = from[j];
       }
-      place[threadIdx.x] = at;
     }
+  };
+  fetch(begin);
+  // place[d] = keys with a lower digit + keys with digit d in earlier tiles: 4 digits a thread, every 8th tile
+  {
+    constexpr int kColumns = kDigits / 4, kGroups = kSortThreads / kColumns;
+    const int column = threadIdx.x % kColumns, group = threadIdx.x / kColumns;
+    uint4 all = make_uint4(0, 0, 0, 0), before = all;
+#pragma unroll 8
+    for (int t = group; t < a.tiles; t += kGroups) {
+      const uint4 c = reinterpret_cast<const uint4*>(a.hist + t * kDigits)[column];
+      const unsigned m = t < (int)blockIdx.x ? 0xffffffffu : 0u;
+      all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
+      before.x += c.x & m, before.y += c.y & m, before.z += c.z & m, before.w += c.w & m;
+    }
+    reinterpret_cast<uint4*>(in_warp[group])[column] = all;
+    reinterpret_cast<uint4*>(in_warp[kGroups + group])[column] = before;
+    static_assert(2 * kGroups <= kSortWarps, "both sums' groups fit in_warp");
     __syncthreads();
+    unsigned sum = 0, earlier = 0;
+    if (threadIdx.x < kDigits) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        sum += in_warp[g][threadIdx.x];
+        earlier += in_warp[kGroups + g][threadIdx.x];
+      }
+    }
+    const unsigned lower = digits_below(sum, place);
+    if (threadIdx.x < kDigits) place[threadIdx.x] = lower + earlier;
+    __syncthreads();
+  }
+  for (int base = begin; base < end; base += kSubTile) {
+    if (base != begin) {
+      __syncthreads();
+      fetch(base);
+    }
+    unsigned digit[kItems], rank[kItems];
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int j = base + (warp * kItems + i) * 32 + lane;
-      if (j < end) to[in_warp[warp][(pair[i].x >> shift) & (kDigits - 1)] + rank[i]] = pair[i];
+      digit[i] = j < end ? (pair[i].x >> shift) & (kDigits - 1) : kNone;
     }
+    rank_items<kItems>(digit, rank, in_warp);
+    place_warps(in_warp, place);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (digit[i] != kNone) to[in_warp[warp][digit[i]] + rank[i]] = pair[i];
+    }
+  }
+}
+
+// Up to kSmall lookups: CTA 0 finds the bags and does all digits in shared memory, the others fill with zeros.
+__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs a, uint2* to, int passes, const ZeroSpan z) {
+  pdl_enter();
+  if (blockIdx.x > 0) {
+    zero_span(z, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
+  __shared__ unsigned place[kDigits];
+  __shared__ unsigned in_warp[kSortWarps][kDigits];
+  __shared__ __align__(16) char buffer[kSmall * sizeof(uint2)];   // the starts, then the pairs between digits
+  static_assert(kSmall >= kStarts, "the starts fit");
+  long long* starts = reinterpret_cast<long long*>(buffer);
+  uint2* pairs = reinterpret_cast<uint2*>(buffer);
+  __shared__ unsigned total[kDigits / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const TileStarts t = find_starts(a, 0, a.n, starts);
+  uint2 pair[kSmallItems];
+#pragma unroll
+  for (int i = 0; i < kSmallItems; ++i) {
+    const int j = (warp * kSmallItems + i) * 32 + lane;
+    int bag = -1;
+    pair[i] = make_uint2(0, 0);
+    if (j < a.n) {
+      bag = bag_of(a, j, t, starts);
+      a.bag_of[j] = bag;
+      pair[i] = make_uint2(row_of(a, j, bag), a.by_bag ? (unsigned)bag : (unsigned)j);
+    }
+    if (a.counted) uncount_padding(a, j, j < a.n, bag);
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    unsigned digit[kSmallItems], rank[kSmallItems];
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) {
+      const int j = (warp * kSmallItems + i) * 32 + lane;
+      digit[i] = j < a.n ? (pair[i].x >> (8 * pass)) & (kDigits - 1) : kNone;
+    }
+    rank_items<kSmallItems>(digit, rank, in_warp);
+    unsigned sum = 0;
+    if (threadIdx.x < kDigits) {
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) sum += in_warp[w][threadIdx.x];
+    }
+    const unsigned lower = digits_below(sum, total);
+    if (threadIdx.x < kDigits) place[threadIdx.x] = lower;
+    __syncthreads();
+    place_warps(in_warp, place);
+    const bool last = pass + 1 == passes;
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) {
+      if (digit[i] == kNone) continue;
+      const unsigned at = in_warp[warp][digit[i]] + rank[i];
+      if (last) to[at] = pair[i]; else pairs[at] = pair[i];
+    }
+    if (last) break;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSmallItems; ++i) {
+      const int j = (warp * kSmallItems + i) * 32 + lane;
+      if (j < a.n) pair[i] = pairs[j];
+    }
+    __syncthreads();
+  }
+}
+
+// won[b][c] = the low byte of the position that won column c of bag b: what the sum below compares in bags of
+// fewer than 256 lookups, an eighth of the pairs' bytes.
+__global__ void __launch_bounds__(256) winner_bytes_kernel(const BackArgs a) {
+  pdl_enter();
+  const long long total = (long long)a.num_bags * a.dim;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long bag = i / a.dim;
+    const int col = (int)(i - bag * a.dim);
+    a.won[bag * a.pstride + col] = (unsigned char)__ldg(&a.winners[bag * a.win_stride + col].y);
   }
 }
 
@@ -291,12 +486,29 @@ __device__ __forceinline__ void store_row(const BackArgs& a, unsigned row, int c
   }
 }
 
-enum Kind { kPlain = 0, kScaled = 1, kMax = 2 };
+template <int VE>
+__device__ __forceinline__ void load_table(const BackArgs& a, unsigned row, int col, float (&x)[VE]) {
+  const char* q = a.table + (long long)row * a.table_stride;
+  if (a.table_f16) {
+    Pack<__half, VE> r;
+    r.load_ro(reinterpret_cast<const __half*>(q) + col);
+    r.get(x);
+  } else {
+    Pack<float, VE> r;
+    r.load_ro(reinterpret_cast<const float*>(q) + col);
+    r.get(x);
+  }
+}
+
+// kPlain adds rows, kScaled takes a factor a lookup, kWeights does so and writes grad_weights, kMax masks columns.
+enum Kind { kPlain = 0, kScaled = 1, kWeights = 2, kMax = 3 };
 
 // A warp per run of 32 sorted lookups; blockIdx.y is a tile of 32 * VE columns.
 template <typename TG, int VE, int KIND>
 __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
   pdl_enter();
+  constexpr int U = VE == 8 && KIND != kPlain && KIND != kScaled ? 4 : 8;   // lookups whose loads are issued together
+  constexpr unsigned kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const int run = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (run >= a.runs) return;
@@ -305,21 +517,21 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
   const bool col_ok = col < a.dim;
   uint2 pair = make_uint2(a.num_rows, 0);
   if (base + lane < a.n) pair = pairs[base + lane];
-  const int valid = __popc(__ballot_sync(0xffffffffu, pair.x < a.num_rows));   // the rest sorts behind
-  if (valid == 0) return;
   const unsigned prev = base > 0 ? pairs[base - 1].x : kNone;
   const unsigned next = base + kRun < a.n ? pairs[base + kRun].x : kNone;
+  const int valid = __popc(__ballot_sync(kAll, pair.x < a.num_rows));   // the rest sorts behind
+  if (KIND == kWeights && lane >= valid && base + lane < a.n) a.grad_weights[pair.y] = 0.0f;
+  if (valid == 0) return;
   int bag = 0, pos = 0;
   float coef = 1.0f;
   if (lane < valid) {
-    const int j = (int)pair.y;
-    bag = a.bag_of[j];
-    if (KIND == kScaled) {
+    bag = a.by_bag ? (int)pair.y : a.bag_of[pair.y];
+    if (KIND == kScaled || KIND == kWeights) {
       if (a.psw) {
-        coef = a.psw[j];
+        coef = a.psw[pair.y];
       } else if (a.counted) {
         coef = 1.0f / (float)a.counted[bag];
-      } else {
+      } else if (a.mean) {
         long long s, e;
         bag_range(a, bag, s, e);
         coef = 1.0f / (float)(e - s);
@@ -327,13 +539,14 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
     } else if (KIND == kMax) {
       long long s, e;
       bag_range(a, bag, s, e);
-      pos = j - (int)s;
+      pos = (int)pair.y - (int)s;
+      if (e - s >= 256) pos |= INT_MIN;      // compare whole positions
     }
   }
   float acc[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
-  unsigned row = __shfl_sync(0xffffffffu, pair.x, 0);
+  unsigned row = __shfl_sync(kAll, pair.x, 0);
   bool began_before = row == prev;
 
   auto put = [&](bool goes_on) {
@@ -346,28 +559,34 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
       r.store(a.partial + ((long long)run * 2 + (began_before ? 0 : 1)) * a.pstride + col);
     }
   };
-  constexpr int U = 8;
+  float x[KIND == kWeights ? VE : 1];     // the table row of the running segment
   for (int e0 = 0; e0 < valid; e0 += U) {
     Pack<TG, VE> g[U];
-    int2 win[KIND == kMax ? U : 1][KIND == kMax ? VE : 1];
+    Pack<unsigned char, VE> won[KIND == kMax ? U : 1];
+    float xs[KIND == kWeights ? U : 1][KIND == kWeights ? VE : 1];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int b = __shfl_sync(0xffffffffu, bag, e0 + u);
+      const int b = __shfl_sync(kAll, bag, e0 + u);
+      const unsigned r = __shfl_sync(kAll, pair.x, e0 + u);
+      const unsigned before = __shfl_sync(kAll, pair.x, (e0 + u - 1) & 31);
       g[u].zero();
       if (e0 + u < valid && col_ok) {
         g[u].load_ro(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
-        if (KIND == kMax) {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) win[u][i] = __ldg(a.winners + (long long)b * a.win_stride + col + i);
+        if constexpr (KIND == kMax) won[u].load_ro(a.won + (long long)b * a.pstride + col);
+        if constexpr (KIND == kWeights) {   // a segment's first lookup in the run brings the row
+          if (e0 + u == 0 || r != before) load_table<VE>(a, r, col, xs[u]);
         }
       }
     }
+    float dot[KIND == kWeights ? U : 1];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const unsigned r = __shfl_sync(0xffffffffu, pair.x, e0 + u);
-      const float c = __shfl_sync(0xffffffffu, coef, e0 + u);
-      const int at = __shfl_sync(0xffffffffu, pos, e0 + u);
+      const unsigned r = __shfl_sync(kAll, pair.x, e0 + u);
+      const float c = __shfl_sync(kAll, coef, e0 + u);
+      const int at = __shfl_sync(kAll, pos, e0 + u);
+      if constexpr (KIND == kWeights) dot[u] = 0.0f;
       if (e0 + u >= valid) continue;
+      const bool starts = e0 + u == 0 || r != row;
       if (r != row) {
         put(false);
         row = r;
@@ -377,12 +596,55 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
       }
       float f[VE];
       g[u].get(f);
+      if constexpr (KIND == kWeights) {
+        if (starts) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        if (KIND == kPlain) acc[i] += f[i];
-        else if (KIND == kScaled) acc[i] = fmaf(c, f[i], acc[i]);
-        else acc[i] += col_ok && win[u][i].y == at ? f[i] : 0.0f;
+          for (int i = 0; i < VE; ++i) x[i] = xs[u][i];
+        }
+        if (col_ok) {
+#pragma unroll
+          for (int i = 0; i < VE; ++i) dot[u] = fmaf(f[i], x[i], dot[u]);
+        }
       }
+      if constexpr (KIND == kMax) {
+        unsigned char w[VE];
+        memcpy(w, won[u].w, sizeof(w));
+        const int b = __shfl_sync(kAll, bag, e0 + u);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          bool mine = w[i] == (unsigned char)at;
+          if (at < 0 && mine && col_ok)
+            mine = __ldg(&a.winners[(long long)b * a.win_stride + col + i].y) == (at & 0x7fffffff);
+          acc[i] += mine ? f[i] : 0.0f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) acc[i] = KIND == kPlain ? acc[i] + f[i] : fmaf(c, f[i], acc[i]);
+      }
+    }
+    if constexpr (KIND == kWeights) {
+      // sums over the lanes of U values at once: a step halves the values a lane carries or the lanes of one
+      int n = U;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const bool upper = (lane & o) != 0;
+        if (n > 1) {
+          n /= 2;
+#pragma unroll
+          for (int k = 0; k < U / 2; ++k) {
+            if (k >= n) break;
+            const float give = upper ? dot[k] : dot[k + n];
+            const float keep = upper ? dot[k + n] : dot[k];
+            dot[k] = keep + __shfl_xor_sync(kAll, give, o);
+          }
+        } else {
+          dot[0] += __shfl_xor_sync(kAll, dot[0], o);
+        }
+      }
+      constexpr int kShift = U == 8 ? 2 : 3;      // lanes that share a value: 2^kShift
+      const int u = lane >> kShift;
+      const unsigned j = __shfl_sync(kAll, pair.y, e0 + u);
+      if ((lane & ((1 << kShift) - 1)) == 0 && e0 + u < valid) a.grad_weights[j] = dot[0];
     }
   }
   put(row == next);
@@ -426,8 +688,9 @@ __global__ void __launch_bounds__(256) segment_block_kernel(const BackArgs a, co
   r.store(a.super + (long long)block * a.pstride + col);
 }
 
-// Rows that cross runs: a CTA looks at 8 runs and joins, one after the other, the rows that start in one of
-// them and go on.  Its 8 warps take consecutive shares of the row's partial sums.
+// Rows that cross runs.  A warp looks at one run: where a row starts in it and goes on, the warp adds the row's
+// pieces itself if they are few, else the CTA's 8 warps share them.
+constexpr int kFewPieces = 24;
 template <int VE>
 __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, const uint2* pairs) {
   pdl_enter();
@@ -440,29 +703,31 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
   int last = -1;          // the row's last run, -1: nothing to join here
   if (run + 1 < a.runs) {
     const unsigned row = pairs[run * kRun + kRun - 1].x;
-    const bool from_before = run > 0 && pairs[run * kRun - 1].x == row;
-    if (row < a.num_rows && first_row(pairs, run + 1) == row && !from_before) {
-      int lo = run + 1, hi = a.runs - 1;    // the last run that starts with the row
-      while (lo < hi) {
-        const int mid = hi - (hi - lo) / 2;
-        if (first_row(pairs, mid) == row) lo = mid; else hi = mid - 1;
+    const unsigned before = run > 0 ? pairs[run * kRun - 1].x : kNone;
+    // the next 32 runs at once; rows of more are searched for
+    const unsigned ahead = run + 1 + lane < a.runs ? first_row(pairs, run + 1 + lane) : kNone;
+    const unsigned same = __ballot_sync(0xffffffffu, ahead == row);
+    if (row < a.num_rows && before != row && (same & 1u)) {
+      if (same != 0xffffffffu) {
+        last = run + __ffs(~same) - 1;
+      } else {
+        int lo = run + 32, hi = a.runs - 1;    // the last run that starts with the row
+        while (lo < hi) {
+          const int mid = hi - (hi - lo) / 2;
+          if (first_row(pairs, mid) == row) lo = mid; else hi = mid - 1;
+        }
+        last = lo;
       }
-      last = lo;
     }
   }
-  if (lane == 0) last_run[warp] = last;
-  __syncthreads();
-  for (int w = 0; w < 8; ++w) {
-    const int to = last_run[w];
-    if (to < 0) continue;              // the same for the whole CTA
-    const int from = blockIdx.x * 8 + w;
-    // the row's pieces: its tail in `from`, single runs up to a block border, whole blocks, single runs
+  float acc[4][VE];
+  // the row's pieces [begin, end) into acc[0]: its tail in `from`, single runs up to a block border, whole
+  // blocks, single runs
+  auto add_pieces = [&](int from, int to, int begin, int end) {
     const int first = from + 1;
     int b0 = (first + kRun - 1) / kRun, b1 = (to + 1) / kRun;     // whole blocks [b0, b1)
     if (!a.super || b1 < b0) b0 = b1 = 0;
-    const bool blocks = b1 > b0;
-    const int head = blocks ? b0 * kRun - first : to - first + 1;
-    const int pieces = 1 + head + (blocks ? (b1 - b0) + (to + 1 - b1 * kRun) : 0);
+    const int head = b1 > b0 ? b0 * kRun - first : to - first + 1;
     auto piece = [&](int i) -> const float* {
       if (i == 0) return a.partial + ((long long)from * 2 + 1) * a.pstride;
       i -= 1;
@@ -471,33 +736,55 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
       if (i < b1 - b0) return a.super + (long long)(b0 + i) * a.pstride;
       return a.partial + (long long)(b1 * kRun + (i - (b1 - b0))) * 2 * a.pstride;
     };
-    const int share = (pieces + 7) / 8;
-    const int begin = warp * share, end = min(pieces, begin + share);
-    float acc[4][VE];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
       for (int i = 0; i < VE; ++i) acc[k][i] = 0.0f;
     }
-    if (col_ok) {
-      for (int i0 = begin; i0 < end; i0 += 4) {
-        Pack<float, VE> p[4];
+    if (!col_ok) return;
+    for (int i0 = begin; i0 < end; i0 += 4) {
+      Pack<float, VE> p[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          p[u].zero();
-          if (i0 + u < end) p[u].load(piece(i0 + u) + col);
-        }
+      for (int u = 0; u < 4; ++u) {
+        p[u].zero();
+        if (i0 + u < end) p[u].load(piece(i0 + u) + col);
+      }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float f[VE];
-          p[u].get(f);
+      for (int u = 0; u < 4; ++u) {
+        float f[VE];
+        p[u].get(f);
 #pragma unroll
-          for (int i = 0; i < VE; ++i) acc[u][i] += f[i];
-        }
+        for (int i = 0; i < VE; ++i) acc[u][i] += f[i];
       }
     }
 #pragma unroll
-    for (int i = 0; i < VE; ++i) part[warp][lane * VE + i] = (acc[0][i] + acc[1][i]) + (acc[2][i] + acc[3][i]);
+    for (int i = 0; i < VE; ++i) acc[0][i] = (acc[0][i] + acc[1][i]) + (acc[2][i] + acc[3][i]);
+  };
+  auto count_pieces = [&](int from, int to) {
+    const int first = from + 1;
+    const int b0 = (first + kRun - 1) / kRun, b1 = (to + 1) / kRun;
+    if (!a.super || b1 <= b0) return 1 + to - first + 1;
+    return 1 + (b0 * kRun - first) + (b1 - b0) + (to + 1 - b1 * kRun);
+  };
+  if (last >= 0) {
+    const int pieces = count_pieces(run, last);
+    if (pieces <= kFewPieces) {
+      add_pieces(run, last, 0, pieces);
+      if (col_ok) store_row<VE>(a, pairs[run * kRun + kRun - 1].x, col, acc[0]);
+      last = -1;
+    }
+  }
+  if (lane == 0) last_run[warp] = last;
+  if (__syncthreads_or(last >= 0) == 0) return;
+  for (int w = 0; w < 8; ++w) {
+    const int to = last_run[w];
+    if (to < 0) continue;              // the same for the whole CTA
+    const int from = blockIdx.x * 8 + w;
+    const int pieces = count_pieces(from, to);
+    const int share = (pieces + 7) / 8;
+    add_pieces(from, to, min(pieces, warp * share), min(pieces, (warp + 1) * share));
+#pragma unroll
+    for (int i = 0; i < VE; ++i) part[warp][lane * VE + i] = acc[0][i];
     __syncthreads();
     if (warp == 0 && col_ok) {
       float sum[VE];
@@ -551,6 +838,7 @@ struct BackPlan {
   int passes;                // of the sort, a digit each
   int ve;                    // columns a lane
   bool want_table;
+  bool fused_weights;        // grad_weights comes out of the segment sum
   size_t bytes;              // workspace
 };
 
@@ -636,13 +924,13 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
 
   pl->passes = 1;
   while (pl->passes < 4 && (a.num_rows >> (8 * pl->passes)) != 0) ++pl->passes;   // num_rows itself is a key
-  const int most_tiles = sm_count();
-  const long long per = ((long long)a.n + most_tiles - 1) / most_tiles;
-  a.tile = (int)((per + kSortThreads - 1) / kSortThreads * kSortThreads);
-  if (a.tile < kSortThreads) a.tile = kSortThreads;
+  const long long per = ((long long)a.n + sm_count() - 1) / sm_count();
+  a.tile = (int)(per < 1024 ? 1024 : (per + 31) / 32 * 32);
   a.tiles = (int)(((long long)a.n + a.tile - 1) / a.tile);
   a.runs = (int)(((long long)a.n + kRun - 1) / kRun);
   a.pstride = (f.dim + 7) / 8 * 8;
+  pl->fused_weights = pl->want_table && a.grad_weights && f.dim <= 32 * pl->ve;
+  a.by_bag = !a.winners && !a.psw && !pl->fused_weights;
 
   // scratch, each part on a 256-byte border
   size_t at = 0;
@@ -665,6 +953,7 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
     const int blocks = a.runs / kRun;
     const size_t super = take((size_t)blocks * a.pstride * 4);
     a.super = blocks > 1 ? reinterpret_cast<float*>(ws + super) : nullptr;
+    a.won = reinterpret_cast<unsigned char*>(ws + take(a.winners ? (size_t)a.num_bags * a.pstride : 0));
   } else {
     a.hist = reinterpret_cast<unsigned*>(ws + take((size_t)a.tiles * kDigits * 4));
   }
@@ -684,6 +973,7 @@ cudaError_t launch_segments(const BackPlan& pl, const uint2* sorted, cudaStream_
   const unsigned tiles = (unsigned)((a.dim + 32 * VE - 1) / (32 * VE));
   const dim3 grid((unsigned)((a.runs + 7) / 8), tiles);
   if (a.winners) FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kMax>, grid, 256, 0, st, a, sorted));
+  else if (pl.fused_weights) FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kWeights>, grid, 256, 0, st, a, sorted));
   else if (a.psw || a.mean) FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kScaled>, grid, 256, 0, st, a, sorted));
   else FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kPlain>, grid, 256, 0, st, a, sorted));
   if (a.super) {
@@ -719,36 +1009,70 @@ cudaError_t launch_weights(const BackPlan& pl, cudaStream_t st) {
   }
 }
 
-cudaError_t launch_backward(const BackPlan& pl, const fwd_eb_backward_params* p, cudaStream_t st) {
-  const BackArgs& a = pl.a;
-  if (pl.want_table && !a.accumulate) {
+// The zeros of a dense gradient, in as many equal spans as there are launches to carry them.
+struct Zeros {
+  ZeroSpan z;
+  long long words;
+  int spans, done;
+  Zeros(const BackPlan& pl, int spans_) : z(), words(0), spans(spans_), done(0) {
+    const BackArgs& a = pl.a;
+    if (!pl.want_table || a.accumulate) return;
     const long long row_bytes = (long long)a.dim * (a.gt_f16 ? 2 : 4);
     const bool wide = aligned_to(a.grad_table, 16) && a.gt_stride % 16 == 0 && row_bytes % 16 == 0;
-    const int word = wide ? 16 : (a.gt_f16 ? 2 : 4);
-    const long long words = row_bytes / word * a.num_rows, most = 8LL * sm_count();
-    const long long blocks = (words + 255) / 256;
-    FWD_EB_TRY(launch_pdl(zero_rows_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, st, a.grad_table,
-                          row_bytes, a.gt_stride, (long long)a.num_rows, word));
+    z.word = wide ? 16 : (a.gt_f16 ? 2 : 4);
+    z.base = a.grad_table;
+    z.stride = a.gt_stride;
+    z.per_row = row_bytes / z.word;
+    words = z.per_row * a.num_rows;
   }
-  if (a.n == 0) return cudaSuccess;
+  ZeroSpan next() {
+    z.begin = words * done / spans;
+    ++done;
+    z.end = words * done / spans;
+    return z;
+  }
+  // CTAs that fill a span beside a sort's: two an SM, fewer for little
+  unsigned ctas() const {
+    const long long most = 2LL * sm_count(), want = (words / spans + 4 * kSortThreads) / (4 * kSortThreads);
+    return words == 0 ? 0u : (unsigned)(want < most ? want : most);
+  }
+};
+
+cudaError_t launch_backward(const BackPlan& pl, const fwd_eb_backward_params* p, cudaStream_t st) {
+  const BackArgs& a = pl.a;
+  const bool small = a.n <= kSmall;
+  Zeros zeros(pl, a.n == 0 || small || !pl.want_table ? 1 : 2 * pl.passes);
+  const unsigned zc = zeros.ctas();
+  if (a.n == 0) return zc == 0 ? cudaSuccess : launch_pdl(zero_kernel, dim3(zc), kSortThreads, 0, st, zeros.next());
   if (a.counted && a.num_bags > 0)
     FWD_EB_TRY(launch_pdl(bag_length_kernel, dim3((unsigned)((a.num_bags + 255) / 256)), 256, 0, st, a));
-  const dim3 tiles((unsigned)a.tiles);
+  if (pl.want_table && a.winners) {
+    const long long blocks = ((long long)a.num_bags * a.dim + 255) / 256, most = 16LL * sm_count();
+    if (blocks > 0)
+      FWD_EB_TRY(launch_pdl(winner_bytes_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, st, a));
+  }
+  const dim3 tiles((unsigned)a.tiles + zc);
   const uint2* none = nullptr;
-  FWD_EB_TRY(launch_pdl(sort_histogram_kernel<true>, tiles, kSortThreads, 0, st, a, none, 0));
-  if (a.grad_weights) {
+  int now = 0;
+  if (small && pl.want_table) {
+    FWD_EB_TRY(launch_pdl(sort_small_kernel, dim3(1 + zc), kSortThreads, 0, st, a, a.pairs[0], pl.passes, zeros.next()));
+  } else {
+    FWD_EB_TRY(launch_pdl(sort_histogram_kernel<true>, tiles, kSortThreads, 0, st, a, none, 0, zeros.next()));
+    if (pl.want_table)
+      FWD_EB_TRY(launch_pdl(sort_scatter_kernel<true>, tiles, kSortThreads, 0, st, a, none, a.pairs[0], 0, zeros.next()));
+    for (int pass = 1; pass < pl.passes && pl.want_table; ++pass, now ^= 1) {
+      const uint2* from = a.pairs[now];
+      FWD_EB_TRY(launch_pdl(sort_histogram_kernel<false>, tiles, kSortThreads, 0, st, a, from, pass * 8, zeros.next()));
+      FWD_EB_TRY(launch_pdl(sort_scatter_kernel<false>, tiles, kSortThreads, 0, st, a, from, a.pairs[now ^ 1], pass * 8,
+                            zeros.next()));
+    }
+  }
+  if (a.grad_weights && !pl.fused_weights) {
     const bool g16 = p->grad_out_dtype == FWD_EB_F16;
     FWD_EB_TRY(g16 ? (a.table_f16 ? launch_weights<__half, __half>(pl, st) : launch_weights<__half, float>(pl, st))
                    : (a.table_f16 ? launch_weights<float, __half>(pl, st) : launch_weights<float, float>(pl, st)));
   }
   if (!pl.want_table) return cudaSuccess;
-  FWD_EB_TRY(launch_pdl(sort_scatter_kernel<true>, tiles, kSortThreads, 0, st, a, none, a.pairs[0], 0));
-  int now = 0;
-  for (int pass = 1; pass < pl.passes; ++pass, now ^= 1) {
-    const uint2* from = a.pairs[now];
-    FWD_EB_TRY(launch_pdl(sort_histogram_kernel<false>, tiles, kSortThreads, 0, st, a, from, pass * 8));
-    FWD_EB_TRY(launch_pdl(sort_scatter_kernel<false>, tiles, kSortThreads, 0, st, a, from, a.pairs[now ^ 1], pass * 8));
-  }
   return p->grad_out_dtype == FWD_EB_F16 ? launch_segments_ve<__half>(pl, a.pairs[now], st)
                                          : launch_segments_ve<float>(pl, a.pairs[now], st);
 }

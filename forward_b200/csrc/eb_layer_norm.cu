@@ -1,13 +1,16 @@
 // Layer norm of pooled rows and its gradients (include/fwd_eb_train.h).
 //
-// Both directions are bound by memory: a row is read once into registers, its statistics are
-// taken from there (mean first, then the squared distances from it: no cancellation), and the
-// result is written once.  TPR threads share a row, NV vectors of VEC elements each; the backward
-// pass walks rows with a fixed grid so that a thread keeps its columns' share of grad_weight and
-// grad_bias in registers, and a second kernel adds the CTAs' shares in CTA order.
+// Both directions are bound by memory as long as few instructions are spent on an element.  TPR threads
+// share a row, up to 16 elements each, and a CTA walks rows with a fixed grid: the next rows are
+// under way to shared memory while this one is worked on (each thread copies what it will read itself, so
+// no barrier stands between), the weights stay in registers, and so do a column's shares of
+// grad_weight and grad_bias, which a second kernel adds in CTA order.  A row's values are converted
+// once and stay in registers as fp32; the mean is taken first, then the squared distances from it (no
+// cancellation).  Arithmetic is done on pairs (sm_100's packed fp32).
 //
 // Rows that do not fit the registers of a CTA take the *_loop kernels, which read them again for
 // each pass.
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -32,23 +35,40 @@ struct NormArgs {
   float eps;
 };
 
-// Sum over the TPR threads of a row, the same value in each; `red` is TPR / 32 floats, used by
-// one sum at a time (a second call may follow at once: it synchronises before it writes).
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
+// Sums over the TPR threads of a row, the same values in each.  `red` belongs to this call alone until every
+// thread of the CTA has passed one more synchronisation: callers alternate between two.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[K]) {
   constexpr int kWidth = TPR < 32 ? TPR : 32;
 #pragma unroll
-  for (int o = kWidth / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = kWidth / 2; o > 0; o >>= 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  }
   if constexpr (TPR > 32) {
     constexpr int kWarps = TPR / 32;
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = (threadIdx.x & 31) < kWarps ? red[threadIdx.x & 31] : 0.0f;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int k = 0; k < K; ++k) {
+      if (lane == k) red[threadIdx.x >> 5][k] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = lane < kWarps ? red[lane][k] : 0.0f;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = __shfl_sync(0xffffffffu, v[k], 0);
   }
-  return v;
+}
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float (*red)[1]) {
+  float one[1] = {v};
+  row_sum<TPR, 1>(one, red);
+  return one[0];
 }
 
 template <int VEC>
@@ -65,49 +85,142 @@ __device__ __forceinline__ void load_weight(const void* w, int dtype, int col, f
 template <int TPR>
 constexpr int kThreads = TPR <= 32 ? 256 : TPR;
 inline int cta_threads(int tpr) { return tpr <= 32 ? 256 : tpr; }
+// Threads an SM holds: the registers a thread may take (85 and 128).
+constexpr int kForwardThreads = 768, kBackwardThreads = 512;
+// Rows under way for each that is worked on.
+constexpr int kForwardDepth = 2;
+template <typename T>
+constexpr int kBackwardDepth = sizeof(T) == 2 ? 3 : 2;
+constexpr int resident_ctas(int threads, int cta) { return threads / cta < 1 ? 1 : threads / cta; }
+
+// Elementwise on V fp32 values, in pairs where there are any.
+template <int V, typename F2, typename F1>
+__device__ __forceinline__ void each(F2 two, F1 one) {
+#pragma unroll
+  for (int i = 0; i + 1 < V; i += 2) two(i);
+  if (V % 2) one(V - 1);
+}
+__device__ __forceinline__ float2 at2(const float* f, int i) { return make_float2(f[i], f[i + 1]); }
+__device__ __forceinline__ void put2(float* f, int i, float2 v) {
+  f[i] = v.x;
+  f[i + 1] = v.y;
+}
+
+// The rows a thread is about to read, ARRAYS arrays of them: DEPTH rows ahead in shared memory where an
+// access is 16 bytes, else one row ahead in registers.
+template <typename T, int VEC, int NV, int TPR, int ARRAYS, int DEPTH>
+struct Ahead {
+  static constexpr bool kAsync = VEC * sizeof(T) == 16;
+  static constexpr int kDepth = kAsync ? DEPTH : 1;
+  static constexpr int kBytes = kAsync ? DEPTH * ARRAYS * NV * kThreads<TPR> * 16 : 0;   // of shared memory
+  uint4* mine;                                  // [DEPTH][ARRAYS][NV][threads], this thread's
+  Pack<T, VEC> reg[kAsync ? 1 : ARRAYS][kAsync ? 1 : NV];
+  int slot;                                     // of the oldest row
+  int cols, lane;
+  __device__ __forceinline__ void init(void* shared, int cols_) {
+    mine = static_cast<uint4*>(shared) + threadIdx.x;
+    slot = 0;
+    cols = cols_;
+    lane = threadIdx.x % TPR;
+  }
+  __device__ __forceinline__ uint4* at(int s, int array, int k) {
+    return mine + ((s * ARRAYS + array) * NV + k) * kThreads<TPR>;
+  }
+  // `from`: the row in each array; `live`: there is such a row.  s: 0 is behind the oldest row, kDepth - 1 the newest.
+  __device__ __forceinline__ void fetch(const T* const (&from)[ARRAYS], bool live, int s) {
+    int to = slot + s;
+    if (to >= kDepth) to -= kDepth;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int col = (k * TPR + lane) * VEC;
+#pragma unroll
+      for (int q = 0; q < ARRAYS; ++q) {
+        if constexpr (kAsync) {
+          if (live && col < cols) copy16_async(at(to, q, k), from[q] + col);
+        } else {
+          reg[q][k].zero();
+          if (live && col < cols) reg[q][k].load(from[q] + col);
+        }
+      }
+    }
+    if constexpr (kAsync) copy_commit();
+  }
+  // The oldest row's values (zeros behind its end) and its slot freed.
+  __device__ __forceinline__ void take(float (&f)[ARRAYS][NV][VEC]) {
+    if constexpr (kAsync) copy_wait<kDepth - 1>();
+#pragma unroll
+    for (int q = 0; q < ARRAYS; ++q) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        Pack<T, VEC> r;
+        if constexpr (kAsync) {
+          r.zero();
+          if ((k * TPR + lane) * VEC < cols) r.load(at(slot, q, k));
+        } else {
+          r = reg[q][k];
+        }
+        r.get(f[q][k]);
+      }
+    }
+    if (++slot == kDepth) slot = 0;
+  }
+};
 
 template <typename T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(kThreads<TPR>)
+__global__ void __launch_bounds__(kThreads<TPR>, kForwardThreads / kThreads<TPR> < 1 ? 1 : kForwardThreads / kThreads<TPR>)
 layer_norm_forward_kernel(const NormArgs a) {
   pdl_enter();
   constexpr int kRows = kThreads<TPR> / TPR;
-  __shared__ float red[32];
+  __shared__ float red[2][32][1];
   const int lane = threadIdx.x % TPR;
+  const float inv_cols = 1.0f / (float)a.cols;
+  float w[NV][VEC], b[NV][VEC];
+  extern __shared__ uint4 ring[];
+  using Rows = Ahead<T, VEC, NV, TPR, 1, kForwardDepth>;
+  Rows ahead;
+  ahead.init(ring, a.cols);
   const long long step = (long long)gridDim.x * kRows;
+  auto fetch = [&](long long row, int s) {
+    const T* from[1] = {reinterpret_cast<const T*>(a.x) + row * a.x_stride};
+    ahead.fetch(from, row < a.rows, s);
+  };
+  for (int s = 0; s < Rows::kDepth; ++s) fetch((long long)blockIdx.x * kRows + threadIdx.x / TPR + s * step, s);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int col = (k * TPR + lane) * VEC;
+    const bool in = col < a.cols;
+    load_weight<VEC>(in ? a.weight : nullptr, a.wtype, col, 1.0f, w[k]);
+    load_weight<VEC>(in ? a.bias : nullptr, a.wtype, col, 0.0f, b[k]);
+  }
   // every thread of the CTA makes the same number of turns
   for (long long base = (long long)blockIdx.x * kRows; base < a.rows; base += step) {
     const long long row = base + threadIdx.x / TPR;
-    const bool live = row < a.rows;
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
-    Pack<T, VEC> raw[NV];
-    float sum = 0.0f;
+    float taken[1][NV][VEC];
+    ahead.take(taken);
+    fetch(row + Rows::kDepth * step, Rows::kDepth - 1);
+    float (&f)[NV][VEC] = taken[0];
+    float2 sum = both(0.0f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      each<VEC>([&](int i) { sum = add2(sum, at2(f[k], i)); }, [&](int i) { sum.x += f[k][i]; });
+    const float mean = row_sum<TPR>(sum.x + sum.y, red[0]) * inv_cols;
+    float2 square = both(0.0f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int col = (k * TPR + lane) * VEC;
-      raw[k].zero();
-      if (live && col < a.cols) raw[k].load(x + col);
+      if ((k * TPR + lane) * VEC >= a.cols) continue;
+      each<VEC>(
+          [&](int i) {
+            const float2 d = add2(at2(f[k], i), both(-mean));
+            put2(f[k], i, d);
+            square = fma2(d, d, square);
+          },
+          [&](int i) {
+            f[k][i] -= mean;
+            square.x = fmaf(f[k][i], f[k][i], square.x);
+          });
     }
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      float f[VEC];
-      raw[k].get(f);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += f[i];
-    }
-    const float mean = row_sum<TPR>(sum, red) / (float)a.cols;
-    float square = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (k * TPR + lane) * VEC;
-      float f[VEC];
-      raw[k].get(f);
-      if (col < a.cols) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) square = fmaf(f[i] - mean, f[i] - mean, square);
-      }
-    }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(square, red) / (float)a.cols + a.eps);
-    if (!live) continue;
+    const float rstd = 1.0f / sqrtf(fmaf(row_sum<TPR>(square.x + square.y, red[1]), inv_cols, a.eps));
+    if (row >= a.rows) continue;
     if (lane == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -117,14 +230,11 @@ layer_norm_forward_kernel(const NormArgs a) {
     for (int k = 0; k < NV; ++k) {
       const int col = (k * TPR + lane) * VEC;
       if (col >= a.cols) continue;
-      float f[VEC], w[VEC], b[VEC];
-      load_weight<VEC>(a.weight, a.wtype, col, 1.0f, w);
-      load_weight<VEC>(a.bias, a.wtype, col, 0.0f, b);
-      raw[k].get(f);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = fmaf((f[i] - mean) * rstd, w[i], b[i]);
-      raw[k].set(f);
-      raw[k].store(y + col);
+      each<VEC>([&](int i) { put2(f[k], i, fma2(mul2(at2(f[k], i), both(rstd)), at2(w[k], i), at2(b[k], i))); },
+                [&](int i) { f[k][i] = fmaf(f[k][i] * rstd, w[k][i], b[k][i]); });
+      Pack<T, VEC> out;
+      out.set(f[k]);
+      out.store(y + col);
     }
   }
 }
@@ -134,7 +244,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(1024)
 layer_norm_forward_loop_kernel(const NormArgs a) {
   pdl_enter();
-  __shared__ float red[32];
+  __shared__ float red[2][32][1];
   const int step = blockDim.x * VEC;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
@@ -148,7 +258,7 @@ layer_norm_forward_loop_kernel(const NormArgs a) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) sum += f[i];
     }
-    const float mean = row_sum<1024>(sum, red) / (float)a.cols;
+    const float mean = row_sum<1024>(sum, red[0]) / (float)a.cols;
     for (int col = threadIdx.x * VEC; col < a.cols; col += step) {
       Pack<T, VEC> r;
       float f[VEC];
@@ -157,7 +267,7 @@ layer_norm_forward_loop_kernel(const NormArgs a) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) square = fmaf(f[i] - mean, f[i] - mean, square);
     }
-    const float rstd = 1.0f / sqrtf(row_sum<1024>(square, red) / (float)a.cols + a.eps);
+    const float rstd = 1.0f / sqrtf(row_sum<1024>(square, red[1]) / (float)a.cols + a.eps);
     if (threadIdx.x == 0) {
       if (a.mean) a.mean[row] = mean;
       if (a.rstd) a.rstd[row] = rstd;
@@ -174,107 +284,148 @@ layer_norm_forward_loop_kernel(const NormArgs a) {
       r.set(f);
       r.store(y + col);
     }
-    // the next row's first row_sum synchronises before it writes `red`
   }
 }
 
 // grad_x of the rows this CTA walks, and its share of grad_weight and grad_bias.
 template <typename T, int VEC, int NV, int TPR>
-__global__ void __launch_bounds__(kThreads<TPR>)
+__global__ void __launch_bounds__(kThreads<TPR>, kBackwardThreads / kThreads<TPR> < 1 ? 1 : kBackwardThreads / kThreads<TPR>)
 layer_norm_backward_kernel(const NormArgs a) {
   pdl_enter();
   constexpr int kRows = kThreads<TPR> / TPR;
-  __shared__ float red[32];
-  extern __shared__ float share[];   // kRows > 1: [2][cols] sums of the CTA's row groups
+  __shared__ float red[2][32][2];
+  // the rows under way; at the end, with more than one row a CTA, [8 warps][2][cols] sums
+  extern __shared__ uint4 ring[];
   const int lane = threadIdx.x % TPR;
-  const int group = threadIdx.x / TPR;
-  float dw[NV][VEC], db[NV][VEC];
+  const float inv_cols = 1.0f / (float)a.cols;
+  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+  using Rows = Ahead<T, VEC, NV, TPR, 2, kBackwardDepth<T>>;
+  Rows ahead;
+  ahead.init(ring, a.cols);
+  const long long step = (long long)gridDim.x * kRows;
+  float mean_next = 0.0f, rstd_next = 0.0f;
+  auto fetch = [&](long long row, int s) {
+    const T* from[2] = {reinterpret_cast<const T*>(a.x) + row * a.x_stride,
+                        reinterpret_cast<const T*>(a.gy) + row * a.gy_stride};
+    ahead.fetch(from, row < a.rows, s);
+  };
+  auto fetch_stats = [&](long long row) {
+    if (row < a.rows) {
+      mean_next = a.mean[row];
+      rstd_next = a.rstd[row];
+    }
+  };
+  {
+    const long long row = (long long)blockIdx.x * kRows + threadIdx.x / TPR;
+    for (int s = 0; s < Rows::kDepth; ++s) fetch(row + s * step, s);
+    fetch_stats(row);
+  }
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
+    const int col = (k * TPR + lane) * VEC;
+    load_weight<VEC>(col < a.cols ? a.weight : nullptr, a.wtype, col, 1.0f, w[k]);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[k][i] = db[k][i] = 0.0f;
   }
-  const long long step = (long long)gridDim.x * kRows;
-  for (long long base = (long long)blockIdx.x * kRows; base < a.rows; base += step) {
-    const long long row = base + group;
+  int turn = 0;
+  for (long long base = (long long)blockIdx.x * kRows; base < a.rows; base += step, turn ^= 1) {
+    const long long row = base + threadIdx.x / TPR;
     const bool live = row < a.rows;
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
-    const T* gy = reinterpret_cast<const T*>(a.gy) + row * a.gy_stride;
-    Pack<T, VEC> rx[NV], rg[NV];
-    const float mean = live ? a.mean[row] : 0.0f;
-    const float rstd = live ? a.rstd[row] : 0.0f;
+    const float mean = mean_next, rstd = rstd_next;
+    float taken[2][NV][VEC];
+    ahead.take(taken);
+    fetch(row + Rows::kDepth * step, Rows::kDepth - 1);
+    fetch_stats(row + step);
+    float (&h)[NV][VEC] = taken[0];   // x, then (x - mean) * rstd
+    float (&g)[NV][VEC] = taken[1];   // grad_y, then grad_y * weight
+    float2 s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int col = (k * TPR + lane) * VEC;
-      rx[k].zero();
-      rg[k].zero();
-      if (live && col < a.cols) {
-        rx[k].load(x + col);
-        rg[k].load(gy + col);
-      }
-    }
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int col = (k * TPR + lane) * VEC;
-      if (!live || col >= a.cols) continue;
-      float fx[VEC], fg[VEC], w[VEC];
-      load_weight<VEC>(a.weight, a.wtype, col, 1.0f, w);
-      rx[k].get(fx);
-      rg[k].get(fg);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float h = (fx[i] - mean) * rstd;
-        const float g = fg[i] * w[i];
-        s1 += g;
-        s2 = fmaf(g, h, s2);
-        dw[k][i] = fmaf(fg[i], h, dw[k][i]);
-        db[k][i] += fg[i];
-      }
+      if (!live || (k * TPR + lane) * VEC >= a.cols) continue;
+      each<VEC>(
+          [&](int i) {
+            const float2 hi = mul2(add2(at2(h[k], i), both(-mean)), both(rstd)), gy = at2(g[k], i);
+            put2(dw[k], i, fma2(gy, hi, at2(dw[k], i)));
+            put2(db[k], i, add2(gy, at2(db[k], i)));
+            const float2 gw = mul2(gy, at2(w[k], i));
+            s1 = add2(s1, gw);
+            s2 = fma2(gw, hi, s2);
+            put2(h[k], i, hi);
+            put2(g[k], i, gw);
+          },
+          [&](int i) {
+            const float hi = (h[k][i] - mean) * rstd;
+            dw[k][i] = fmaf(g[k][i], hi, dw[k][i]);
+            db[k][i] += g[k][i];
+            const float gw = g[k][i] * w[k][i];
+            s1.x += gw;
+            s2.x = fmaf(gw, hi, s2.x);
+            h[k][i] = hi;
+            g[k][i] = gw;
+          });
     }
     if (a.out) {
-      s1 = row_sum<TPR>(s1, red) / (float)a.cols;
-      s2 = row_sum<TPR>(s2, red) / (float)a.cols;
+      float s[2] = {s1.x + s1.y, s2.x + s2.y};
+      row_sum<TPR, 2>(s, red[turn]);
+      const float m1 = s[0] * inv_cols, m2 = s[1] * inv_cols;
       T* gx = reinterpret_cast<T*>(a.out) + row * a.out_stride;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int col = (k * TPR + lane) * VEC;
         if (!live || col >= a.cols) continue;
-        float fx[VEC], fg[VEC], w[VEC];
-        load_weight<VEC>(a.weight, a.wtype, col, 1.0f, w);
-        rx[k].get(fx);
-        rg[k].get(fg);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float h = (fx[i] - mean) * rstd;
-          fg[i] = rstd * (fmaf(fg[i], w[i], -s1) - h * s2);
-        }
-        rg[k].set(fg);
-        rg[k].store(gx + col);
+        each<VEC>(
+            [&](int i) {
+              const float2 d = fma2(at2(h[k], i), both(-m2), add2(at2(g[k], i), both(-m1)));
+              put2(g[k], i, mul2(d, both(rstd)));
+            },
+            [&](int i) { g[k][i] = rstd * fmaf(h[k][i], -m2, g[k][i] - m1); });
+        Pack<T, VEC> out;
+        out.set(g[k]);
+        out.store(gx + col);
       }
     }
   }
   if (!a.partial) return;
   float* mine = a.partial + (long long)blockIdx.x * 2 * a.cols;
   if constexpr (kRows > 1) {
-    // the CTA's row groups take turns, so the order of the additions is fixed
-    for (int i = threadIdx.x; i < 2 * a.cols; i += blockDim.x) share[i] = 0.0f;
-    for (int g = 0; g < kRows; ++g) {
+    // the row groups of a warp by shuffles, then the warps in order: the order of the additions is fixed
+    constexpr int kWarps = kThreads<TPR> / 32;
+#pragma unroll
+    for (int o = TPR; o < 32; o <<= 1) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          dw[k][i] += __shfl_xor_sync(0xffffffffu, dw[k][i], o);
+          db[k][i] += __shfl_xor_sync(0xffffffffu, db[k][i], o);
+        }
+      }
+    }
+    float* share = reinterpret_cast<float*>(ring);
+    if constexpr (Rows::kAsync) {   // nobody's copies land here any more
+      copy_wait<0>();
       __syncthreads();
-      if (group != g) continue;
+    }
+    if ((threadIdx.x & 31) < TPR) {
+      float* to = share + (threadIdx.x >> 5) * 2 * a.cols;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int col = (k * TPR + lane) * VEC;
         if (col >= a.cols) continue;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          share[col + i] += dw[k][i];
-          share[a.cols + col + i] += db[k][i];
+          to[col + i] = dw[k][i];
+          to[a.cols + col + i] = db[k][i];
         }
       }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * a.cols; i += blockDim.x) mine[i] = share[i];
+    for (int i = threadIdx.x; i < 2 * a.cols; i += kThreads<TPR>) {
+      float sum = share[i];
+#pragma unroll
+      for (int k = 1; k < kWarps; ++k) sum += share[k * 2 * a.cols + i];
+      mine[i] = sum;
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -294,7 +445,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(1024)
 layer_norm_backward_loop_kernel(const NormArgs a) {
   pdl_enter();
-  __shared__ float red[32];
+  __shared__ float red[2][32][1];
   const int step = blockDim.x * VEC;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_stride;
@@ -317,8 +468,8 @@ layer_norm_backward_loop_kernel(const NormArgs a) {
         s2 = fmaf(g, (fx[i] - mean) * rstd, s2);
       }
     }
-    s1 = row_sum<1024>(s1, red) / (float)a.cols;
-    s2 = row_sum<1024>(s2, red) / (float)a.cols;
+    s1 = row_sum<1024>(s1, red[0]) / (float)a.cols;
+    s2 = row_sum<1024>(s2, red[1]) / (float)a.cols;
     for (int col = threadIdx.x * VEC; col < a.cols; col += step) {
       Pack<T, VEC> rx, rg;
       float fx[VEC], fg[VEC], w[VEC];
@@ -385,9 +536,11 @@ layer_norm_join_kernel(const float* partial, int parts, int cols, int wtype, voi
 
 // ---- host -----------------------------------------------------------------------------
 
-// How a call runs: vector width, threads a row and vectors a thread; tpr = 0 is the loop kernel.
+constexpr int kLaneElements = 16;   // elements of a row a thread keeps
+
+// How a call runs: elements a load and threads a row; tpr = 0 is the loop kernel.
 struct NormPlan {
-  int vec, nv, tpr;
+  int vec, tpr;
   int grid;        // CTAs of the main kernel
   int parts;       // backward: rows of the partial sums
 };
@@ -439,73 +592,91 @@ NormPlan plan_norm(const fwd_eb_layer_norm_params* p, bool backward) {
                    sb % full == 0 && aligned_to(p->x, 16) && aligned_to(a, 16) && aligned_to(b, 16) &&
                    aligned_to(p->weight, wbytes) && (backward || aligned_to(p->bias, wbytes));
   pl.vec = vec ? full : 1;
-  const int64_t n = p->cols / pl.vec;   // vectors a row
-  const int most = backward ? 512 : 1024;
-  const int tprs[] = {8, 32, 128, 256, 512, 1024};
+  const int tprs[] = {8, 16, 32, 64, 128, 256, 512};
   for (int t : tprs) {
-    if (t > most || n > 4LL * t) continue;
+    if (p->cols > (int64_t)kLaneElements * t) continue;
     pl.tpr = t;
-    pl.nv = n <= t ? 1 : (n <= 2 * t ? 2 : 4);
     break;
   }
-  const int64_t groups = pl.tpr == 0 ? p->rows : (p->rows + cta_threads(pl.tpr) / pl.tpr - 1) / (cta_threads(pl.tpr) / pl.tpr);
-  if (!backward) {
-    pl.grid = (int)(groups < INT_MAX ? groups : INT_MAX);
+  if (pl.tpr != 0) {
+    // as many CTAs as the SMs hold, or fewer with the same number of turns each
+    const int cta = cta_threads(pl.tpr), rows = cta / pl.tpr;
+    const int64_t groups = (p->rows + rows - 1) / rows;
+    const int64_t resident = (int64_t)sm_count() * resident_ctas(backward ? kBackwardThreads : kForwardThreads, cta);
+    const int64_t turns = (groups + resident - 1) / resident;
+    pl.grid = (int)(turns > 0 ? (groups + turns - 1) / turns : 0);
+    pl.parts = pl.grid;
     return pl;
   }
-  const int64_t resident = (int64_t)sm_count() * (pl.tpr == 0 || pl.tpr > 256 ? 2 : 4);
-  pl.grid = (int)(groups < resident ? groups : resident);
-  pl.parts = pl.grid;
-  if (pl.tpr == 0) {   // row slices of the column kernel: about four CTAs an SM
+  const int64_t resident = 2LL * sm_count();
+  pl.grid = (int)(p->rows < resident ? p->rows : resident);
+  if (backward) {   // row slices of the column kernel: about four CTAs an SM
     const int64_t tiles = (p->cols + 255) / 256;
     int64_t slices = (4LL * sm_count() + tiles - 1) / tiles;
     if (slices > p->rows) slices = p->rows;
     if (slices > 256) slices = 256;
-    pl.parts = (int)(slices < 1 ? 1 : slices);
-    if (p->rows == 0) pl.parts = 0;
+    pl.parts = (int)slices;
   }
   return pl;
 }
 
-template <typename T, int VEC, int NV>
-cudaError_t launch_norm_nv(const NormPlan& pl, const NormArgs& a, bool backward, cudaStream_t st) {
-  const dim3 grid((unsigned)pl.grid);
-  const size_t share = backward && pl.tpr <= 32 && a.partial ? (size_t)2 * a.cols * sizeof(float) : 0;
-#define FWD_EB_NORM(TPR)                                                                                     \
-  case TPR:                                                                                                  \
-    return backward ? launch_pdl(layer_norm_backward_kernel<T, VEC, NV, TPR>, grid, kThreads<TPR>, share, \
-                                 st, a)                                                                      \
-                    : launch_pdl(layer_norm_forward_kernel<T, VEC, NV, TPR>, grid, kThreads<TPR>, 0, st, a)
-  switch (pl.tpr) {
-    FWD_EB_NORM(8);
-    FWD_EB_NORM(32);
-    FWD_EB_NORM(128);
-    FWD_EB_NORM(256);
-    FWD_EB_NORM(512);
-    default:
-      return launch_pdl(layer_norm_forward_kernel<T, VEC, NV, 1024>, grid, 1024, 0, st, a);
+// Launches a kernel that takes up to MOST bytes of dynamic shared memory; more than the default 48 KB (what is
+// static counts too) has to be allowed once a device.
+template <auto KERNEL, int MOST>
+cudaError_t launch_ring(dim3 grid, int threads, int bytes, cudaStream_t st, const NormArgs& a) {
+  if (MOST > 40 * 1024) {
+    static std::atomic<uint64_t> allowed{0};   // a bit a device
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+      e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
+      if (e != cudaSuccess) return e;
+      allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
-#undef FWD_EB_NORM
+  return launch_pdl(KERNEL, grid, threads, (size_t)bytes, st, a);
+}
+
+template <typename T, int VEC, int TPR>
+cudaError_t launch_norm_tpr(const NormPlan& pl, const NormArgs& a, bool backward, cudaStream_t st) {
+  constexpr int NV = kLaneElements / VEC;
+  const dim3 grid((unsigned)pl.grid);
+  if (!backward) {
+    constexpr int ring = Ahead<T, VEC, NV, TPR, 1, kForwardDepth>::kBytes;
+    return launch_ring<layer_norm_forward_kernel<T, VEC, NV, TPR>, ring>(grid, kThreads<TPR>, ring, st, a);
+  }
+  constexpr int ring = Ahead<T, VEC, NV, TPR, 2, kBackwardDepth<T>>::kBytes;
+  // the sums of 8 warps over rows of up to 512 columns
+  constexpr int most = TPR <= 32 && kThreads<TPR> / 32 * 2 * kLaneElements * TPR * 4 > ring
+                           ? kThreads<TPR> / 32 * 2 * kLaneElements * TPR * 4 : ring;
+  const int share = TPR <= 32 && a.partial ? kThreads<TPR> / 32 * 2 * a.cols * (int)sizeof(float) : 0;
+  return launch_ring<layer_norm_backward_kernel<T, VEC, NV, TPR>, most>(grid, kThreads<TPR>, share > ring ? share : ring,
+                                                                        st, a);
 }
 
 template <typename T, int VEC>
 cudaError_t launch_norm_vec(const NormPlan& pl, const NormArgs& a, bool backward, cudaStream_t st) {
-  if (pl.tpr == 0) {
-    if (!backward) return launch_pdl(layer_norm_forward_loop_kernel<T, VEC>, dim3((unsigned)pl.grid), 1024, 0, st, a);
-    // the column sums first: grad_x may be written over grad_y or x
-    if (a.partial) {
-      const dim3 grid((unsigned)((a.cols + 255) / 256), (unsigned)pl.parts);
-      cudaError_t e = launch_pdl(layer_norm_columns_kernel<T>, grid, 256, 0, st, a);
-      if (e != cudaSuccess) return e;
-    }
-    if (!a.out) return cudaSuccess;
-    return launch_pdl(layer_norm_backward_loop_kernel<T, VEC>, dim3((unsigned)pl.grid), 1024, 0, st, a);
+  switch (pl.tpr) {
+    case 8: return launch_norm_tpr<T, VEC, 8>(pl, a, backward, st);
+    case 16: return launch_norm_tpr<T, VEC, 16>(pl, a, backward, st);
+    case 32: return launch_norm_tpr<T, VEC, 32>(pl, a, backward, st);
+    case 64: return launch_norm_tpr<T, VEC, 64>(pl, a, backward, st);
+    case 128: return launch_norm_tpr<T, VEC, 128>(pl, a, backward, st);
+    case 256: return launch_norm_tpr<T, VEC, 256>(pl, a, backward, st);
+    case 512: return launch_norm_tpr<T, VEC, 512>(pl, a, backward, st);
+    default: break;
   }
-  switch (pl.nv) {
-    case 1: return launch_norm_nv<T, VEC, 1>(pl, a, backward, st);
-    case 2: return launch_norm_nv<T, VEC, 2>(pl, a, backward, st);
-    default: return launch_norm_nv<T, VEC, 4>(pl, a, backward, st);
+  if (!backward) return launch_pdl(layer_norm_forward_loop_kernel<T, VEC>, dim3((unsigned)pl.grid), 1024, 0, st, a);
+  // the column sums first: grad_x may be written over grad_y or x
+  if (a.partial) {
+    const dim3 grid((unsigned)((a.cols + 255) / 256), (unsigned)pl.parts);
+    cudaError_t e = launch_pdl(layer_norm_columns_kernel<T>, grid, 256, 0, st, a);
+    if (e != cudaSuccess) return e;
   }
+  if (!a.out) return cudaSuccess;
+  return launch_pdl(layer_norm_backward_loop_kernel<T, VEC>, dim3((unsigned)pl.grid), 1024, 0, st, a);
 }
 
 cudaError_t launch_norm(const NormPlan& pl, const NormArgs& a, int dtype, bool backward, cudaStream_t st) {

@@ -8,6 +8,7 @@ Every result is deterministic.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -60,15 +61,15 @@ class AdamWConfig(C.Structure):
 
 SIGNATURES = {
     "fwd_eb_backward_params_size": (C.c_size_t, []),
-    "fwd_eb_backward_workspace_size": (C.c_size_t, [C.POINTER(BackwardParams)]),
-    "fwd_eb_backward": (C.c_int, [C.POINTER(BackwardParams), _p]),
+    "fwd_eb_backward_workspace_size": (C.c_size_t, [_p]),
+    "fwd_eb_backward": (C.c_int, [_p, _p]),
     "fwd_eb_layer_norm_params_size": (C.c_size_t, []),
-    "fwd_eb_layer_norm_workspace_size": (C.c_size_t, [C.POINTER(LayerNormParams)]),
-    "fwd_eb_layer_norm_forward": (C.c_int, [C.POINTER(LayerNormParams), _p]),
-    "fwd_eb_layer_norm_backward": (C.c_int, [C.POINTER(LayerNormParams), _p]),
+    "fwd_eb_layer_norm_workspace_size": (C.c_size_t, [_p]),
+    "fwd_eb_layer_norm_forward": (C.c_int, [_p, _p]),
+    "fwd_eb_layer_norm_backward": (C.c_int, [_p, _p]),
     "fwd_eb_adamw_tensor_size": (C.c_size_t, []),
     "fwd_eb_adamw_config_size": (C.c_size_t, []),
-    "fwd_eb_adamw_step": (C.c_int, [C.POINTER(AdamWTensor), _i32, C.POINTER(AdamWConfig), _p]),
+    "fwd_eb_adamw_step": (C.c_int, [_p, _i32, _p, _p]),
 }
 
 _bound = None
@@ -102,53 +103,68 @@ def _dtype(t, what: str) -> int:
     return code
 
 
-def _device_of(tensors) -> torch.device:
-    """The one CUDA device of the (name, tensor) pairs; None tensors are skipped."""
-    device = None
-    for name, t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor; there is no CPU path")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+# A struct is handed over as bytes: for a call of a few microseconds, filling a ctypes.Structure field
+# by field is a third of the host's time.
+_FORMATS = {C.c_void_p: "Q", _i32: "i", _i64: "q", C.c_size_t: "Q", C.c_uint32: "I", C.c_double: "d", C.c_float: "f"}
+
+
+def _packer(cls):
+    """struct.Struct with the layout of a ctypes.Structure (nested ones flattened)."""
+    def of(c):
+        return "".join(of(t) if issubclass(t, C.Structure) else _FORMATS[t] for _, t in c._fields_)
+    packer = struct.Struct("@" + of(cls))
+    assert packer.size == C.sizeof(cls)
+    return packer.pack
+
+
+_pack_backward, _pack_norm = _packer(BackwardParams), _packer(LayerNormParams)
+
+
+def _device_of(names, tensors) -> int:
+    """Ordinal of the one CUDA device of the tensors (None ones are skipped; the first is not None)."""
+    device = tensors[0].get_device()
+    if device < 0:
+        raise ValueError(f"{names[0]} must be a CUDA tensor; there is no CPU path")
+    for name, t in zip(names, tensors):
+        if t is not None and t.get_device() != device:
+            if not t.is_cuda:
+                raise ValueError(f"{name} must be a CUDA tensor; there is no CPU path")
+            raise ValueError(f"{name} is on {t.device}, {names[0]} on {tensors[0].device}")
     return device
 
 
-class _On:
-    """Makes a device current for the launch, when it is not already."""
-
-    def __init__(self, device):
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        return _p(torch.cuda.current_stream().cuda_stream)
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _scratch(nbytes: int, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _on(device: int, run, *args):
+    """run(stream, *args) with the device current."""
+    if device == torch.cuda.current_device():
+        return run(_raw_stream(device), *args)
+    with torch.cuda.device(device):
+        return run(_raw_stream(device), *args)
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _rows(t, name: str, cols: int, rows: int | None = None) -> int:
     """Row stride of a 2-D tensor with unit column stride (0, that is `cols`, when it has at most
     one row); raises unless it is [rows, cols]."""
-    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {cols}], got {list(t.shape)}")
-    if cols > 1 and t.shape[0] > 0 and t.stride(1) != 1:
-        raise ValueError(f"{name} must have unit column stride")
-    if t.shape[0] <= 1:
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {cols}], got {list(shape)}")
+    if shape[0] == 0:
         return 0
-    if t.stride(0) < cols:
-        raise ValueError(f"{name}: rows overlap (row stride {t.stride(0)}, {cols} columns)")
-    return t.stride(0)
+    row, col = t.stride()
+    if col != 1 and cols > 1:
+        raise ValueError(f"{name} must have unit column stride")
+    if shape[0] == 1:
+        return 0
+    if row < cols:
+        raise ValueError(f"{name}: rows overlap (row stride {row}, {cols} columns)")
+    return row
 
 
 # ---- gradient of the pooled lookup ----------------------------------------------------
@@ -159,17 +175,22 @@ def embedding_bag_winners(table, indices, offsets=None, *, fixed_len=0, include_
     """A max-pooled call that keeps what its gradient needs: fp32 pairs [num_bags, dim, 2] of the value and, as
     int32 bits, the position in the bag of the index that supplied it (FWD_EB_F32_POS).  The pooled
     rows are pairs[..., 0]; the whole tensor is embedding_bag_backward's `winners`."""
-    device = _device_of([("table", table), ("indices", indices), ("offsets", offsets)])
+    device = _device_of(("table", "indices", "offsets"), (table, indices, offsets))
     if fixed_len == 0 and offsets is None:
         raise ValueError("offsets is None and fixed_len is 0")
     bags = indices.numel() // fixed_len if fixed_len else offsets.numel() - int(include_last_offset)
-    with _On(device) as stream:
-        pairs = torch.empty((max(bags, 0), table.shape[1], 2), dtype=torch.float32, device=device)
+
+    def run(stream):
+        pairs = table.new_empty((max(bags, 0), table.shape[1], 2), dtype=torch.float32)
         p = capi.make_params(table, indices, offsets, out=pairs, mode=capi.MODE_MAX, fixed_len=fixed_len,
                              include_last_offset=include_last_offset, padding_idx=padding_idx, row_lo=row_lo)
         p.out_dtype, p.out_stride = capi.F32_POS, 0
         capi.check(_lib().fwd_eb_forward(C.byref(p), stream))
-    return pairs
+        return pairs
+    return _on(device, run)
+
+
+_BACKWARD_NAMES = ("grad_out", "table", "indices", "offsets", "per_sample_weights", "winners", "grad_table")
 
 
 def embedding_bag_backward(grad_out, table, indices, offsets=None, *, mode=capi.MODE_SUM, fixed_len=0,
@@ -184,9 +205,7 @@ def embedding_bag_backward(grad_out, table, indices, offsets=None, *, mode=capi.
     table.  grad_weights is fp32, [num_indices].  What is not asked for is None.  MODE_MAX takes
     `winners` from embedding_bag_winners.
     """
-    device = _device_of([("grad_out", grad_out), ("table", table), ("indices", indices), ("offsets", offsets),
-                         ("per_sample_weights", per_sample_weights), ("winners", winners),
-                         ("grad_table", grad_table)])
+    device = _device_of(_BACKWARD_NAMES, (grad_out, table, indices, offsets, per_sample_weights, winners, grad_table))
     if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError("table must be 2-D with unit column stride")
     rows, dim = table.shape
@@ -227,49 +246,50 @@ def embedding_bag_backward(grad_out, table, indices, offsets=None, *, mode=capi.
             raise ValueError("winners must be rows of adjacent pairs")
         win_stride = winners.stride(0) // 2 if bags > 1 else 0
     go_stride = _rows(grad_out, "grad_out", dim, bags)
-    lib = _lib()
-    with _On(device) as stream:
-        if need_table:
-            if grad_table is None:
-                grad_table = torch.empty((rows, dim), dtype=grad_dtype or table.dtype, device=device)
-            if grad_table.dtype not in (torch.float32, torch.float16):
-                raise TypeError(f"grad_table: unsupported dtype {grad_table.dtype}")
-            gt_stride = _rows(grad_table, "grad_table", dim, rows)
-        grad_weights = torch.empty(n, dtype=torch.float32, device=device) if need_weights else None
+    if grad_table is None:
+        gt_dtype = grad_dtype or table.dtype
+    else:
+        gt_dtype = grad_table.dtype
+        gt_stride = _rows(grad_table, "grad_table", dim, rows)
+    if need_table and gt_dtype not in (torch.float32, torch.float16):
+        raise TypeError(f"grad_table: unsupported dtype {gt_dtype}")
+    table_code, index_code = capi._torch_dtype_code(table), capi._index_code(indices)
+
+    def run(stream):
+        gt, gs = grad_table, 0 if grad_table is None else gt_stride
+        if need_table and gt is None:
+            gt = table.new_empty((rows, dim), dtype=gt_dtype)
+        gw = table.new_empty(n, dtype=torch.float32) if need_weights else None
         if (rows == 0 or not need_table) and (n == 0 or not need_weights):
-            return grad_table, grad_weights   # nothing to compute; torch gives empty tensors no address
-        psw = per_sample_weights
-        p = BackwardParams(
-            capi.Params(
-                table.data_ptr(), capi._torch_dtype_code(table), dim, rows, row_lo,
-                table.stride(0) if rows > 1 else 0, indices.data_ptr(),
-                None if offsets is None else offsets.data_ptr(), capi._index_code(indices),
-                0 if gather else fixed_len, n, 0 if gather else bags, None if psw is None else psw.data_ptr(), mode,
-                int(include_last_offset), padding_idx, None, 0, 0, 0, None, 0, flags, 0),
-            grad_out.data_ptr(), _DTYPES[grad_out.dtype], _DTYPES[grad_table.dtype] if need_table else 0, go_stride,
-            grad_table.data_ptr() if need_table else None, gt_stride if need_table else 0,
-            grad_weights.data_ptr() if need_weights else None, None if winners is None else winners.data_ptr(),
-            win_stride, None, 0, BACKWARD_ACCUMULATE if accumulate else 0, 0)
-        need = lib.fwd_eb_backward_workspace_size(C.byref(p))
-        if need:
-            ws = _scratch(need, device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), need
-        capi.check(lib.fwd_eb_backward(C.byref(p), stream))
-    return grad_table, grad_weights
+            return gt, gw   # nothing to compute; torch gives empty tensors no address
+
+        def pack(ws, nbytes):
+            return _pack_backward(
+                table.data_ptr(), table_code, dim, rows, row_lo, table.stride(0) if rows > 1 else 0,
+                indices.data_ptr(), _ptr(offsets), index_code, 0 if gather else fixed_len, n, 0 if gather else bags,
+                _ptr(per_sample_weights), mode, include_last_offset, padding_idx, 0, 0, 0, 0, 0, 0, flags, 0,
+                grad_out.data_ptr(), _DTYPES[grad_out.dtype], _DTYPES[gt_dtype], go_stride, _ptr(gt), gs, _ptr(gw),
+                _ptr(winners), win_stride, ws, nbytes, accumulate, 0)
+        lib = _lib()
+        need = lib.fwd_eb_backward_workspace_size(pack(0, 0))
+        ws = table.new_empty(need, dtype=torch.uint8) if need else None
+        capi.check(lib.fwd_eb_backward(pack(_ptr(ws), need), stream))
+        return gt, gw
+    return _on(device, run)
 
 
 # ---- layer norm -------------------------------------------------------------------------
 
 
 def _vector(t, name: str, cols: int, like=None):
-    if t.dim() != 1 or t.shape[0] != cols or (cols > 1 and t.stride(0) != 1):
+    if t.dim() != 1 or t.numel() != cols or (cols > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be contiguous [{cols}]")
     if like is not None and t.dtype != like.dtype:
         raise TypeError(f"{name} must have the weight's dtype")
 
 
 def _stats(t, name: str, rows: int):
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != rows or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous fp32 [{rows}]")
 
 
@@ -278,31 +298,35 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
 
     Returns y of x's dtype (`out`, which may be x, or a new tensor), or (y, mean, rstd) with
     return_stats=True: the fp32 statistics that layer_norm_backward takes."""
-    device = _device_of([("x", x), ("weight", weight), ("bias", bias), ("out", out)])
+    device = _device_of(("x", "weight", "bias", "out"), (x, weight, bias, out))
     if x.dim() != 2:
         raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
     rows, cols = x.shape
     code = _dtype(x, "x")
     x_stride = _rows(x, "x", cols)
     wtype = 0
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _vector(t, name, cols, weight)
-            wtype = _dtype(t, name)
-    if out is not None and out.dtype != x.dtype:
-        raise TypeError("out must have x's dtype")
-    with _On(device) as stream:
-        y = torch.empty((rows, cols), dtype=x.dtype, device=device) if out is None else out
-        y_stride = _rows(y, "out", cols, rows)
+    if weight is not None:
+        _vector(weight, "weight", cols)
+        wtype = _dtype(weight, "weight")
+    if bias is not None:
+        _vector(bias, "bias", cols, weight)
+        wtype = _dtype(bias, "bias")
+    y_stride = 0
+    if out is not None:
+        if out.dtype != x.dtype:
+            raise TypeError("out must have x's dtype")
+        y_stride = _rows(out, "out", cols, rows)
+
+    def run(stream):
+        y = x.new_empty((rows, cols)) if out is None else out
         mean = rstd = None
         if return_stats:
-            mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=device)
-        p = LayerNormParams(
-            x.data_ptr(), code, wtype, rows, cols, x_stride, None if weight is None else weight.data_ptr(),
-            None if bias is None else bias.data_ptr(), eps, mean.data_ptr() if return_stats else None,
-            rstd.data_ptr() if return_stats else None, y.data_ptr(), y_stride)
-        capi.check(_lib().fwd_eb_layer_norm_forward(C.byref(p), stream))
-    return (y, mean, rstd) if return_stats else y
+            mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+        capi.check(_lib().fwd_eb_layer_norm_forward(_pack_norm(
+            x.data_ptr(), code, wtype, rows, cols, x_stride, _ptr(weight), _ptr(bias), eps, _ptr(mean), _ptr(rstd),
+            y.data_ptr(), y_stride, 0, 0, 0, 0, 0, 0, 0, 0), stream))
+        return (y, mean, rstd) if return_stats else y
+    return _on(device, run)
 
 
 def layer_norm_backward(grad_y, x, mean, rstd, weight=None, *, grad_x=None, need_x=True, need_params=True,
@@ -312,8 +336,7 @@ def layer_norm_backward(grad_y, x, mean, rstd, weight=None, *, grad_x=None, need
     mean and rstd are the forward call's.  grad_x (x's dtype) may be given, and may be grad_y or x
     itself.  grad_weight and grad_bias have the weight's dtype, or `param_dtype` (default fp32)
     where there is no weight.  What is not asked for is None."""
-    device = _device_of([("x", x), ("grad_y", grad_y), ("mean", mean), ("rstd", rstd), ("weight", weight),
-                         ("grad_x", grad_x)])
+    device = _device_of(("x", "grad_y", "mean", "rstd", "weight", "grad_x"), (x, grad_y, mean, rstd, weight, grad_x))
     if x.dim() != 2:
         raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
     rows, cols = x.shape
@@ -331,29 +354,26 @@ def layer_norm_backward(grad_y, x, mean, rstd, weight=None, *, grad_x=None, need
     param_dtype = param_dtype or torch.float32
     if param_dtype not in _DTYPES:
         raise TypeError(f"param_dtype: unsupported dtype {param_dtype}")
-    lib = _lib()
-    with _On(device) as stream:
-        gx_stride = 0
-        if need_x:
-            if grad_x is None:
-                grad_x = torch.empty((rows, cols), dtype=x.dtype, device=device)
-            gx_stride = _rows(grad_x, "grad_x", cols, rows)
+    gx_stride = 0 if grad_x is None else _rows(grad_x, "grad_x", cols, rows)
+
+    def run(stream):
+        gx = grad_x
+        if need_x and gx is None:
+            gx = x.new_empty((rows, cols))
         gw = gb = None
         if need_params:
-            gw = torch.empty(cols, dtype=param_dtype, device=device)
-            gb = torch.empty(cols, dtype=param_dtype, device=device)
-        p = LayerNormParams(
-            x.data_ptr(), code, _DTYPES[param_dtype], rows, cols, x_stride,
-            None if weight is None else weight.data_ptr(), None, 0.0, mean.data_ptr(), rstd.data_ptr(), None, 0,
-            grad_y.data_ptr(), gy_stride, grad_x.data_ptr() if need_x else None, gx_stride,
-            gw.data_ptr() if need_params else None, gb.data_ptr() if need_params else None, None, 0)
-        if need_params:
-            need = lib.fwd_eb_layer_norm_workspace_size(C.byref(p))
-            if need:
-                ws = _scratch(need, device)
-                p.workspace, p.workspace_bytes = ws.data_ptr(), need
-        capi.check(lib.fwd_eb_layer_norm_backward(C.byref(p), stream))
-    return grad_x, gw, gb
+            gw, gb = x.new_empty(cols, dtype=param_dtype), x.new_empty(cols, dtype=param_dtype)
+
+        def pack(ws, nbytes):
+            return _pack_norm(
+                x.data_ptr(), code, _DTYPES[param_dtype], rows, cols, x_stride, _ptr(weight), 0, 0.0, mean.data_ptr(),
+                rstd.data_ptr(), 0, 0, grad_y.data_ptr(), gy_stride, _ptr(gx), gx_stride, _ptr(gw), _ptr(gb), ws, nbytes)
+        lib = _lib()
+        need = lib.fwd_eb_layer_norm_workspace_size(pack(0, 0)) if need_params else 0
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
+        capi.check(lib.fwd_eb_layer_norm_backward(pack(_ptr(ws), need), stream))
+        return gx, gw, gb
+    return _on(device, run)
 
 
 # ---- AdamW ------------------------------------------------------------------------------
@@ -381,7 +401,8 @@ class AdamW:
             raise ValueError("AdamW needs at least one parameter")
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits is 32 or 8 (got {state_bits})")
-        self.device = _device_of([(f"params[{i}]", p) for i, p in enumerate(self.params)])
+        self._ordinal = _device_of([f"params[{i}]" for i in range(len(self.params))], self.params)
+        self.device = self.params[0].device
         self.state_bits = state_bits
         self.step_count = int(step)
         n = len(self.params)
@@ -440,6 +461,7 @@ class AdamW:
             self.lr_tensor = torch.full((1,), lr, dtype=torch.float32, device=self.device)
             self._config.d_step, self._config.d_lr = self.step_tensor.data_ptr(), self.lr_tensor.data_ptr()
             self._config.step = 1
+        self._config_ref = C.byref(self._config)
         self._grads = None
         self._lib = _lib()
 
@@ -481,14 +503,16 @@ class AdamW:
         else:
             cfg.d_grad_scale, cfg.grad_scale = None, grad_scale
         cfg.d_skip = None if skip is None else skip.data_ptr()
-        with _On(self.device) as stream:
-            if self.step_tensor is not None:
-                if lr is not None:
-                    self.lr_tensor.fill_(lr)
-                self.step_tensor.add_(1)
-            else:
-                if lr is not None:
-                    cfg.lr = lr
-                cfg.step = self.step_count + 1
-            capi.check(self._lib.fwd_eb_adamw_step(self._table, len(self._table), C.byref(cfg), stream))
+        if self.step_tensor is None:
+            if lr is not None:
+                cfg.lr = lr
+            cfg.step = self.step_count + 1
+        _on(self._ordinal, self._launch, lr)
         self.step_count += 1
+
+    def _launch(self, stream, lr):
+        if self.step_tensor is not None:
+            if lr is not None:
+                self.lr_tensor.fill_(lr)
+            self.step_tensor.add_(1)
+        capi.check(self._lib.fwd_eb_adamw_step(self._table, len(self._table), self._config_ref, stream))

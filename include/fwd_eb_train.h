@@ -159,11 +159,12 @@ typedef struct fwd_eb_adamw_tensor {
  *       - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * in fp32.  8-bit states: each block of FWD_EB_ADAMW_BLOCK elements holds x as
  * scale * e4m3(x / scale), scale = max|x| / 448, rounded to nearest, for x = m and
- * x = sqrt(v); a sqrt(v) above zero never rounds to zero.  The update itself uses the
+ * x = sqrt(v); a sqrt(v) of 2^-63 and more never rounds to zero.  The update itself uses the
  * unrounded m and v.  An 8-bit v only follows changes larger than half a code (about 6 %
  * of sqrt(v)) within a step relative to its block's largest: it suits beta2 of 0.95 or so.
- * A gradient that is not finite makes the states of its element (8 bits: of its block) and
- * the parameter NaN or infinite; d_skip is there to leave such a step out.
+ * A gradient that is not finite makes the states of its element NaN or infinite, and the
+ * parameter from then on; in 8 bits an infinity does that to its whole block.  d_skip is there to
+ * leave such a step out.
  *
  * The d_* pointers are for captured graphs, which replay launches with the numbers they were
  * captured with: where one is not NULL, the kernel reads the value from the device and the
@@ -186,7 +187,7 @@ size_t fwd_eb_adamw_config_size(void);
 
 /* One step over `count` tensors (a host array, read before the call returns; it needs not
  * outlive it).  No two tensors may overlap.  Everything is checked before the first launch;
- * one launch covers up to 256 tensors. */
+ * one launch covers up to 256 tensors of one state width. */
 int fwd_eb_adamw_step(const fwd_eb_adamw_tensor* tensors, int32_t count,
                       const fwd_eb_adamw_config* cfg, void* stream);
 

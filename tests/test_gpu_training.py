@@ -715,10 +715,9 @@ def test_adamw_nonfinite_gradient_stays_in_its_element_or_block():
         assert bad[300] and bad[800] and int(bad.sum()) == 2
         opt.step([torch.full((1024,), 0.5, device=DEV)])
         clean = torch.ones(1024, dtype=torch.bool, device=DEV)
-        if bits == 8:
-            clean[256:512] = clean[768:] = False
-        else:
-            clean[300] = clean[800] = False
+        clean[300] = clean[800] = False
+        if bits == 8:                       # an infinity takes its block with it, a NaN does not
+            clean[768:] = False
         assert torch.isfinite(p[clean]).all() and not torch.isfinite(p[~clean]).any()
 
 
