@@ -2,17 +2,22 @@
 //
 // grad_table[r] is the sum of the grad_out rows of all lookups of r: a reduction by key whose keys
 // are the indices.  Adding with atomics would take them in any order, so the lookups are
-// sorted by row first: a stable radix sort of (row, payload) pairs, digits of 8 bits, two kernels
-// a digit (histogram of every tile, then scatter; up to 4096 lookups: one kernel in one CTA).  The
-// sort is bound by latency and leaves the memory idle, so the same launches carry CTAs that fill
-// the dense gradient with zeros.
+// sorted by row first: a stable radix sort of (row, payload) pairs by digits of up to 8 bits.  Two kernels
+// a digit: one counts it in every tile (the first also makes the pairs), one moves the pairs, brought
+// into the digit's order in shared memory first so that neighbours are stored together.  Up to kSmall
+// lookups are sorted in one CTA.
 //
 // A warp then takes a run of 32 sorted lookups, keeps its columns' running sum in registers,
 // and stores a row's sum where the row's lookups end.  The weights' gradient falls out of the same
 // pass: the table row is read once for all its lookups.  A row whose lookups cross from one run into
 // the next leaves partial sums, which a last kernel adds in run order; a popular row's thousands
 // of runs are first added 32 at a time.  Every sum has one order, whatever the schedule.
+//
+// The rows of a dense gradient that no lookup names are filled with zeros by other CTAs of the same launch, which
+// find the named ones in the sorted pairs: every row is written once, and the sums, bound by
+// instructions and the L2, run beside the zeros, bound by DRAM.
 #include <climits>
+#include <cstddef>
 
 #include "eb_train.cuh"
 
@@ -21,22 +26,15 @@ namespace {
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kItems = 5;                          // pairs a thread ranks at a time
+constexpr int kItems = 9;                          // pairs a thread ranks at a time
 constexpr int kSubTile = kSortThreads * kItems;
 constexpr int kSmallItems = 7;                     // ... in the kernel that sorts all of a small call
 constexpr int kSmall = kSortThreads * kSmallItems;
-constexpr int kDigits = 256;
+constexpr int kDigits = 256;                       // at most
 constexpr int kStarts = 2048;                      // bag starts a tile keeps in shared memory
 constexpr int kRun = 32;                           // sorted lookups of a run, runs of a block of runs
 constexpr unsigned kNone = 0xffffffffu;
-
-struct ZeroSpan {          // words of grad_table that a launch fills with zeros
-  char* base;
-  long long stride;        // bytes between rows
-  long long per_row;       // words a row
-  long long begin, end;
-  int word;                // bytes: 16, 4 or 2
-};
+constexpr int kMostColumns = 1 << 24;
 
 struct BackArgs {
   // the lookups
@@ -49,6 +47,8 @@ struct BackArgs {
   int n;                  // lookups
   int num_bags;
   int fixed_len;          // 1 for GATHER: every lookup is a bag
+  unsigned fixed_magic;   // j / fixed_len = j * fixed_magic >> 31 + fixed_shift for j below 2^31
+  int fixed_shift;
   int idx64, include_last;
   int mean, mean_raw;
   // the gradients
@@ -69,22 +69,25 @@ struct BackArgs {
   int* counted;           // [num_bags]: non-padding lookups (mean with a padding index)
   uint2* pairs[2];        // [n] {row, payload}
   int by_bag;             // the payload is the bag (-1 with a row of num_rows), else the lookup
-  unsigned* hist;         // [tiles][kDigits]
+  unsigned* hist;         // [tiles][kDigits]: pairs of a tile by digit
   float* partial;         // [runs][2][pstride]: sums of a run's first row, when it began before the run,
                           // and of its last, when it began in the run and goes on
   float* super;           // [runs / 32][pstride]
   int pstride;
   int tiles, tile;        // sort tiles and lookups a tile
+  int passes, bits;       // digits of the sort and bits of a digit
   int runs;
+  // zeros
+  int zero_rows, zero_blocks;   // table rows a CTA fills, and such CTAs (0: none)
+  int word;                     // bytes of a store: 16, 4 or 2
 };
 
 __device__ __forceinline__ long long index_at(const void* p, int idx64, long long i) {
   return idx64 ? __ldg(static_cast<const long long*>(p) + i) : (long long)__ldg(static_cast<const int*>(p) + i);
 }
 
-// Row of lookup j in the table window, or num_rows where it contributes nothing.
-__device__ __forceinline__ unsigned row_of(const BackArgs& a, int j, int bag) {
-  const long long idx = index_at(a.indices, a.idx64, j);
+// Row of a lookup's index in the table window, or num_rows where it contributes nothing.
+__device__ __forceinline__ unsigned row_of(const BackArgs& a, long long idx, int bag) {
   const unsigned long long r = (unsigned long long)idx - (unsigned long long)a.row_lo;
   const bool ok = bag >= 0 && !(a.padding_idx >= 0 && idx == a.padding_idx) && r < a.num_rows;
   return ok ? (unsigned)r : a.num_rows;
@@ -113,39 +116,28 @@ __device__ __forceinline__ int upper_bound(Start start, long long j, int lo, int
   }
   return lo;
 }
-// The same over all starts by a whole CTA: every thread tests one start a round.
+// The same for two values over all starts by a whole CTA: every thread tests one start a round.
 template <int THREADS>
-__device__ __forceinline__ int upper_bound_cta(const BackArgs& a, long long j, int n) {
-  int lo = 0, len = n;
-  while (len > 0) {
-    const int step = (len + THREADS - 1) / THREADS;
-    const long long at = lo + (long long)(threadIdx.x + 1) * step - 1;
-    const int c = __syncthreads_count(at < lo + len && index_at(a.offsets, a.idx64, at) <= j);
-    const int next = lo + c * step;
-    len = min(step - 1, lo + len - next);
-    lo = next;
+__device__ __forceinline__ int2 upper_bound_cta(const BackArgs& a, long long j0, long long j1, int n) {
+  int lo0 = 0, len0 = n, lo1 = 0, len1 = n;
+  while (len0 > 0 || len1 > 0) {
+    const int step0 = (len0 + THREADS - 1) / THREADS, step1 = (len1 + THREADS - 1) / THREADS;
+    const long long at0 = lo0 + (long long)(threadIdx.x + 1) * step0 - 1;
+    const long long at1 = lo1 + (long long)(threadIdx.x + 1) * step1 - 1;
+    const bool in0 = step0 > 0 && at0 < lo0 + len0, in1 = step1 > 0 && at1 < lo1 + len1;
+    const long long v0 = in0 ? index_at(a.offsets, a.idx64, at0) : 0;
+    const long long v1 = in1 ? index_at(a.offsets, a.idx64, at1) : 0;
+    const int c0 = __syncthreads_count(in0 && v0 <= j0), c1 = __syncthreads_count(in1 && v1 <= j1);
+    const int next0 = lo0 + c0 * step0, next1 = lo1 + c1 * step1;
+    len0 = step0 > 0 ? min(step0 - 1, lo0 + len0 - next0) : 0;
+    len1 = step1 > 0 ? min(step1 - 1, lo1 + len1 - next1) : 0;
+    lo0 = next0;
+    lo1 = next1;
   }
-  return lo;
+  return make_int2(lo0, lo1);
 }
 
-__device__ __forceinline__ void zero_span(const ZeroSpan& z, int part, int parts) {
-  const long long total = z.end - z.begin;
-  const bool dense = z.per_row * z.word == z.stride;
-  for (long long k = (long long)part * blockDim.x + threadIdx.x; k < total; k += (long long)parts * blockDim.x) {
-    const long long i = z.begin + k;
-    char* q = dense ? z.base + i * z.word : z.base + (i / z.per_row) * z.stride + (i % z.per_row) * z.word;
-    if (z.word == 16) *reinterpret_cast<uint4*>(q) = make_uint4(0, 0, 0, 0);
-    else if (z.word == 4) *reinterpret_cast<unsigned*>(q) = 0;
-    else *reinterpret_cast<unsigned short*>(q) = 0;
-  }
-}
-
-__global__ void __launch_bounds__(kSortThreads) zero_kernel(const ZeroSpan z) {
-  pdl_enter();
-  zero_span(z, blockIdx.x, gridDim.x);
-}
-
-// counted[b] = length of bag b; the histogram kernel takes the padding off.
+// counted[b] = length of bag b; the kernel that makes the pairs takes the padding off.
 __global__ void __launch_bounds__(256) bag_length_kernel(const BackArgs a) {
   pdl_enter();
   const int b = blockIdx.x * 256 + threadIdx.x;
@@ -160,75 +152,149 @@ struct TileStarts {
   int lo, hi;        // the number of starts <= a lookup lies in [lo, hi]
   bool in_shared;    // starts [lo, hi) are in shared memory
 };
-__device__ __forceinline__ TileStarts find_starts(const BackArgs& a, int begin, int end, long long* shared) {
+__device__ __forceinline__ int clamp_start(long long s) { return s < 0 ? -1 : (s > INT_MAX ? INT_MAX : (int)s); }
+__device__ __forceinline__ TileStarts find_starts(const BackArgs& a, int begin, int end, int* shared) {
   TileStarts t = {0, 0, false};
   if (a.fixed_len > 0 || begin >= end) return t;
   const int n = a.num_bags > 0 ? a.num_bags + (a.include_last ? 1 : 0) : 0;
-  t.lo = upper_bound_cta<kSortThreads>(a, begin, n);
-  t.hi = max(t.lo, upper_bound_cta<kSortThreads>(a, end - 1, n));
+  const int2 found = upper_bound_cta<kSortThreads>(a, begin, end - 1, n);
+  t.lo = found.x;
+  t.hi = max(found.x, found.y);
   t.in_shared = t.hi - t.lo <= kStarts;
   if (t.in_shared) {
-    for (int i = t.lo + threadIdx.x; i < t.hi; i += kSortThreads) shared[i - t.lo] = index_at(a.offsets, a.idx64, i);
+    for (int i = t.lo + threadIdx.x; i < t.hi; i += kSortThreads)
+      shared[i - t.lo] = clamp_start(index_at(a.offsets, a.idx64, i));
     __syncthreads();
   }
   return t;
 }
-// The bag that holds lookup j: the last one that starts at or before it; -1 where there is none.
-__device__ __forceinline__ int bag_of(const BackArgs& a, int j, const TileStarts& t, const long long* shared) {
-  if (a.fixed_len > 0) {
-    const int bag = j / a.fixed_len;
-    return bag < a.num_bags ? bag : -1;
+// The bags of consecutive lookups, 32 at a time: a lane's bag is the last one that starts at or before its lookup, -1 where
+// there is none.  The warp keeps the number of starts before its lookups and looks at the next 32.
+struct BagWalk {
+  int known;         // starts <= the last lookup walked
+  template <typename Start>
+  __device__ __forceinline__ int step(const BackArgs& a, int j, const TileStarts& t, Start start) {
+    constexpr unsigned kAll = 0xffffffffu;
+    const int lane = threadIdx.x & 31;
+    const int s = known + lane < t.hi ? start(known + lane) : INT_MAX;
+    const int last = __shfl_sync(kAll, j, 31);
+    int count;
+    if (__shfl_sync(kAll, s, 31) <= last) {          // more starts than lanes (empty bags): search all of them
+      count = upper_bound(start, j, known, t.hi);
+    } else {
+      int at = 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const int v = __shfl_sync(kAll, s, at + o - 1);
+        at += v <= j ? o : 0;
+      }
+      count = known + at;
+    }
+    known = __shfl_sync(kAll, count, 31);
+    const int bag = count - 1;
+    return bag < a.num_bags ? bag : -1;              // behind the last offset of include_last_offset
   }
-  const int bag = (t.in_shared ? upper_bound([&](int i) { return shared[i - t.lo]; }, j, t.lo, t.hi)
-                               : upper_bound([&](int i) { return index_at(a.offsets, a.idx64, i); }, j, t.lo, t.hi)) - 1;
-  return bag < a.num_bags ? bag : -1;     // behind the last offset of include_last_offset
+};
+// Calls visit(i, bag) for a warp's lookups begin + 32 i + lane, ITEMS of them a lane, those at `end` and behind with -1.
+template <int ITEMS, typename Visit>
+__device__ __forceinline__ void walk_bags(const BackArgs& a, int begin, int end, const TileStarts& t, const int* shared,
+                                          BagWalk& walk, Visit visit) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int j = begin + i * 32 + lane;
+    int bag;
+    if (a.fixed_len > 0) {
+      bag = (int)(((unsigned long long)(unsigned)j * a.fixed_magic) >> (31 + a.fixed_shift));
+      if (bag >= a.num_bags) bag = -1;
+    } else if (t.in_shared) {
+      bag = walk.step(a, j, t, [&](int k) { return shared[k - t.lo]; });
+    } else {
+      bag = walk.step(a, j, t, [&](int k) { return clamp_start(index_at(a.offsets, a.idx64, k)); });
+    }
+    visit(i, j < end ? bag : -1);
+  }
 }
+__device__ __forceinline__ BagWalk walk_from(const BackArgs& a, int begin, const TileStarts& t, const int* shared) {
+  BagWalk w = {t.lo};
+  if (a.fixed_len == 0)
+    w.known = t.in_shared ? upper_bound([&](int k) { return shared[k - t.lo]; }, begin - 1, t.lo, t.hi)
+                          : upper_bound([&](int k) { return clamp_start(index_at(a.offsets, a.idx64, k)); }, begin - 1, t.lo, t.hi);
+  return w;
+}
+
 // Padding is not counted for a mean: one subtraction a warp and bag.  All lanes of the warp call it.
-__device__ __forceinline__ void uncount_padding(const BackArgs& a, int j, bool in, int bag) {
-  const bool pad = in && bag >= 0 && index_at(a.indices, a.idx64, j) == a.padding_idx;
+__device__ __forceinline__ void uncount_padding(const BackArgs& a, long long idx, bool in, int bag) {
+  const bool pad = in && bag >= 0 && idx == a.padding_idx;
   const unsigned same = __match_any_sync(0xffffffffu, pad ? bag : -1);
   if (pad && (threadIdx.x & 31) == __ffs(same) - 1) atomicSub(a.counted + bag, __popc(same));
 }
 
-// hist[tile][d] = keys of the tile whose digit is d.  FIRST: the keys are made from the indices, and
-// bag_of is written.  CTAs from `tiles` on fill their span with zeros.
-template <bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const BackArgs a, const uint2* from, int shift,
-                                                                      const ZeroSpan z) {
+// Every lookup's pair (and bag, where it is wanted apart), and the histogram of the first digit.  A warp takes consecutive
+// lookups; all its indices are asked for at once (they may come from DRAM, a microsecond and a half a round).
+__global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs a, uint2* to) {
   pdl_enter();
-  if ((int)blockIdx.x >= a.tiles) {
-    zero_span(z, blockIdx.x - a.tiles, gridDim.x - a.tiles);
-    return;
-  }
   __shared__ unsigned count[kDigits];
-  __shared__ long long starts[FIRST ? kStarts : 1];
+  __shared__ int starts[kStarts];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
   const int begin = blockIdx.x * a.tile;
   const int end = min(a.n, begin + a.tile);
-  TileStarts t = {};
-  if (FIRST) t = find_starts(a, begin, end, starts);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int share = (a.tile / 32 + kSortWarps - 1) / kSortWarps * 32;
+  const int first = begin + warp * share, last = min(end, first + share);
+  long long index[kItems];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int j = base + i * 32 + lane;
+      index[i] = j < last ? index_at(a.indices, a.idx64, j) : 0;
+    }
+  };
+  fetch(first);
+  const TileStarts t = find_starts(a, begin, end, starts);
   __syncthreads();
+  BagWalk walk = walk_from(a, first, t, starts);
+  const unsigned mask = (1u << a.bits) - 1u;
+  for (int base = first; base < last; base += kItems * 32) {
+    if (base != first) fetch(base);
+    walk_bags<kItems>(a, base, last, t, starts, walk, [&](int i, int bag) {
+      const int j = base + i * 32 + lane;
+      if (j < last) {
+        if (a.bag_of) a.bag_of[j] = bag;
+        if (to) {
+          const unsigned row = row_of(a, index[i], bag);
+          to[j] = make_uint2(row, a.by_bag ? (unsigned)bag : (unsigned)j);
+          atomicAdd(&count[row & mask], 1u);
+        }
+      }
+      if (a.counted) uncount_padding(a, index[i], j < last, bag);
+    });
+  }
+  __syncthreads();
+  if (to) {
+    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) a.hist[blockIdx.x * kDigits + d] = count[d];
+  }
+}
+
+// The histogram of a later digit.
+__global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const BackArgs a, const uint2* from, int pass) {
+  pdl_enter();
+  __shared__ unsigned count[kDigits];
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
+  __syncthreads();
+  const int begin = blockIdx.x * a.tile;
+  const int end = min(a.n, begin + a.tile);
+  const unsigned mask = (1u << a.bits) - 1u;
   for (int base = begin; base < end; base += kSubTile) {
     unsigned key[kItems];
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int j = base + i * kSortThreads + threadIdx.x;
-      key[i] = 0;
-      if (FIRST) {
-        int bag = -1;
-        if (j < end) {
-          bag = bag_of(a, j, t, starts);
-          a.bag_of[j] = bag;
-          key[i] = row_of(a, j, bag);
-        }
-        if (a.counted) uncount_padding(a, j, j < end, bag);
-      } else if (j < end) {
-        key[i] = from[j].x;
-      }
+      key[i] = j < end ? __ldg(&from[j].x) : 0;
     }
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      if (base + i * kSortThreads + (int)threadIdx.x < end) atomicAdd(&count[(key[i] >> shift) & (kDigits - 1)], 1u);
+      if (base + i * kSortThreads + (int)threadIdx.x < end) atomicAdd(&count[(key[i] >> (pass * a.bits)) & mask], 1u);
     }
   }
   __syncthreads();
@@ -239,17 +305,28 @@ __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const Back
 // in_warp[w][d] becomes the number of warp w's items with digit d.  kNone is no digit.
 template <int ITEMS>
 __device__ __forceinline__ void rank_items(const unsigned (&digit)[ITEMS], unsigned (&rank)[ITEMS],
-                                           unsigned (*in_warp)[kDigits]) {
+                                           unsigned (*in_warp)[kDigits], int bits) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&in_warp[0][0])[i] = 0;
   __syncthreads();
+  const unsigned below = (1u << lane) - 1u;
+  unsigned same[ITEMS];      // lanes with the same digit, by a vote a bit
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) same[i] = __ballot_sync(0xffffffffu, digit[i] != kNone);
+  for (int bit = 0; bit < bits; ++bit) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const bool set = (digit[i] >> bit) & 1u;
+      const unsigned vote = __ballot_sync(0xffffffffu, set);
+      same[i] &= set ? vote : ~vote;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const unsigned same = __match_any_sync(0xffffffffu, digit[i]);
     const bool in = digit[i] != kNone;
-    rank[i] = in ? in_warp[warp][digit[i]] + __popc(same & ((1u << lane) - 1u)) : 0;
+    rank[i] = in ? in_warp[warp][digit[i]] + __popc(same[i] & below) : 0;
     __syncwarp();
-    if (in && lane == __ffs(same) - 1) in_warp[warp][digit[i]] += __popc(same);
+    if (in && (same[i] & below) == 0) in_warp[warp][digit[i]] += __popc(same[i]);
     __syncwarp();
   }
   __syncthreads();
@@ -286,62 +363,65 @@ __device__ __forceinline__ unsigned digits_below(unsigned mine, unsigned* total)
   return sum - mine;
 }
 
-// Moves a tile's pairs to their place in the order of the digit, ties in the order they came.
-template <bool FIRST>
-__global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const BackArgs a, const uint2* from, uint2* to,
-                                                                    int shift, const ZeroSpan z) {
+// Moves a tile's pairs to their place in the order of digit `pass`, ties in the order they came.
+struct DigitShared {
+  uint2 pairs[kSubTile];                   // in the digit's order
+  unsigned in_warp[kSortWarps][kDigits];
+  unsigned place[kDigits];                 // next free place of a digit
+  unsigned local[kDigits];                 // first place of a digit in `pairs`
+  unsigned total[kDigits / 32];
+};
+__global__ void __launch_bounds__(kSortThreads) sort_digit_kernel(const BackArgs a, const uint2* from, uint2* to, int pass) {
   pdl_enter();
-  if ((int)blockIdx.x >= a.tiles) {
-    zero_span(z, blockIdx.x - a.tiles, gridDim.x - a.tiles);
-    return;
-  }
-  __shared__ unsigned place[kDigits];                    // next free place of a digit
-  __shared__ unsigned in_warp[kSortWarps][kDigits];
+  extern __shared__ uint4 dynamic[];
+  DigitShared& s = *reinterpret_cast<DigitShared*>(dynamic);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int begin = blockIdx.x * a.tile;
   const int end = min(a.n, begin + a.tile);
+  const int shift = pass * a.bits;
+  const unsigned mask = (1u << a.bits) - 1u;
   uint2 pair[kItems];
   auto fetch = [&](int base) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int j = base + (warp * kItems + i) * 32 + lane;
-      pair[i] = make_uint2(0, 0);
-      if (j >= end) continue;
-      if (FIRST) {
-        const int bag = a.bag_of[j];
-        pair[i] = make_uint2(row_of(a, j, bag), a.by_bag ? (unsigned)bag : (unsigned)j);
-      } else {
-        pair[i] = from[j];
-      }
+      pair[i] = j < end ? __ldg(from + j) : make_uint2(0, 0);
     }
   };
   fetch(begin);
-  // place[d] = keys with a lower digit + keys with digit d in earlier tiles: 4 digits a thread, every 8th tile
+  // place[d] = keys with a lower digit + keys with digit d in earlier tiles: 4 digits a thread, and the tiles
+  // shared among the threads of a digit, so that a thread's loads are few and all under way together
   {
-    constexpr int kColumns = kDigits / 4, kGroups = kSortThreads / kColumns;
-    const int column = threadIdx.x % kColumns, group = threadIdx.x / kColumns;
+    const int digits = (int)mask + 1, columns = digits < 4 ? 1 : digits / 4, groups = min(kSortThreads / columns, 32);
+    const int column = threadIdx.x % columns, group = threadIdx.x / columns;
     uint4 all = make_uint4(0, 0, 0, 0), before = all;
-#pragma unroll 8
-    for (int t = group; t < a.tiles; t += kGroups) {
-      const uint4 c = reinterpret_cast<const uint4*>(a.hist + t * kDigits)[column];
-      const unsigned m = t < (int)blockIdx.x ? 0xffffffffu : 0u;
-      all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
-      before.x += c.x & m, before.y += c.y & m, before.z += c.z & m, before.w += c.w & m;
-    }
-    reinterpret_cast<uint4*>(in_warp[group])[column] = all;
-    reinterpret_cast<uint4*>(in_warp[kGroups + group])[column] = before;
-    static_assert(2 * kGroups <= kSortWarps, "both sums' groups fit in_warp");
-    __syncthreads();
-    unsigned sum = 0, earlier = 0;
-    if (threadIdx.x < kDigits) {
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        sum += in_warp[g][threadIdx.x];
-        earlier += in_warp[kGroups + g][threadIdx.x];
+    if (group < groups) {
+#pragma unroll 10
+      for (int t = group; t < a.tiles; t += groups) {
+        const uint4 c = reinterpret_cast<const uint4*>(a.hist + t * kDigits)[column];
+        const unsigned m = t < (int)blockIdx.x ? 0xffffffffu : 0u;
+        all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
+        before.x += c.x & m, before.y += c.y & m, before.z += c.z & m, before.w += c.w & m;
       }
     }
-    const unsigned lower = digits_below(sum, place);
-    if (threadIdx.x < kDigits) place[threadIdx.x] = lower + earlier;
+    // scratch: `pairs`, for 2 * groups * max(digits, 4) words
+    uint4* scratch = reinterpret_cast<uint4*>(s.pairs);
+    static_assert(sizeof(s.pairs) >= 2 * 4 * kSortThreads * 4, "a uint4 a thread, twice");
+    if (group < groups) {
+      scratch[group * columns + column] = all;
+      scratch[(groups + group) * columns + column] = before;
+    }
+    __syncthreads();
+    unsigned sum = 0, earlier = 0;
+    if ((int)threadIdx.x < digits) {
+      const unsigned* words = reinterpret_cast<const unsigned*>(s.pairs);
+      for (int g = 0; g < groups; ++g) {
+        sum += words[g * columns * 4 + threadIdx.x];
+        earlier += words[(groups + g) * columns * 4 + threadIdx.x];
+      }
+    }
+    const unsigned lower = digits_below(sum, s.total);
+    if (threadIdx.x < kDigits) s.place[threadIdx.x] = lower + earlier;
     __syncthreads();
   }
   for (int base = begin; base < end; base += kSubTile) {
@@ -353,54 +433,84 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const BackAr
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int j = base + (warp * kItems + i) * 32 + lane;
-      digit[i] = j < end ? (pair[i].x >> shift) & (kDigits - 1) : kNone;
+      digit[i] = j < end ? (pair[i].x >> shift) & mask : kNone;
     }
-    rank_items<kItems>(digit, rank, in_warp);
-    place_warps(in_warp, place);
+    rank_items<kItems>(digit, rank, s.in_warp, a.bits);
+    unsigned sum = 0;
+    if (threadIdx.x < kDigits) {
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) sum += s.in_warp[w][threadIdx.x];
+    }
+    const unsigned local = digits_below(sum, s.total);
+    if (threadIdx.x < kDigits) s.local[threadIdx.x] = local;
+    __syncthreads();
+    unsigned moved = local;
+    if (threadIdx.x < kDigits) {     // in_warp: where a warp's first item of the digit goes in `pairs`
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) {
+        const unsigned c = s.in_warp[w][threadIdx.x];
+        s.in_warp[w][threadIdx.x] = moved;
+        moved += c;
+      }
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      if (digit[i] != kNone) to[in_warp[warp][digit[i]] + rank[i]] = pair[i];
+      if (digit[i] != kNone) s.pairs[s.in_warp[warp][digit[i]] + rank[i]] = pair[i];
     }
+    __syncthreads();
+    const int count = min(kSubTile, end - base);
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int k = i * kSortThreads + threadIdx.x;
+      if (k >= count) continue;
+      const uint2 p = s.pairs[k];
+      const unsigned d = (p.x >> shift) & mask;
+      to[s.place[d] + (k - s.local[d])] = p;
+    }
+    __syncthreads();
+    if (threadIdx.x < kDigits) s.place[threadIdx.x] += sum;
   }
 }
 
-// Up to kSmall lookups: CTA 0 finds the bags and does all digits in shared memory, the others fill with zeros.
-__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs a, uint2* to, int passes, const ZeroSpan z) {
+// Up to kSmall lookups: one CTA finds the bags and does all digits in shared memory.
+__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs a, uint2* to) {
   pdl_enter();
-  if (blockIdx.x > 0) {
-    zero_span(z, blockIdx.x - 1, gridDim.x - 1);
-    return;
-  }
   __shared__ unsigned place[kDigits];
   __shared__ unsigned in_warp[kSortWarps][kDigits];
-  __shared__ __align__(16) char buffer[kSmall * sizeof(uint2)];   // the starts, then the pairs between digits
-  static_assert(kSmall >= kStarts, "the starts fit");
-  long long* starts = reinterpret_cast<long long*>(buffer);
-  uint2* pairs = reinterpret_cast<uint2*>(buffer);
+  __shared__ uint2 pairs[kSmall];
   __shared__ unsigned total[kDigits / 32];
+  int* starts = reinterpret_cast<int*>(pairs);   // before the first digit
+  static_assert(sizeof(pairs) >= kStarts * sizeof(int), "the starts fit");
+  const unsigned mask = (1u << a.bits) - 1u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const TileStarts t = find_starts(a, 0, a.n, starts);
-  uint2 pair[kSmallItems];
+  const int first = warp * kSmallItems * 32;
+  long long index[kSmallItems];
 #pragma unroll
   for (int i = 0; i < kSmallItems; ++i) {
-    const int j = (warp * kSmallItems + i) * 32 + lane;
-    int bag = -1;
+    const int j = first + i * 32 + lane;
+    index[i] = j < a.n ? index_at(a.indices, a.idx64, j) : 0;
+  }
+  const TileStarts t = find_starts(a, 0, a.n, starts);
+  uint2 pair[kSmallItems];
+  BagWalk walk = walk_from(a, first, t, starts);
+  walk_bags<kSmallItems>(a, first, a.n, t, starts, walk, [&](int i, int bag) {
+    const int j = first + i * 32 + lane;
     pair[i] = make_uint2(0, 0);
     if (j < a.n) {
-      bag = bag_of(a, j, t, starts);
-      a.bag_of[j] = bag;
-      pair[i] = make_uint2(row_of(a, j, bag), a.by_bag ? (unsigned)bag : (unsigned)j);
+      if (a.bag_of) a.bag_of[j] = bag;
+      pair[i] = make_uint2(row_of(a, index[i], bag), a.by_bag ? (unsigned)bag : (unsigned)j);
     }
-    if (a.counted) uncount_padding(a, j, j < a.n, bag);
-  }
-  for (int pass = 0; pass < passes; ++pass) {
+    if (a.counted) uncount_padding(a, index[i], j < a.n, bag);
+  });
+  for (int pass = 0; pass < a.passes; ++pass) {
     unsigned digit[kSmallItems], rank[kSmallItems];
 #pragma unroll
     for (int i = 0; i < kSmallItems; ++i) {
       const int j = (warp * kSmallItems + i) * 32 + lane;
-      digit[i] = j < a.n ? (pair[i].x >> (8 * pass)) & (kDigits - 1) : kNone;
+      digit[i] = j < a.n ? (pair[i].x >> (a.bits * pass)) & mask : kNone;
     }
-    rank_items<kSmallItems>(digit, rank, in_warp);
+    rank_items<kSmallItems>(digit, rank, in_warp, a.bits);
     unsigned sum = 0;
     if (threadIdx.x < kDigits) {
 #pragma unroll
@@ -410,7 +520,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs
     if (threadIdx.x < kDigits) place[threadIdx.x] = lower;
     __syncthreads();
     place_warps(in_warp, place);
-    const bool last = pass + 1 == passes;
+    const bool last = pass + 1 == a.passes;
 #pragma unroll
     for (int i = 0; i < kSmallItems; ++i) {
       if (digit[i] == kNone) continue;
@@ -440,80 +550,241 @@ __global__ void __launch_bounds__(256) winner_bytes_kernel(const BackArgs a) {
   }
 }
 
+template <int VE>
+__device__ __forceinline__ void load_either(const char* row, int f16, int col, float (&x)[VE]) {
+  if (f16) {
+    Pack<__half, VE> r;
+    r.load(reinterpret_cast<const __half*>(row) + col);
+    r.get(x);
+  } else {
+    Pack<float, VE> r;
+    r.load(reinterpret_cast<const float*>(row) + col);
+    r.get(x);
+  }
+}
+template <int VE>
+__device__ __forceinline__ void store_either(char* row, int f16, int col, const float (&x)[VE]) {
+  if (f16) {
+    Pack<__half, VE> r;
+    r.set(x);
+    r.store(reinterpret_cast<__half*>(row) + col);
+  } else {
+    Pack<float, VE> r;
+    r.set(x);
+    r.store(reinterpret_cast<float*>(row) + col);
+  }
+}
+// row += x.  fp32 adds where the row lies, in the L2: one addition an element and call, so its order does not
+// matter, and the warp waits for nothing.  fp16 adds in fp32 and rounds once.
+template <int VE>
+__device__ __forceinline__ void add_either(char* row, int f16, int col, const float (&x)[VE]) {
+  if (f16) {
+    float old[VE];
+    load_either<VE>(row, 1, col, old);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) old[i] += x[i];
+    store_either<VE>(row, 1, col, old);
+    return;
+  }
+  float* to = reinterpret_cast<float*>(row) + col;
+  if constexpr (VE % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < VE; i += 4)
+      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                   :: "l"(to + i), "f"(x[i]), "f"(x[i + 1]), "f"(x[i + 2]), "f"(x[i + 3]) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) asm volatile("red.global.add.f32 [%0], %1;" :: "l"(to + i), "f"(x[i]) : "memory");
+  }
+}
+
+// Each nibble 8 + k of `which` makes a byte of copies of byte k's top bit.
+__device__ __forceinline__ unsigned spread_top(unsigned x, unsigned which) {
+  unsigned y;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(y) : "r"(x), "r"(which));
+  return y;
+}
+
+// acc[i] += g[i] in the columns whose byte of `won` is `at` (below 255).
+template <typename TG, int VE>
+__device__ __forceinline__ void add_won(float (&acc)[VE], const Pack<TG, VE>& g, const Pack<unsigned char, VE>& won, unsigned at) {
+  if constexpr (VE % 4 == 0) {
+    unsigned w[VE / 4], v[VE * sizeof(TG) / 4];
+    memcpy(w, won.w, sizeof(w));
+    memcpy(v, g.w, sizeof(v));
+#pragma unroll
+    for (int k = 0; k < VE / 4; ++k) {
+      const unsigned d = w[k] ^ (at * 0x01010101u);
+      const unsigned hit = ~(((d & 0x7f7f7f7fu) + 0x7f7f7f7fu) | d) & 0x80808080u;   // the top bit of each zero byte
+      if constexpr (sizeof(TG) == 2) {
+        // a byte's top bit spread over a half, and over the next
+        const unsigned lo = v[2 * k] & spread_top(hit, 0x9988), hi = v[2 * k + 1] & spread_top(hit, 0xbbaa);
+        asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(acc[4 * k]) : "h"((unsigned short)lo));
+        asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(acc[4 * k + 1]) : "h"((unsigned short)(lo >> 16)));
+        asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(acc[4 * k + 2]) : "h"((unsigned short)hi));
+        asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(acc[4 * k + 3]) : "h"((unsigned short)(hi >> 16)));
+      } else {
+        acc[4 * k] += __uint_as_float(v[4 * k] & spread_top(hit, 0x8888));
+        acc[4 * k + 1] += __uint_as_float(v[4 * k + 1] & spread_top(hit, 0x9999));
+        acc[4 * k + 2] += __uint_as_float(v[4 * k + 2] & spread_top(hit, 0xaaaa));
+        acc[4 * k + 3] += __uint_as_float(v[4 * k + 3] & spread_top(hit, 0xbbbb));
+      }
+    }
+  } else {
+    unsigned char w[VE];
+    float f[VE];
+    memcpy(w, won.w, sizeof(w));
+    g.get(f);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] += w[i] == at ? f[i] : 0.0f;
+  }
+}
+
 // Store the finished sum of a row.
 template <int VE>
 __device__ __forceinline__ void store_row(const BackArgs& a, unsigned row, int col, float (&acc)[VE]) {
+  char* to = a.grad_table + (long long)row * a.gt_stride;
   if (a.square) {
     float x[VE];
-    const char* q = a.table + (long long)row * a.table_stride;
-    if (a.table_f16) {
-      Pack<__half, VE> r;
-      r.load_ro(reinterpret_cast<const __half*>(q) + col);
-      r.get(x);
-    } else {
-      Pack<float, VE> r;
-      r.load_ro(reinterpret_cast<const float*>(q) + col);
-      r.get(x);
-    }
+    load_either<VE>(a.table + (long long)row * a.table_stride, a.table_f16, col, x);
 #pragma unroll
     for (int i = 0; i < VE; ++i) acc[i] *= 2.0f * x[i];
   }
-  char* q = a.grad_table + (long long)row * a.gt_stride;
-  if (a.gt_f16) {
-    Pack<__half, VE> r;
-    __half* to = reinterpret_cast<__half*>(q) + col;
-    if (a.accumulate) {
-      float old[VE];
-      r.load(to);
-      r.get(old);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] += old[i];
-    }
-    r.set(acc);
-    r.store(to);
-  } else {
-    Pack<float, VE> r;
-    float* to = reinterpret_cast<float*>(q) + col;
-    if (a.accumulate) {
-      float old[VE];
-      r.load(to);
-      r.get(old);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] += old[i];
-    }
-    r.set(acc);
-    r.store(to);
-  }
+  if (a.accumulate) add_either<VE>(to, a.gt_f16, col, acc);
+  else store_either<VE>(to, a.gt_f16, col, acc);
 }
 
-template <int VE>
-__device__ __forceinline__ void load_table(const BackArgs& a, unsigned row, int col, float (&x)[VE]) {
-  const char* q = a.table + (long long)row * a.table_stride;
-  if (a.table_f16) {
-    Pack<__half, VE> r;
-    r.load_ro(reinterpret_cast<const __half*>(q) + col);
-    r.get(x);
-  } else {
-    Pack<float, VE> r;
-    r.load_ro(reinterpret_cast<const float*>(q) + col);
-    r.get(x);
-  }
-}
+// kPlain adds rows, kScaled takes a factor a lookup, kWeights does so and writes grad_weights, kMax masks columns,
+// kSquare multiplies the sum by twice the table row.
+enum Kind { kPlain = 0, kScaled = 1, kWeights = 2, kMax = 3, kSquare = 4 };
 
-// kPlain adds rows, kScaled takes a factor a lookup, kWeights does so and writes grad_weights, kMax masks columns.
-enum Kind { kPlain = 0, kScaled = 1, kWeights = 2, kMax = 3 };
-
-// A warp per run of 32 sorted lookups; blockIdx.y is a tile of 32 * VE columns.
-template <typename TG, int VE, int KIND>
-__global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
-  pdl_enter();
-  constexpr int U = VE == 8 && KIND != kPlain && KIND != kScaled ? 4 : 8;   // lookups whose loads are issued together
+// The first pair whose row is >= each of two rows, by a warp: 32 probes a round.
+__device__ __forceinline__ int2 find_rows(const uint2* pairs, int n, unsigned row0, unsigned row1) {
   constexpr unsigned kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
-  const int run = blockIdx.x * 8 + (threadIdx.x >> 5);
+  int lo0 = 0, len0 = n, lo1 = 0, len1 = n;
+  while (len0 > 0 || len1 > 0) {
+    const int step0 = (len0 + 31) / 32, step1 = (len1 + 31) / 32;
+    const long long at0 = lo0 + (lane + 1LL) * step0 - 1, at1 = lo1 + (lane + 1LL) * step1 - 1;
+    const bool in0 = step0 > 0 && at0 < lo0 + len0, in1 = step1 > 0 && at1 < lo1 + len1;
+    const unsigned v0 = in0 ? __ldg(&pairs[at0].x) : kNone, v1 = in1 ? __ldg(&pairs[at1].x) : kNone;
+    const int c0 = __popc(__ballot_sync(kAll, in0 && v0 < row0)), c1 = __popc(__ballot_sync(kAll, in1 && v1 < row1));
+    const int next0 = lo0 + c0 * step0, next1 = lo1 + c1 * step1;
+    len0 = step0 > 0 ? min(step0 - 1, lo0 + len0 - next0) : 0;
+    len1 = step1 > 0 ? min(step1 - 1, lo1 + len1 - next1) : 0;
+    lo0 = next0;
+    lo1 = next1;
+  }
+  return make_int2(lo0, lo1);
+}
+
+// Fills the rows of a block of the table that no lookup names with zeros.
+constexpr int kZeroRows = 1024;      // at most, of a block
+__device__ __forceinline__ void zero_block(const BackArgs& a, const uint2* pairs, int block) {
+  __shared__ unsigned named[kZeroRows / 32];
+  __shared__ int2 span;
+  const long long first = (long long)block * a.zero_rows;
+  const int rows = (int)min((long long)a.zero_rows, a.num_rows - first);
+  for (int i = threadIdx.x; i < kZeroRows / 32; i += blockDim.x) named[i] = 0;
+  if (threadIdx.x < 32) {
+    const int2 found = find_rows(pairs, a.n, (unsigned)first, (unsigned)(first + rows));
+    if (threadIdx.x == 0) span = found;
+  }
+  __syncthreads();
+  // A lane looks at 32 pairs by their ends: one row's lookups (a popular row has thousands of such) need one mark; the
+  // warp goes through the others together.
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  auto mark = [&](unsigned row) {
+    const unsigned k = row - (unsigned)first;
+    atomicOr(&named[k >> 5], 1u << (k & 31));
+  };
+  for (int base = span.x + (threadIdx.x >> 5) * 1024; base < span.y; base += warps * 1024) {
+    const int from = base + lane * 32, to = min(from + 32, span.y);
+    unsigned row = kNone;
+    bool mixed = false;
+    if (from < to) {
+      row = __ldg(&pairs[from].x);
+      mixed = __ldg(&pairs[to - 1].x) != row;
+      if (!mixed) mark(row);
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, mixed); left != 0;) {
+      unsigned rows4[4];
+      bool in[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        in[u] = false;
+        if (left == 0) continue;
+        const int i = base + (__ffs(left) - 1) * 32 + lane;
+        left &= left - 1;
+        in[u] = i < span.y;
+        if (in[u]) rows4[u] = __ldg(&pairs[i].x);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (in[u]) mark(rows4[u]);
+      }
+    }
+  }
+  __syncthreads();
+  const int per_row = a.dim * (a.gt_f16 ? 2 : 4) / a.word;      // stores a row
+  int shift = 5;                                                // a warp's lanes share 1, 2, 4, ... rows
+  while (shift > 0 && (1 << (shift - 1)) >= per_row) --shift;
+  const int at = lane & ((1 << shift) - 1), sub = lane >> shift, together = 32 >> shift;
+  char* base = a.grad_table + first * a.gt_stride;
+  if (a.word == 16 && per_row <= 1 << shift && at < per_row) {
+    // a store a lane and row: 32 rows of one mark word at a time
+    for (int g = threadIdx.x >> 5; g * 32 < rows; g += warps) {
+      const unsigned word = named[g];
+      const int most = min(32, rows - g * 32);
+      char* to = base + (long long)(g * 32 + sub) * a.gt_stride + at * 16;
+#pragma unroll 4
+      for (int r = sub; r < most; r += together, to += together * a.gt_stride) {
+        if (!(word >> r & 1u)) *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+  for (int r = (threadIdx.x >> 5) * together + sub; r < rows; r += warps * together) {
+    if (named[r >> 5] >> (r & 31) & 1u) continue;
+    char* to = base + r * a.gt_stride;
+    for (int w = at; w < per_row; w += 1 << shift) {
+      if (a.word == 16) reinterpret_cast<uint4*>(to)[w] = make_uint4(0, 0, 0, 0);
+      else if (a.word == 4) reinterpret_cast<unsigned*>(to)[w] = 0;
+      else reinterpret_cast<unsigned short*>(to)[w] = 0;
+    }
+  }
+}
+__global__ void __launch_bounds__(256) zero_kernel(const BackArgs a) {     // no lookups at all
+  pdl_enter();
+  zero_block(a, nullptr, blockIdx.x);
+}
+
+// A warp per run of 32 sorted lookups and tile of 32 * VE columns.  The CTAs that fill with zeros are spread evenly
+// among those that add.  ACC: what grad_table holds is added.
+// A table row that is wanted is read with the loads of the row's first lookup, so that no load is waited for alone.
+template <typename TG, int VE, int KIND, bool ACC>
+__global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
+  pdl_enter();
+  int cta = blockIdx.x;
+  if (!ACC && a.zero_blocks > 0) {
+    const int before = (int)((long long)cta * a.zero_blocks / gridDim.x);        // zero CTAs among the earlier ones
+    if ((int)((long long)(cta + 1) * a.zero_blocks / gridDim.x) != before) {
+      zero_block(a, pairs, before);
+      return;
+    }
+    cta -= before;
+  }
+  const int of_run = (a.runs + 7) / 8;          // CTAs a tile of columns
+  const int tile = cta / of_run;
+  cta -= tile * of_run;
+  constexpr bool kTable = KIND == kWeights || KIND == kSquare;
+  constexpr int U = kTable || VE == 8 ? 4 : 8;   // lookups whose loads are issued together
+  constexpr unsigned kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  const int run = cta * 8 + (threadIdx.x >> 5);
   if (run >= a.runs) return;
   const int base = run * kRun;
-  const int col = (blockIdx.y * 32 + lane) * VE;
+  const int col = (tile * 32 + lane) * VE;
   const bool col_ok = col < a.dim;
   uint2 pair = make_uint2(a.num_rows, 0);
   if (base + lane < a.n) pair = pairs[base + lane];
@@ -543,83 +814,106 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
       if (e - s >= 256) pos |= INT_MIN;      // compare whole positions
     }
   }
+  const unsigned left_row = __shfl_up_sync(kAll, pair.x, 1);
+  // lookups at which a row begins (the run's first always counts)
+  const unsigned heads = __ballot_sync(kAll, lane == 0 || (lane < valid && pair.x != left_row));
   float acc[VE];
+  float x[kTable ? VE : 1];     // the running row of the table
 #pragma unroll
   for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
-  unsigned row = __shfl_sync(kAll, pair.x, 0);
-  bool began_before = row == prev;
+  bool began_before = __shfl_sync(kAll, pair.x, 0) == prev;
 
-  auto put = [&](bool goes_on) {
-    if (!col_ok) return;
-    if (!began_before && !goes_on) {
-      store_row<VE>(a, row, col, acc);
-    } else {
-      Pack<float, VE> r;
-      r.set(acc);
-      r.store(a.partial + ((long long)run * 2 + (began_before ? 0 : 1)) * a.pstride + col);
+  auto put = [&](int last, bool goes_on) {         // the row whose last lookup here is `last` is done
+    const unsigned row = __shfl_sync(kAll, pair.x, last);
+    if (col_ok) {
+      if (!began_before && !goes_on) {
+        if constexpr (KIND == kSquare) {
+#pragma unroll
+          for (int i = 0; i < VE; ++i) acc[i] *= 2.0f * x[i];
+        }
+        char* to = a.grad_table + (long long)row * a.gt_stride;
+        if constexpr (ACC) add_either<VE>(to, a.gt_f16, col, acc);
+        else store_either<VE>(to, a.gt_f16, col, acc);
+      } else {
+        Pack<float, VE> r;
+        r.set(acc);
+        r.store(a.partial + ((long long)run * 2 + (began_before ? 0 : 1)) * a.pstride + col);
+      }
     }
+    began_before = false;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
   };
-  float x[KIND == kWeights ? VE : 1];     // the table row of the running segment
   for (int e0 = 0; e0 < valid; e0 += U) {
     Pack<TG, VE> g[U];
-    Pack<unsigned char, VE> won[KIND == kMax ? U : 1];
-    float xs[KIND == kWeights ? U : 1][KIND == kWeights ? VE : 1];
+    [[maybe_unused]] Pack<unsigned char, VE> won[KIND == kMax ? U : 1];
+    [[maybe_unused]] float xs[kTable ? U : 1][kTable ? VE : 1];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int b = __shfl_sync(kAll, bag, e0 + u);
-      const unsigned r = __shfl_sync(kAll, pair.x, e0 + u);
-      const unsigned before = __shfl_sync(kAll, pair.x, (e0 + u - 1) & 31);
+      const bool in = e0 + u < valid && col_ok;
       g[u].zero();
-      if (e0 + u < valid && col_ok) {
-        g[u].load_ro(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
-        if constexpr (KIND == kMax) won[u].load_ro(a.won + (long long)b * a.pstride + col);
-        if constexpr (KIND == kWeights) {   // a segment's first lookup in the run brings the row
-          if (e0 + u == 0 || r != before) load_table<VE>(a, r, col, xs[u]);
-        }
+      if (in) g[u].load_ro(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
+      if constexpr (KIND == kMax) {
+        won[u].zero();
+        if (in) won[u].load_ro(a.won + (long long)b * a.pstride + col);
+      }
+      if constexpr (kTable) {
+        const unsigned r = __shfl_sync(kAll, pair.x, e0 + u);
+        if (in && (heads >> (e0 + u) & 1u)) load_either<VE>(a.table + (long long)r * a.table_stride, a.table_f16, col, xs[u]);
       }
     }
-    float dot[KIND == kWeights ? U : 1];
+    [[maybe_unused]] float dot[KIND == kWeights ? U : 1];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const unsigned r = __shfl_sync(kAll, pair.x, e0 + u);
-      const float c = __shfl_sync(kAll, coef, e0 + u);
-      const int at = __shfl_sync(kAll, pos, e0 + u);
       if constexpr (KIND == kWeights) dot[u] = 0.0f;
       if (e0 + u >= valid) continue;
-      const bool starts = e0 + u == 0 || r != row;
-      if (r != row) {
-        put(false);
-        row = r;
-        began_before = false;
+      if (heads >> (e0 + u) & 1u) {
+        if (e0 + u > 0) put(e0 + u - 1, false);
+        if constexpr (kTable) {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
+          for (int i = 0; i < VE; ++i) x[i] = xs[u][i];
+        }
+      }
+      if constexpr (KIND == kMax) {
+        const int at = __shfl_sync(kAll, pos, e0 + u);
+        if (at >= 0) {
+          add_won<TG, VE>(acc, g[u], won[u], (unsigned)at);
+        } else {
+          const int b = __shfl_sync(kAll, bag, e0 + u);
+          float f[VE];
+          g[u].get(f);
+          if (col_ok) {
+            for (int i = 0; i < VE; ++i) {
+              if (__ldg(&a.winners[(long long)b * a.win_stride + col + i].y) == (at & INT_MAX)) acc[i] += f[i];
+            }
+          }
+        }
+        continue;
       }
       float f[VE];
       g[u].get(f);
       if constexpr (KIND == kWeights) {
-        if (starts) {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) x[i] = xs[u][i];
-        }
         if (col_ok) {
 #pragma unroll
           for (int i = 0; i < VE; ++i) dot[u] = fmaf(f[i], x[i], dot[u]);
         }
       }
-      if constexpr (KIND == kMax) {
-        unsigned char w[VE];
-        memcpy(w, won[u].w, sizeof(w));
-        const int b = __shfl_sync(kAll, bag, e0 + u);
+      if constexpr (KIND == kScaled || KIND == kWeights) {
+        const float c = __shfl_sync(kAll, coef, e0 + u);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          bool mine = w[i] == (unsigned char)at;
-          if (at < 0 && mine && col_ok)
-            mine = __ldg(&a.winners[(long long)b * a.win_stride + col + i].y) == (at & 0x7fffffff);
-          acc[i] += mine ? f[i] : 0.0f;
+        for (int i = 0; i + 1 < VE; i += 2) {
+          const float2 t = fma2(both(c), make_float2(f[i], f[i + 1]), make_float2(acc[i], acc[i + 1]));
+          acc[i] = t.x, acc[i + 1] = t.y;
         }
+        if (VE == 1) acc[0] = fmaf(c, f[0], acc[0]);
       } else {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) acc[i] = KIND == kPlain ? acc[i] + f[i] : fmaf(c, f[i], acc[i]);
+        for (int i = 0; i + 1 < VE; i += 2) {
+          const float2 t = add2(make_float2(f[i], f[i + 1]), make_float2(acc[i], acc[i + 1]));
+          acc[i] = t.x, acc[i + 1] = t.y;
+        }
+        if (VE == 1) acc[0] += f[0];
       }
     }
     if constexpr (KIND == kWeights) {
@@ -641,13 +935,13 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
           dot[0] += __shfl_xor_sync(kAll, dot[0], o);
         }
       }
-      constexpr int kShift = U == 8 ? 2 : 3;      // lanes that share a value: 2^kShift
-      const int u = lane >> kShift;
+      static_assert(U == 4, "8 lanes share a value");
+      const int u = lane >> 3;
       const unsigned j = __shfl_sync(kAll, pair.y, e0 + u);
-      if ((lane & ((1 << kShift) - 1)) == 0 && e0 + u < valid) a.grad_weights[j] = dot[0];
+      if ((lane & 7) == 0 && e0 + u < valid) a.grad_weights[j] = dot[0];
     }
   }
-  put(row == next);
+  put(valid - 1, __shfl_sync(kAll, pair.x, valid - 1) == next);
 }
 
 __device__ __forceinline__ unsigned first_row(const uint2* pairs, int run) { return pairs[run * kRun].x; }
@@ -711,10 +1005,14 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
       if (same != 0xffffffffu) {
         last = run + __ffs(~same) - 1;
       } else {
-        int lo = run + 32, hi = a.runs - 1;    // the last run that starts with the row
-        while (lo < hi) {
-          const int mid = hi - (hi - lo) / 2;
-          if (first_row(pairs, mid) == row) lo = mid; else hi = mid - 1;
+        int lo = run + 32, len = a.runs - 1 - lo;    // the last run that starts with the row: 32 probes a round
+        while (len > 0) {
+          const int step = (len + 31) / 32;
+          const long long at = lo + (lane + 1LL) * step;
+          const bool mine = at <= (long long)lo + len && first_row(pairs, (int)at) == row;
+          const int c = __popc(__ballot_sync(0xffffffffu, mine));
+          len = min(step - 1, len - c * step);
+          lo += c * step;
         }
         last = lo;
       }
@@ -742,19 +1040,20 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
       for (int i = 0; i < VE; ++i) acc[k][i] = 0.0f;
     }
     if (!col_ok) return;
-    for (int i0 = begin; i0 < end; i0 += 4) {
-      Pack<float, VE> p[4];
+    constexpr int kTogether = VE == 8 ? 4 : 8;
+    for (int i0 = begin; i0 < end; i0 += kTogether) {
+      Pack<float, VE> p[kTogether];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kTogether; ++u) {
         p[u].zero();
         if (i0 + u < end) p[u].load(piece(i0 + u) + col);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kTogether; ++u) {
         float f[VE];
         p[u].get(f);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) acc[u][i] += f[i];
+        for (int i = 0; i < VE; ++i) acc[u & 3][i] += f[i];
       }
     }
 #pragma unroll
@@ -766,16 +1065,14 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
     if (!a.super || b1 <= b0) return 1 + to - first + 1;
     return 1 + (b0 * kRun - first) + (b1 - b0) + (to + 1 - b1 * kRun);
   };
-  if (last >= 0) {
-    const int pieces = count_pieces(run, last);
-    if (pieces <= kFewPieces) {
-      add_pieces(run, last, 0, pieces);
-      if (col_ok) store_row<VE>(a, pairs[run * kRun + kRun - 1].x, col, acc[0]);
-      last = -1;
-    }
+  const int mine = last >= 0 ? count_pieces(run, last) : 0;
+  if (lane == 0) last_run[warp] = mine > kFewPieces ? last : -1;
+  const bool shared_work = __syncthreads_or(mine > kFewPieces);
+  if (mine > 0 && mine <= kFewPieces) {
+    add_pieces(run, last, 0, mine);
+    if (col_ok) store_row<VE>(a, pairs[run * kRun + kRun - 1].x, col, acc[0]);
   }
-  if (lane == 0) last_run[warp] = last;
-  if (__syncthreads_or(last >= 0) == 0) return;
+  if (!shared_work) return;
   for (int w = 0; w < 8; ++w) {
     const int to = last_run[w];
     if (to < 0) continue;              // the same for the whole CTA
@@ -808,7 +1105,7 @@ __global__ void __launch_bounds__(256) weight_gradient_kernel(const BackArgs a) 
   const long long step = (long long)gridDim.x * 8;
   for (long long j = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); j < a.n; j += step) {
     const int bag = a.bag_of[j];
-    const unsigned row = row_of(a, (int)j, bag);
+    const unsigned row = row_of(a, index_at(a.indices, a.idx64, j), bag);
     float s = 0.0f;
     if (row < a.num_rows) {
       const TG* g = reinterpret_cast<const TG*>(a.grad_out + (long long)bag * a.go_stride);
@@ -835,7 +1132,6 @@ __global__ void __launch_bounds__(256) weight_gradient_kernel(const BackArgs a) 
 
 struct BackPlan {
   BackArgs a;
-  int passes;                // of the sort, a digit each
   int ve;                    // columns a lane
   bool want_table;
   bool fused_weights;        // grad_weights comes out of the segment sum
@@ -854,6 +1150,7 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
   if (p->flags & ~(uint32_t)FWD_EB_BACKWARD_ACCUMULATE) return fail(FWD_EB_EINVAL, "unknown flags %u", p->flags);
   if (f.num_indices > INT_MAX - 65536 || f.num_bags > INT_MAX - 65536)
     return fail(FWD_EB_ETOOBIG, "the gradient takes fewer than 2^31 - 65536 indices and bags");
+  if (f.dim > kMostColumns) return fail(FWD_EB_ETOOBIG, "the gradient takes rows of up to 2^24 columns");
   const bool gather = f.mode == FWD_EB_MODE_GATHER;
   if (p->grad_out_dtype != FWD_EB_F32 && p->grad_out_dtype != FWD_EB_F16)
     return fail(FWD_EB_EINVAL, "unknown grad_out_dtype %d", p->grad_out_dtype);
@@ -922,15 +1219,30 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
   pl->ve = 1;
   for (int ve = 2; ve <= (ge == 2 ? 8 : 4) && pl->ve * 32 < f.dim && fits(ve); ve *= 2) pl->ve = ve;
 
-  pl->passes = 1;
-  while (pl->passes < 4 && (a.num_rows >> (8 * pl->passes)) != 0) ++pl->passes;   // num_rows itself is a key
+  int bits = 1;
+  while (bits < 32 && (a.num_rows >> bits) != 0) ++bits;     // num_rows itself is a key
+  a.passes = (bits + 7) / 8;
+  a.bits = (bits + a.passes - 1) / a.passes;
   const long long per = ((long long)a.n + sm_count() - 1) / sm_count();
   a.tile = (int)(per < 1024 ? 1024 : (per + 31) / 32 * 32);
   a.tiles = (int)(((long long)a.n + a.tile - 1) / a.tile);
   a.runs = (int)(((long long)a.n + kRun - 1) / kRun);
   a.pstride = (f.dim + 7) / 8 * 8;
   pl->fused_weights = pl->want_table && a.grad_weights && f.dim <= 32 * pl->ve;
+  if (a.fixed_len > 0) {
+    while ((1LL << a.fixed_shift) < a.fixed_len) ++a.fixed_shift;
+    a.fixed_magic = (unsigned)(((1ull << (31 + a.fixed_shift)) + a.fixed_len - 1) / a.fixed_len);
+  }
+  if (pl->want_table && !a.accumulate) {   // about 128 KB a CTA
+    const long long row_bytes = (long long)f.dim * (int64_t)te;
+    a.word = aligned_to(a.grad_table, 16) && a.gt_stride % 16 == 0 && row_bytes % 16 == 0 ? 16 : (int)te;
+    const long long rows = (128 * 1024 + row_bytes - 1) / row_bytes;
+    a.zero_rows = (int)(rows > kZeroRows ? kZeroRows : rows);
+    const long long blocks = (f.num_rows + a.zero_rows - 1) / a.zero_rows;
+    a.zero_blocks = (int)blocks;
+  }
   a.by_bag = !a.winners && !a.psw && !pl->fused_weights;
+  const bool bags_apart = !a.by_bag || (a.grad_weights && !pl->fused_weights);
 
   // scratch, each part on a 256-byte border
   size_t at = 0;
@@ -941,13 +1253,14 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
   };
   char* ws = static_cast<char*>(p->workspace);
   const size_t n = (size_t)a.n;
-  a.bag_of = reinterpret_cast<int*>(ws + take(n * 4));
+  const size_t bag = take(bags_apart ? n * 4 : 0);
+  a.bag_of = bags_apart ? reinterpret_cast<int*>(ws + bag) : nullptr;
   const bool count = a.mean && !a.mean_raw && a.padding_idx >= 0;
   const size_t counted = take(count ? (size_t)a.num_bags * 4 : 0);
   a.counted = count ? reinterpret_cast<int*>(ws + counted) : nullptr;
   if (pl->want_table) {
     a.pairs[0] = reinterpret_cast<uint2*>(ws + take(n * 8));
-    a.pairs[1] = reinterpret_cast<uint2*>(ws + take(pl->passes > 1 ? n * 8 : 0));
+    a.pairs[1] = reinterpret_cast<uint2*>(ws + take(n * 8));
     a.hist = reinterpret_cast<unsigned*>(ws + take((size_t)a.tiles * kDigits * 4));
     a.partial = reinterpret_cast<float*>(ws + take((size_t)a.runs * 2 * a.pstride * 4));
     const int blocks = a.runs / kRun;
@@ -955,27 +1268,37 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
     a.super = blocks > 1 ? reinterpret_cast<float*>(ws + super) : nullptr;
     a.won = reinterpret_cast<unsigned char*>(ws + take(a.winners ? (size_t)a.num_bags * a.pstride : 0));
   } else {
-    a.hist = reinterpret_cast<unsigned*>(ws + take((size_t)a.tiles * kDigits * 4));
+    a.passes = 0;
   }
   pl->bytes = a.n > 0 ? at : 0;
   return 0;
 }
 
-#define FWD_EB_TRY(call)                 \
+#define FWD_EB_TRY(...)                  \
   do {                                   \
-    cudaError_t e_ = (call);             \
+    cudaError_t e_ = (__VA_ARGS__);      \
     if (e_ != cudaSuccess) return e_;    \
   } while (0)
+
+template <typename TG, int VE, bool ACC>
+cudaError_t launch_sums(const BackPlan& pl, dim3 grid, const uint2* sorted, cudaStream_t st) {
+  const BackArgs& a = pl.a;
+  if (a.winners) return launch_pdl(segment_sum_kernel<TG, VE, kMax, ACC>, grid, 256, 0, st, a, sorted);
+  if (a.square) return launch_pdl(segment_sum_kernel<TG, VE, kSquare, ACC>, grid, 256, 0, st, a, sorted);
+  if (pl.fused_weights) return launch_pdl(segment_sum_kernel<TG, VE, kWeights, ACC>, grid, 256, 0, st, a, sorted);
+  if (a.psw || a.mean) return launch_pdl(segment_sum_kernel<TG, VE, kScaled, ACC>, grid, 256, 0, st, a, sorted);
+  return launch_pdl(segment_sum_kernel<TG, VE, kPlain, ACC>, grid, 256, 0, st, a, sorted);
+}
 
 template <typename TG, int VE>
 cudaError_t launch_segments(const BackPlan& pl, const uint2* sorted, cudaStream_t st) {
   const BackArgs& a = pl.a;
   const unsigned tiles = (unsigned)((a.dim + 32 * VE - 1) / (32 * VE));
   const dim3 grid((unsigned)((a.runs + 7) / 8), tiles);
-  if (a.winners) FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kMax>, grid, 256, 0, st, a, sorted));
-  else if (pl.fused_weights) FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kWeights>, grid, 256, 0, st, a, sorted));
-  else if (a.psw || a.mean) FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kScaled>, grid, 256, 0, st, a, sorted));
-  else FWD_EB_TRY(launch_pdl(segment_sum_kernel<TG, VE, kPlain>, grid, 256, 0, st, a, sorted));
+  const long long ctas = (long long)grid.x * tiles + a.zero_blocks;
+  if (ctas > INT_MAX) return cudaErrorInvalidConfiguration;
+  const dim3 sums((unsigned)ctas);
+  FWD_EB_TRY(a.accumulate ? launch_sums<TG, VE, true>(pl, sums, sorted, st) : launch_sums<TG, VE, false>(pl, sums, sorted, st));
   if (a.super) {
     const dim3 blocks((unsigned)((a.runs / kRun + 7) / 8), tiles);
     FWD_EB_TRY(launch_pdl(segment_block_kernel<VE>, blocks, 256, 0, st, a, sorted));
@@ -1009,41 +1332,9 @@ cudaError_t launch_weights(const BackPlan& pl, cudaStream_t st) {
   }
 }
 
-// The zeros of a dense gradient, in as many equal spans as there are launches to carry them.
-struct Zeros {
-  ZeroSpan z;
-  long long words;
-  int spans, done;
-  Zeros(const BackPlan& pl, int spans_) : z(), words(0), spans(spans_), done(0) {
-    const BackArgs& a = pl.a;
-    if (!pl.want_table || a.accumulate) return;
-    const long long row_bytes = (long long)a.dim * (a.gt_f16 ? 2 : 4);
-    const bool wide = aligned_to(a.grad_table, 16) && a.gt_stride % 16 == 0 && row_bytes % 16 == 0;
-    z.word = wide ? 16 : (a.gt_f16 ? 2 : 4);
-    z.base = a.grad_table;
-    z.stride = a.gt_stride;
-    z.per_row = row_bytes / z.word;
-    words = z.per_row * a.num_rows;
-  }
-  ZeroSpan next() {
-    z.begin = words * done / spans;
-    ++done;
-    z.end = words * done / spans;
-    return z;
-  }
-  // CTAs that fill a span beside a sort's: two an SM, fewer for little
-  unsigned ctas() const {
-    const long long most = 2LL * sm_count(), want = (words / spans + 4 * kSortThreads) / (4 * kSortThreads);
-    return words == 0 ? 0u : (unsigned)(want < most ? want : most);
-  }
-};
-
 cudaError_t launch_backward(const BackPlan& pl, const fwd_eb_backward_params* p, cudaStream_t st) {
   const BackArgs& a = pl.a;
-  const bool small = a.n <= kSmall;
-  Zeros zeros(pl, a.n == 0 || small || !pl.want_table ? 1 : 2 * pl.passes);
-  const unsigned zc = zeros.ctas();
-  if (a.n == 0) return zc == 0 ? cudaSuccess : launch_pdl(zero_kernel, dim3(zc), kSortThreads, 0, st, zeros.next());
+  if (a.n == 0) return a.zero_blocks > 0 ? launch_pdl(zero_kernel, dim3((unsigned)a.zero_blocks), 256, 0, st, a) : cudaSuccess;
   if (a.counted && a.num_bags > 0)
     FWD_EB_TRY(launch_pdl(bag_length_kernel, dim3((unsigned)((a.num_bags + 255) / 256)), 256, 0, st, a));
   if (pl.want_table && a.winners) {
@@ -1051,20 +1342,19 @@ cudaError_t launch_backward(const BackPlan& pl, const fwd_eb_backward_params* p,
     if (blocks > 0)
       FWD_EB_TRY(launch_pdl(winner_bytes_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, st, a));
   }
-  const dim3 tiles((unsigned)a.tiles + zc);
-  const uint2* none = nullptr;
   int now = 0;
-  if (small && pl.want_table) {
-    FWD_EB_TRY(launch_pdl(sort_small_kernel, dim3(1 + zc), kSortThreads, 0, st, a, a.pairs[0], pl.passes, zeros.next()));
+  if (a.n <= kSmall && pl.want_table) {
+    FWD_EB_TRY(launch_pdl(sort_small_kernel, dim3(1), kSortThreads, 0, st, a, a.pairs[0]));
   } else {
-    FWD_EB_TRY(launch_pdl(sort_histogram_kernel<true>, tiles, kSortThreads, 0, st, a, none, 0, zeros.next()));
-    if (pl.want_table)
-      FWD_EB_TRY(launch_pdl(sort_scatter_kernel<true>, tiles, kSortThreads, 0, st, a, none, a.pairs[0], 0, zeros.next()));
-    for (int pass = 1; pass < pl.passes && pl.want_table; ++pass, now ^= 1) {
+    const dim3 tiles((unsigned)a.tiles);
+    uint2* first = pl.want_table ? a.pairs[1] : nullptr;
+    FWD_EB_TRY(launch_pdl(make_pairs_kernel, tiles, kSortThreads, 0, st, a, first));
+    now = 1;
+    for (int pass = 0; pass < a.passes; ++pass, now ^= 1) {
       const uint2* from = a.pairs[now];
-      FWD_EB_TRY(launch_pdl(sort_histogram_kernel<false>, tiles, kSortThreads, 0, st, a, from, pass * 8, zeros.next()));
-      FWD_EB_TRY(launch_pdl(sort_scatter_kernel<false>, tiles, kSortThreads, 0, st, a, from, a.pairs[now ^ 1], pass * 8,
-                            zeros.next()));
+      if (pass > 0) FWD_EB_TRY(launch_pdl(sort_histogram_kernel, tiles, kSortThreads, 0, st, a, from, pass));
+      FWD_EB_TRY(allow_shared<sort_digit_kernel, (int)sizeof(DigitShared)>());
+      FWD_EB_TRY(launch_pdl(sort_digit_kernel, tiles, kSortThreads, sizeof(DigitShared), st, a, from, a.pairs[now ^ 1], pass));
     }
   }
   if (a.grad_weights && !pl.fused_weights) {

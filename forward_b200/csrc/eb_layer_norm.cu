@@ -10,7 +10,6 @@
 //
 // Rows that do not fit the registers of a CTA take the *_loop kernels, which read them again for
 // each pass.
-#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -620,23 +619,10 @@ NormPlan plan_norm(const fwd_eb_layer_norm_params* p, bool backward) {
   return pl;
 }
 
-// Launches a kernel that takes up to MOST bytes of dynamic shared memory; more than the default 48 KB (what is
-// static counts too) has to be allowed once a device.
 template <auto KERNEL, int MOST>
 cudaError_t launch_ring(dim3 grid, int threads, int bytes, cudaStream_t st, const NormArgs& a) {
-  if (MOST > 40 * 1024) {
-    static std::atomic<uint64_t> allowed{0};   // a bit a device
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return e;
-    const uint64_t bit = device < 64 ? 1ull << device : 0;
-    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-      e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
-      if (e != cudaSuccess) return e;
-      allowed.fetch_or(bit, std::memory_order_relaxed);
-    }
-  }
-  return launch_pdl(KERNEL, grid, threads, (size_t)bytes, st, a);
+  cudaError_t e = allow_shared<KERNEL, MOST>();
+  return e == cudaSuccess ? launch_pdl(KERNEL, grid, threads, (size_t)bytes, st, a) : e;
 }
 
 template <typename T, int VEC, int TPR>

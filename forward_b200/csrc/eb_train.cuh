@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -38,6 +39,22 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, int threads, 
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
   count_launch();
   return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+// Lets a kernel take up to BYTES of dynamic shared memory; more than the default 48 KB (what is static counts
+// too) has to be allowed once a device.
+template <auto KERNEL, int BYTES>
+inline cudaError_t allow_shared() {
+  if (BYTES <= 40 * 1024) return cudaSuccess;
+  static std::atomic<uint64_t> allowed{0};   // a bit a device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+  if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 inline int dtype_size(int dtype) { return dtype == FWD_EB_F32 ? 4 : 2; }

@@ -86,6 +86,7 @@ def test_struct_mirrors():
     (dict(fwd_flags=capi.FLAG_OFFSET_PAIRS), capi.EUNSUPPORTED),
     (dict(fwd_num_indices=2**31 - 1), capi.ETOOBIG),
     (dict(fwd_num_rows=2**31), capi.ETOOBIG),
+    (dict(fwd_dim=2**24 + 1), capi.ETOOBIG),
     (dict(fwd_offsets=None), capi.EINVAL),
     (dict(fwd_fixed_len=7), capi.EINVAL),
     (dict(grad_out=0x10001), capi.EALIGN),
@@ -105,7 +106,7 @@ def test_backward_workspace():
     need = lib.fwd_eb_backward_workspace_size(C.byref(_back()))
     n, dim = 4000, 128
     runs = n // 32
-    assert need >= n * 4 + n * 16 + runs * 2 * dim * 4
+    assert need >= n * 16 + runs * 2 * dim * 4
     assert lib.fwd_eb_backward_workspace_size(C.byref(_back(grad_table=None, grad_weights=0x50000))) < need
     assert lib.fwd_eb_backward_workspace_size(C.byref(_back(fwd_num_indices=0))) == 0
     assert lib.fwd_eb_backward_workspace_size(C.byref(_back(fwd_mode=77))) == 0
