@@ -8,6 +8,7 @@ Outputs (git-ignored, next to the sources so they travel with the tree):
     forward_b200/lib/libfwd_eb.so          kernels + C ABI (include/*.h)
     forward_b200/lib/libfwd_eb_plugin.so   EmbeddingBag_TRT plugin, creators and
                                            the host driver used by the tests
+    forward_b200/lib/_training_ops.so      CPython module behind forward_b200.training
 """
 from __future__ import annotations
 
@@ -171,6 +172,29 @@ def build_torch(force: bool = False, verbose: bool = False) -> str | None:
     return target
 
 
+def build_training_ops(force: bool = False, verbose: bool = False) -> str | None:
+    """The CPython module behind forward_b200.training (needs torch's C++ headers)."""
+    import sysconfig
+    try:
+        import torch
+    except ImportError:
+        return None
+    src = os.path.join(CSRC, "torch_ops", "training_ops.cpp")
+    target = os.path.join(LIBDIR, "_training_ops.so")
+    if force or _stale(target, [src] + _walk(INCLUDE, (".h",))):
+        os.makedirs(LIBDIR, exist_ok=True)
+        troot = os.path.dirname(torch.__file__)
+        tinc, tlib = os.path.join(troot, "include"), os.path.join(troot, "lib")
+        abi = int(torch.compiled_with_cxx11_abi())
+        cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", sysconfig.get_paths()["include"], "-I", tinc,
+               "-I", os.path.join(tinc, "torch", "csrc", "api", "include"), "-I", "/usr/local/cuda/include",
+               "-I", INCLUDE, "-o", target, src, "-L", tlib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+               "-lc10_cuda", "-Wl,-rpath," + tlib]
+        _run(cmd, verbose)
+    return target
+
+
 def build_tf(force: bool = False, verbose: bool = False) -> str | None:
     """The TensorFlow parser slice (own GraphDef reader: no TensorFlow needed)."""
     tdir = os.path.join(CSRC, "tf_cvt")
@@ -192,7 +216,7 @@ def build_tf(force: bool = False, verbose: bool = False) -> str | None:
 
 def build_all(force: bool = False, verbose: bool = False) -> list[str]:
     out = [build_core(force, verbose)]
-    for step in (build_plugin, build_tf, build_torch):
+    for step in (build_training_ops, build_plugin, build_tf, build_torch):
         p = step(force, verbose)
         if p:
             out.append(p)

@@ -8,7 +8,8 @@ Every result is deterministic.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
-import struct
+import importlib.util
+import os
 
 import torch
 
@@ -103,21 +104,27 @@ def _dtype(t, what: str) -> int:
     return code
 
 
-# A struct is handed over as bytes: for a call of a few microseconds, filling a ctypes.Structure field
-# by field is a third of the host's time.
-_FORMATS = {C.c_void_p: "Q", _i32: "i", _i64: "q", C.c_size_t: "Q", C.c_uint32: "I", C.c_double: "d", C.c_float: "f"}
+_OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_training_ops.so")
+_loaded_ops = None
 
 
-def _packer(cls):
-    """struct.Struct with the layout of a ctypes.Structure (nested ones flattened)."""
-    def of(c):
-        return "".join(of(t) if issubclass(t, C.Structure) else _FORMATS[t] for _, t in c._fields_)
-    packer = struct.Struct("@" + of(cls))
-    assert packer.size == C.sizeof(cls)
-    return packer.pack
-
-
-_pack_backward, _pack_norm = _packer(BackwardParams), _packer(LayerNormParams)
+def _ops():
+    """The CPython module that checks the arguments and makes the calls (csrc/torch_ops/training_ops.cpp), bound to the
+    loaded library; built first if it is not there."""
+    global _loaded_ops
+    if _loaded_ops is None:
+        if not os.path.exists(_OPS_PATH):
+            from . import build as _build
+            _build.build_training_ops()
+        spec = importlib.util.spec_from_file_location("_training_ops", _OPS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        lib = _lib()
+        module.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "fwd_eb_layer_norm_forward", "fwd_eb_layer_norm_backward", "fwd_eb_layer_norm_workspace_size",
+            "fwd_eb_backward", "fwd_eb_backward_workspace_size")))
+        _loaded_ops = module
+    return _loaded_ops
 
 
 def _device_of(names, tensors) -> int:
@@ -133,38 +140,13 @@ def _device_of(names, tensors) -> int:
     return device
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda device: torch.cuda.current_stream(device).cuda_stream)
-
-
 def _on(device: int, run, *args):
     """run(stream, *args) with the device current."""
+    stream = (_loaded_ops or _ops()).current_stream(device)
     if device == torch.cuda.current_device():
-        return run(_raw_stream(device), *args)
+        return run(stream, *args)
     with torch.cuda.device(device):
-        return run(_raw_stream(device), *args)
-
-
-def _ptr(t) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
-def _rows(t, name: str, cols: int, rows: int | None = None) -> int:
-    """Row stride of a 2-D tensor with unit column stride (0, that is `cols`, when it has at most
-    one row); raises unless it is [rows, cols]."""
-    shape = t.shape
-    if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
-        raise ValueError(f"{name} must be [{'n' if rows is None else rows}, {cols}], got {list(shape)}")
-    if shape[0] == 0:
-        return 0
-    row, col = t.stride()
-    if col != 1 and cols > 1:
-        raise ValueError(f"{name} must have unit column stride")
-    if shape[0] == 1:
-        return 0
-    if row < cols:
-        raise ValueError(f"{name}: rows overlap (row stride {row}, {cols} columns)")
-    return row
+        return run(stream, *args)
 
 
 # ---- gradient of the pooled lookup ----------------------------------------------------
@@ -190,9 +172,6 @@ def embedding_bag_winners(table, indices, offsets=None, *, fixed_len=0, include_
     return _on(device, run)
 
 
-_BACKWARD_NAMES = ("grad_out", "table", "indices", "offsets", "per_sample_weights", "winners", "grad_table")
-
-
 def embedding_bag_backward(grad_out, table, indices, offsets=None, *, mode=capi.MODE_SUM, fixed_len=0,
                            per_sample_weights=None, include_last_offset=False, padding_idx=-1, row_lo=0, flags=0,
                            winners=None, grad_table=None, grad_dtype=None, accumulate=False, need_table=True,
@@ -205,92 +184,24 @@ def embedding_bag_backward(grad_out, table, indices, offsets=None, *, mode=capi.
     table.  grad_weights is fp32, [num_indices].  What is not asked for is None.  MODE_MAX takes
     `winners` from embedding_bag_winners.
     """
-    device = _device_of(_BACKWARD_NAMES, (grad_out, table, indices, offsets, per_sample_weights, winners, grad_table))
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError("table must be 2-D with unit column stride")
-    rows, dim = table.shape
-    if not indices.is_contiguous():
-        raise ValueError("indices must be contiguous")
-    n = indices.numel()
-    gather = mode == capi.MODE_GATHER
-    if gather:
-        bags, offsets = n, None
-    elif fixed_len > 0:
-        bags, offsets = n // fixed_len, None
-    else:
-        if offsets is None:
-            raise ValueError("offsets is None and fixed_len is 0")
-        if offsets.dtype != indices.dtype or not offsets.is_contiguous():
-            raise ValueError("offsets must be a contiguous tensor of the indices' dtype")
-        bags = offsets.numel() - int(include_last_offset)
-    if bags < 0:
-        raise ValueError("offsets is empty, include_last_offset wants an entry")
-    if accumulate and grad_table is None:
-        raise ValueError("accumulate=True adds to a grad_table that the caller gives")
-    if not need_table and not need_weights:
-        raise ValueError("neither gradient is asked for")
-    if grad_table is not None and not need_table:
-        raise ValueError("grad_table is given but need_table is False")
-    if grad_out.dtype not in (torch.float32, torch.float16):
-        raise TypeError(f"grad_out: unsupported dtype {grad_out.dtype}")
-    if per_sample_weights is not None and (per_sample_weights.dtype != torch.float32
-                                           or not per_sample_weights.is_contiguous()
-                                           or per_sample_weights.numel() != n):
-        raise ValueError("per_sample_weights must be contiguous fp32, one per index")
-    win_stride = 0
-    if winners is not None:
-        if winners.dtype != torch.float32 or tuple(winners.shape) != (bags, dim, 2):
-            raise ValueError(f"winners must be fp32 [{bags}, {dim}, 2]")
-        if bags > 0 and (winners.stride(2) != 1 or (dim > 1 and winners.stride(1) != 2)
-                         or (bags > 1 and (winners.stride(0) % 2 or winners.stride(0) < 2 * dim))):
-            raise ValueError("winners must be rows of adjacent pairs")
-        win_stride = winners.stride(0) // 2 if bags > 1 else 0
-    go_stride = _rows(grad_out, "grad_out", dim, bags)
-    if grad_table is None:
-        gt_dtype = grad_dtype or table.dtype
-    else:
-        gt_dtype = grad_table.dtype
-        gt_stride = _rows(grad_table, "grad_table", dim, rows)
-    if need_table and gt_dtype not in (torch.float32, torch.float16):
-        raise TypeError(f"grad_table: unsupported dtype {gt_dtype}")
-    table_code, index_code = capi._torch_dtype_code(table), capi._index_code(indices)
+    result = (_loaded_ops or _ops()).embedding_bag_backward(
+        grad_out, table, indices, offsets, mode, fixed_len, per_sample_weights, include_last_offset, padding_idx, row_lo,
+        flags, winners, grad_table, _asked(grad_dtype, "grad_dtype"), accumulate, need_table, need_weights)
+    if type(result) is int:
+        capi.check(result)
+    return result
 
-    def run(stream):
-        gt, gs = grad_table, 0 if grad_table is None else gt_stride
-        if need_table and gt is None:
-            gt = table.new_empty((rows, dim), dtype=gt_dtype)
-        gw = table.new_empty(n, dtype=torch.float32) if need_weights else None
-        if (rows == 0 or not need_table) and (n == 0 or not need_weights):
-            return gt, gw   # nothing to compute; torch gives empty tensors no address
 
-        def pack(ws, nbytes):
-            return _pack_backward(
-                table.data_ptr(), table_code, dim, rows, row_lo, table.stride(0) if rows > 1 else 0,
-                indices.data_ptr(), _ptr(offsets), index_code, 0 if gather else fixed_len, n, 0 if gather else bags,
-                _ptr(per_sample_weights), mode, include_last_offset, padding_idx, 0, 0, 0, 0, 0, 0, flags, 0,
-                grad_out.data_ptr(), _DTYPES[grad_out.dtype], _DTYPES[gt_dtype], go_stride, _ptr(gt), gs, _ptr(gw),
-                _ptr(winners), win_stride, ws, nbytes, accumulate, 0)
-        lib = _lib()
-        need = lib.fwd_eb_backward_workspace_size(pack(0, 0))
-        ws = table.new_empty(need, dtype=torch.uint8) if need else None
-        capi.check(lib.fwd_eb_backward(pack(_ptr(ws), need), stream))
-        return gt, gw
-    return _on(device, run)
+def _asked(dtype, what: str) -> int:
+    """The code of a dtype that was asked for, -1 for None."""
+    if dtype is None:
+        return -1
+    if dtype not in _DTYPES:
+        raise TypeError(f"{what}: unsupported dtype {dtype}")
+    return _DTYPES[dtype]
 
 
 # ---- layer norm -------------------------------------------------------------------------
-
-
-def _vector(t, name: str, cols: int, like=None):
-    if t.dim() != 1 or t.numel() != cols or (cols > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name} must be contiguous [{cols}]")
-    if like is not None and t.dtype != like.dtype:
-        raise TypeError(f"{name} must have the weight's dtype")
-
-
-def _stats(t, name: str, rows: int):
-    if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != rows or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous fp32 [{rows}]")
 
 
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=False):
@@ -298,35 +209,10 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None, return_stats=Fa
 
     Returns y of x's dtype (`out`, which may be x, or a new tensor), or (y, mean, rstd) with
     return_stats=True: the fp32 statistics that layer_norm_backward takes."""
-    device = _device_of(("x", "weight", "bias", "out"), (x, weight, bias, out))
-    if x.dim() != 2:
-        raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
-    rows, cols = x.shape
-    code = _dtype(x, "x")
-    x_stride = _rows(x, "x", cols)
-    wtype = 0
-    if weight is not None:
-        _vector(weight, "weight", cols)
-        wtype = _dtype(weight, "weight")
-    if bias is not None:
-        _vector(bias, "bias", cols, weight)
-        wtype = _dtype(bias, "bias")
-    y_stride = 0
-    if out is not None:
-        if out.dtype != x.dtype:
-            raise TypeError("out must have x's dtype")
-        y_stride = _rows(out, "out", cols, rows)
-
-    def run(stream):
-        y = x.new_empty((rows, cols)) if out is None else out
-        mean = rstd = None
-        if return_stats:
-            mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
-        capi.check(_lib().fwd_eb_layer_norm_forward(_pack_norm(
-            x.data_ptr(), code, wtype, rows, cols, x_stride, _ptr(weight), _ptr(bias), eps, _ptr(mean), _ptr(rstd),
-            y.data_ptr(), y_stride, 0, 0, 0, 0, 0, 0, 0, 0), stream))
-        return (y, mean, rstd) if return_stats else y
-    return _on(device, run)
+    result = (_loaded_ops or _ops()).layer_norm(x, weight, bias, eps, out, return_stats)
+    if type(result) is int:
+        capi.check(result)
+    return result
 
 
 def layer_norm_backward(grad_y, x, mean, rstd, weight=None, *, grad_x=None, need_x=True, need_params=True,
@@ -336,44 +222,11 @@ def layer_norm_backward(grad_y, x, mean, rstd, weight=None, *, grad_x=None, need
     mean and rstd are the forward call's.  grad_x (x's dtype) may be given, and may be grad_y or x
     itself.  grad_weight and grad_bias have the weight's dtype, or `param_dtype` (default fp32)
     where there is no weight.  What is not asked for is None."""
-    device = _device_of(("x", "grad_y", "mean", "rstd", "weight", "grad_x"), (x, grad_y, mean, rstd, weight, grad_x))
-    if x.dim() != 2:
-        raise ValueError(f"x must be [rows, cols], got {list(x.shape)}")
-    rows, cols = x.shape
-    code = _dtype(x, "x")
-    if grad_y.dtype != x.dtype or (grad_x is not None and grad_x.dtype != x.dtype):
-        raise TypeError("grad_y and grad_x must have x's dtype")
-    if grad_x is not None and not need_x:
-        raise ValueError("grad_x is given but need_x is False")
-    x_stride, gy_stride = _rows(x, "x", cols), _rows(grad_y, "grad_y", cols, rows)
-    _stats(mean, "mean", rows)
-    _stats(rstd, "rstd", rows)
-    if weight is not None:
-        _vector(weight, "weight", cols)
-        param_dtype = weight.dtype
-    param_dtype = param_dtype or torch.float32
-    if param_dtype not in _DTYPES:
-        raise TypeError(f"param_dtype: unsupported dtype {param_dtype}")
-    gx_stride = 0 if grad_x is None else _rows(grad_x, "grad_x", cols, rows)
-
-    def run(stream):
-        gx = grad_x
-        if need_x and gx is None:
-            gx = x.new_empty((rows, cols))
-        gw = gb = None
-        if need_params:
-            gw, gb = x.new_empty(cols, dtype=param_dtype), x.new_empty(cols, dtype=param_dtype)
-
-        def pack(ws, nbytes):
-            return _pack_norm(
-                x.data_ptr(), code, _DTYPES[param_dtype], rows, cols, x_stride, _ptr(weight), 0, 0.0, mean.data_ptr(),
-                rstd.data_ptr(), 0, 0, grad_y.data_ptr(), gy_stride, _ptr(gx), gx_stride, _ptr(gw), _ptr(gb), ws, nbytes)
-        lib = _lib()
-        need = lib.fwd_eb_layer_norm_workspace_size(pack(0, 0)) if need_params else 0
-        ws = x.new_empty(need, dtype=torch.uint8) if need else None
-        capi.check(lib.fwd_eb_layer_norm_backward(pack(_ptr(ws), need), stream))
-        return gx, gw, gb
-    return _on(device, run)
+    result = (_loaded_ops or _ops()).layer_norm_backward(grad_y, x, mean, rstd, weight, grad_x, need_x, need_params,
+                                                         _asked(param_dtype, "param_dtype"))
+    if type(result) is int:
+        capi.check(result)
+    return result
 
 
 # ---- AdamW ------------------------------------------------------------------------------
