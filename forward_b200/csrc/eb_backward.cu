@@ -30,6 +30,7 @@ constexpr int kItems = 9;                          // pairs a thread ranks at a 
 constexpr int kSubTile = kSortThreads * kItems;
 constexpr int kSmallItems = 7;                     // ... in the kernel that sorts all of a small call
 constexpr int kSmall = kSortThreads * kSmallItems;
+constexpr int kTiny = 2 * kSortThreads;            // lookups of a call that one launch does
 constexpr int kDigits = 256;                       // at most
 constexpr int kStarts = 2048;                      // bag starts a tile keeps in shared memory
 constexpr int kRun = 32;                           // sorted lookups of a run, runs of a block of runs
@@ -153,6 +154,7 @@ struct TileStarts {
   bool in_shared;    // starts [lo, hi) are in shared memory
 };
 __device__ __forceinline__ int clamp_start(long long s) { return s < 0 ? -1 : (s > INT_MAX ? INT_MAX : (int)s); }
+template <int MOST>   // starts that fit `shared`
 __device__ __forceinline__ TileStarts find_starts(const BackArgs& a, int begin, int end, int* shared) {
   TileStarts t = {0, 0, false};
   if (a.fixed_len > 0 || begin >= end) return t;
@@ -160,7 +162,7 @@ __device__ __forceinline__ TileStarts find_starts(const BackArgs& a, int begin, 
   const int2 found = upper_bound_cta<kSortThreads>(a, begin, end - 1, n);
   t.lo = found.x;
   t.hi = max(found.x, found.y);
-  t.in_shared = t.hi - t.lo <= kStarts;
+  t.in_shared = t.hi - t.lo <= MOST;
   if (t.in_shared) {
     for (int i = t.lo + threadIdx.x; i < t.hi; i += kSortThreads)
       shared[i - t.lo] = clamp_start(index_at(a.offsets, a.idx64, i));
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs
     }
   };
   fetch(first);
-  const TileStarts t = find_starts(a, begin, end, starts);
+  const TileStarts t = find_starts<kStarts>(a, begin, end, starts);
   __syncthreads();
   BagWalk walk = walk_from(a, first, t, starts);
   const unsigned mask = (1u << a.bits) - 1u;
@@ -473,69 +475,80 @@ __global__ void __launch_bounds__(kSortThreads) sort_digit_kernel(const BackArgs
   }
 }
 
-// Up to kSmall lookups: one CTA finds the bags and does all digits in shared memory.
-__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs a, uint2* to) {
-  pdl_enter();
-  __shared__ unsigned place[kDigits];
-  __shared__ unsigned in_warp[kSortWarps][kDigits];
-  __shared__ uint2 pairs[kSmall];
-  __shared__ unsigned total[kDigits / 32];
-  int* starts = reinterpret_cast<int*>(pairs);   // before the first digit
-  static_assert(sizeof(pairs) >= kStarts * sizeof(int), "the starts fit");
+// What a CTA needs to sort up to ITEMS * kSortThreads lookups by itself.
+template <int ITEMS>
+struct SmallSort {
+  uint2 pairs[ITEMS * kSortThreads];     // the bag starts before the first digit, then the pairs between digits
+  unsigned place[kDigits];
+  unsigned in_warp[kSortWarps][kDigits];
+  unsigned total[kDigits / 32];
+};
+// Finds the bags of all lookups and sorts them by row into `to` (shared or global memory).
+template <int ITEMS>
+__device__ __forceinline__ void sort_all(const BackArgs& a, SmallSort<ITEMS>& s, uint2* to, bool keep_bags) {
+  int* starts = reinterpret_cast<int*>(s.pairs);
+  constexpr int kFit = ITEMS * kSortThreads * 2;        // starts that fit there
   const unsigned mask = (1u << a.bits) - 1u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = warp * kSmallItems * 32;
-  long long index[kSmallItems];
+  const int first = warp * ITEMS * 32;
+  long long index[ITEMS];
 #pragma unroll
-  for (int i = 0; i < kSmallItems; ++i) {
+  for (int i = 0; i < ITEMS; ++i) {
     const int j = first + i * 32 + lane;
     index[i] = j < a.n ? index_at(a.indices, a.idx64, j) : 0;
   }
-  const TileStarts t = find_starts(a, 0, a.n, starts);
-  uint2 pair[kSmallItems];
+  const TileStarts t = find_starts<(kFit < kStarts ? kFit : kStarts)>(a, 0, a.n, starts);
+  uint2 pair[ITEMS];
   BagWalk walk = walk_from(a, first, t, starts);
-  walk_bags<kSmallItems>(a, first, a.n, t, starts, walk, [&](int i, int bag) {
+  walk_bags<ITEMS>(a, first, a.n, t, starts, walk, [&](int i, int bag) {
     const int j = first + i * 32 + lane;
     pair[i] = make_uint2(0, 0);
     if (j < a.n) {
-      if (a.bag_of) a.bag_of[j] = bag;
+      if (keep_bags && a.bag_of) a.bag_of[j] = bag;
       pair[i] = make_uint2(row_of(a, index[i], bag), a.by_bag ? (unsigned)bag : (unsigned)j);
     }
-    if (a.counted) uncount_padding(a, index[i], j < a.n, bag);
+    if (a.counted && keep_bags) uncount_padding(a, index[i], j < a.n, bag);
   });
   for (int pass = 0; pass < a.passes; ++pass) {
-    unsigned digit[kSmallItems], rank[kSmallItems];
+    unsigned digit[ITEMS], rank[ITEMS];
 #pragma unroll
-    for (int i = 0; i < kSmallItems; ++i) {
-      const int j = (warp * kSmallItems + i) * 32 + lane;
+    for (int i = 0; i < ITEMS; ++i) {
+      const int j = first + i * 32 + lane;
       digit[i] = j < a.n ? (pair[i].x >> (a.bits * pass)) & mask : kNone;
     }
-    rank_items<kSmallItems>(digit, rank, in_warp, a.bits);
+    rank_items<ITEMS>(digit, rank, s.in_warp, a.bits);
     unsigned sum = 0;
     if (threadIdx.x < kDigits) {
 #pragma unroll
-      for (int w = 0; w < kSortWarps; ++w) sum += in_warp[w][threadIdx.x];
+      for (int w = 0; w < kSortWarps; ++w) sum += s.in_warp[w][threadIdx.x];
     }
-    const unsigned lower = digits_below(sum, total);
-    if (threadIdx.x < kDigits) place[threadIdx.x] = lower;
+    const unsigned lower = digits_below(sum, s.total);
+    if (threadIdx.x < kDigits) s.place[threadIdx.x] = lower;
     __syncthreads();
-    place_warps(in_warp, place);
+    place_warps(s.in_warp, s.place);
     const bool last = pass + 1 == a.passes;
 #pragma unroll
-    for (int i = 0; i < kSmallItems; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       if (digit[i] == kNone) continue;
-      const unsigned at = in_warp[warp][digit[i]] + rank[i];
-      if (last) to[at] = pair[i]; else pairs[at] = pair[i];
+      const unsigned at = s.in_warp[warp][digit[i]] + rank[i];
+      if (last) to[at] = pair[i]; else s.pairs[at] = pair[i];
     }
-    if (last) break;
     __syncthreads();
+    if (last) break;
 #pragma unroll
-    for (int i = 0; i < kSmallItems; ++i) {
-      const int j = (warp * kSmallItems + i) * 32 + lane;
-      if (j < a.n) pair[i] = pairs[j];
+    for (int i = 0; i < ITEMS; ++i) {
+      const int j = first + i * 32 + lane;
+      if (j < a.n) pair[i] = s.pairs[j];
     }
     __syncthreads();
   }
+}
+
+// Up to kSmall lookups: one CTA sorts them.
+__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs a, uint2* to) {
+  pdl_enter();
+  __shared__ SmallSort<kSmallItems> s;
+  sort_all<kSmallItems>(a, s, to, a.bag_of != nullptr || a.counted != nullptr);
 }
 
 // won[b][c] = the low byte of the position that won column c of bag b: what the sum below compares in bags of
@@ -678,8 +691,39 @@ __device__ __forceinline__ int2 find_rows(const uint2* pairs, int n, unsigned ro
   return make_int2(lo0, lo1);
 }
 
-// Fills the rows of a block of the table that no lookup names with zeros.
 constexpr int kZeroRows = 1024;      // at most, of a block
+// Zeros in the rows [first, first + rows) of the table that are not marked in `named`, by a CTA.
+__device__ __forceinline__ void fill_zeros(const BackArgs& a, const unsigned* named, long long first, int rows) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int per_row = a.dim * (a.gt_f16 ? 2 : 4) / a.word;      // stores a row
+  int shift = 5;                                                // a warp's lanes share 1, 2, 4, ... rows
+  while (shift > 0 && (1 << (shift - 1)) >= per_row) --shift;
+  const int at = lane & ((1 << shift) - 1), sub = lane >> shift, together = 32 >> shift;
+  char* base = a.grad_table + first * a.gt_stride;
+  if (a.word == 16 && per_row <= 1 << shift && at < per_row) {
+    // a store a lane and row: 32 rows of one mark word at a time
+    for (int g = threadIdx.x >> 5; g * 32 < rows; g += warps) {
+      const unsigned word = named[g];
+      const int most = min(32, rows - g * 32);
+      char* to = base + (long long)(g * 32 + sub) * a.gt_stride + at * 16;
+#pragma unroll 4
+      for (int r = sub; r < most; r += together, to += together * a.gt_stride) {
+        if (!(word >> r & 1u)) *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+  for (int r = (threadIdx.x >> 5) * together + sub; r < rows; r += warps * together) {
+    if (named[r >> 5] >> (r & 31) & 1u) continue;
+    char* to = base + r * a.gt_stride;
+    for (int w = at; w < per_row; w += 1 << shift) {
+      if (a.word == 16) reinterpret_cast<uint4*>(to)[w] = make_uint4(0, 0, 0, 0);
+      else if (a.word == 4) reinterpret_cast<unsigned*>(to)[w] = 0;
+      else reinterpret_cast<unsigned short*>(to)[w] = 0;
+    }
+  }
+}
+// Fills the rows of a block of the table that no lookup names with zeros.
 __device__ __forceinline__ void zero_block(const BackArgs& a, const uint2* pairs, int block) {
   __shared__ unsigned named[kZeroRows / 32];
   __shared__ int2 span;
@@ -726,33 +770,7 @@ __device__ __forceinline__ void zero_block(const BackArgs& a, const uint2* pairs
     }
   }
   __syncthreads();
-  const int per_row = a.dim * (a.gt_f16 ? 2 : 4) / a.word;      // stores a row
-  int shift = 5;                                                // a warp's lanes share 1, 2, 4, ... rows
-  while (shift > 0 && (1 << (shift - 1)) >= per_row) --shift;
-  const int at = lane & ((1 << shift) - 1), sub = lane >> shift, together = 32 >> shift;
-  char* base = a.grad_table + first * a.gt_stride;
-  if (a.word == 16 && per_row <= 1 << shift && at < per_row) {
-    // a store a lane and row: 32 rows of one mark word at a time
-    for (int g = threadIdx.x >> 5; g * 32 < rows; g += warps) {
-      const unsigned word = named[g];
-      const int most = min(32, rows - g * 32);
-      char* to = base + (long long)(g * 32 + sub) * a.gt_stride + at * 16;
-#pragma unroll 4
-      for (int r = sub; r < most; r += together, to += together * a.gt_stride) {
-        if (!(word >> r & 1u)) *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
-      }
-    }
-    return;
-  }
-  for (int r = (threadIdx.x >> 5) * together + sub; r < rows; r += warps * together) {
-    if (named[r >> 5] >> (r & 31) & 1u) continue;
-    char* to = base + r * a.gt_stride;
-    for (int w = at; w < per_row; w += 1 << shift) {
-      if (a.word == 16) reinterpret_cast<uint4*>(to)[w] = make_uint4(0, 0, 0, 0);
-      else if (a.word == 4) reinterpret_cast<unsigned*>(to)[w] = 0;
-      else reinterpret_cast<unsigned short*>(to)[w] = 0;
-    }
-  }
+  fill_zeros(a, named, first, rows);
 }
 __global__ void __launch_bounds__(256) zero_kernel(const BackArgs a) {     // no lookups at all
   pdl_enter();
@@ -817,6 +835,14 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
   const unsigned left_row = __shfl_up_sync(kAll, pair.x, 1);
   // lookups at which a row begins (the run's first always counts)
   const unsigned heads = __ballot_sync(kAll, lane == 0 || (lane < valid && pair.x != left_row));
+  if constexpr (kTable) {
+    // the table rows of the run are asked for together: they come from DRAM, most of grad_out from the L2
+    if (heads >> lane & 1u) {
+      const char* row = a.table + (long long)pair.x * a.table_stride + (long long)tile * 32 * VE * (a.table_f16 ? 2 : 4);
+      const int bytes = min(32 * VE, a.dim - tile * 32 * VE) * (a.table_f16 ? 2 : 4);
+      for (int b = 0; b < bytes; b += 128) asm volatile("prefetch.global.L2 [%0];" :: "l"(row + b));
+    }
+  }
   float acc[VE];
   float x[kTable ? VE : 1];     // the running row of the table
 #pragma unroll
@@ -962,13 +988,14 @@ __global__ void __launch_bounds__(256) segment_block_kernel(const BackArgs a, co
 #pragma unroll
     for (int i = 0; i < VE; ++i) acc[k][i] = 0.0f;
   }
+  constexpr int kTogether = VE == 8 ? 16 : 32;
 #pragma unroll
-  for (int r = 0; r < kRun; r += 8) {
-    Pack<float, VE> p[8];
+  for (int r = 0; r < kRun; r += kTogether) {
+    Pack<float, VE> p[kTogether];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) p[u].load(a.partial + (long long)(run0 + r + u) * 2 * a.pstride + col);
+    for (int u = 0; u < kTogether; ++u) p[u].load(a.partial + (long long)(run0 + r + u) * 2 * a.pstride + col);
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < kTogether; ++u) {
       float f[VE];
       p[u].get(f);
 #pragma unroll
@@ -982,43 +1009,62 @@ __global__ void __launch_bounds__(256) segment_block_kernel(const BackArgs a, co
   r.store(a.super + (long long)block * a.pstride + col);
 }
 
-// Rows that cross runs.  A warp looks at one run: where a row starts in it and goes on, the warp adds the row's
-// pieces itself if they are few, else the CTA's 8 warps share them.
+// Rows that cross runs.  A warp looks at 8 runs at once.  Most rows that start in one of them and go on end in the next:
+// two pieces, added for four rows at a time.  Of the others the warp adds the pieces itself if they are few;
+// else the CTA's 8 warps share them.
 constexpr int kFewPieces = 24;
+constexpr int kJoinRuns = 8;       // of a warp
 template <int VE>
 __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, const uint2* pairs) {
   pdl_enter();
-  __shared__ int last_run[8];
+  constexpr unsigned kAll = 0xffffffffu;
+  __shared__ int long_from[8 * kJoinRuns], long_to[8 * kJoinRuns];
+  __shared__ int longs;
   __shared__ float part[8][32 * VE];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (blockIdx.y * 32 + lane) * VE;
   const bool col_ok = col < a.dim;
-  const int run = blockIdx.x * 8 + warp;
-  int last = -1;          // the row's last run, -1: nothing to join here
-  if (run + 1 < a.runs) {
-    const unsigned row = pairs[run * kRun + kRun - 1].x;
-    const unsigned before = run > 0 ? pairs[run * kRun - 1].x : kNone;
-    // the next 32 runs at once; rows of more are searched for
-    const unsigned ahead = run + 1 + lane < a.runs ? first_row(pairs, run + 1 + lane) : kNone;
-    const unsigned same = __ballot_sync(0xffffffffu, ahead == row);
-    if (row < a.num_rows && before != row && (same & 1u)) {
-      if (same != 0xffffffffu) {
-        last = run + __ffs(~same) - 1;
-      } else {
-        int lo = run + 32, len = a.runs - 1 - lo;    // the last run that starts with the row: 32 probes a round
-        while (len > 0) {
-          const int step = (len + 31) / 32;
-          const long long at = lo + (lane + 1LL) * step;
-          const bool mine = at <= (long long)lo + len && first_row(pairs, (int)at) == row;
-          const int c = __popc(__ballot_sync(0xffffffffu, mine));
-          len = min(step - 1, len - c * step);
-          lo += c * step;
-        }
-        last = lo;
-      }
-    }
+  if (threadIdx.x == 0) longs = 0;
+  __syncthreads();
+  const int run0 = (blockIdx.x * 8 + warp) * kJoinRuns;
+  unsigned row = kNone;
+  bool crosses = false, two = false;
+  if (lane < kJoinRuns && run0 + lane + 1 < a.runs) {
+    const int run = run0 + lane;
+    row = __ldg(&pairs[run * kRun + kRun - 1].x);
+    const unsigned before = run > 0 ? __ldg(&pairs[run * kRun - 1].x) : kNone;
+    const unsigned next = first_row(pairs, run + 1);
+    const unsigned next2 = run + 2 < a.runs ? first_row(pairs, run + 2) : kNone;
+    crosses = row < a.num_rows && before != row && next == row;
+    two = crosses && next2 != row;
   }
   float acc[4][VE];
+  for (unsigned left = __ballot_sync(kAll, two); left != 0;) {
+    Pack<float, VE> tail[4], head[4];
+    int at[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      at[u] = left != 0 ? __ffs(left) - 1 : -1;
+      if (left != 0) left &= left - 1;
+      if (at[u] >= 0 && col_ok) {
+        const float* p = a.partial + (long long)(run0 + at[u]) * 2 * a.pstride + col;
+        tail[u].load(p + a.pstride);
+        head[u].load(p + 2 * a.pstride);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (at[u] < 0) continue;
+      const unsigned r = __shfl_sync(kAll, row, at[u]);
+      if (!col_ok) continue;
+      float t[VE], h[VE];
+      tail[u].get(t);
+      head[u].get(h);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) t[i] += h[i];
+      store_row<VE>(a, r, col, t);
+    }
+  }
   // the row's pieces [begin, end) into acc[0]: its tail in `from`, single runs up to a block border, whole
   // blocks, single runs
   auto add_pieces = [&](int from, int to, int begin, int end) {
@@ -1065,18 +1111,40 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
     if (!a.super || b1 <= b0) return 1 + to - first + 1;
     return 1 + (b0 * kRun - first) + (b1 - b0) + (to + 1 - b1 * kRun);
   };
-  const int mine = last >= 0 ? count_pieces(run, last) : 0;
-  if (lane == 0) last_run[warp] = mine > kFewPieces ? last : -1;
-  const bool shared_work = __syncthreads_or(mine > kFewPieces);
-  if (mine > 0 && mine <= kFewPieces) {
-    add_pieces(run, last, 0, mine);
-    if (col_ok) store_row<VE>(a, pairs[run * kRun + kRun - 1].x, col, acc[0]);
+  for (unsigned left = __ballot_sync(kAll, crosses && !two); left != 0; left &= left - 1) {
+    const int from = run0 + __ffs(left) - 1;
+    const unsigned r = __shfl_sync(kAll, row, from - run0);
+    // the last run that starts with the row: the next 32 at once, then 32 probes a round
+    const unsigned ahead = from + 1 + lane < a.runs ? first_row(pairs, from + 1 + lane) : kNone;
+    const unsigned same = __ballot_sync(kAll, ahead == r);
+    int to = from + __ffs(~same) - 1;
+    if (same == kAll) {
+      to = from + 32;
+      int len = a.runs - 1 - to;
+      while (len > 0) {
+        const int step = (len + 31) / 32;
+        const long long at = to + (lane + 1LL) * step;
+        const bool mine = at <= (long long)to + len && first_row(pairs, (int)at) == r;
+        const int c = __popc(__ballot_sync(kAll, mine));
+        len = min(step - 1, len - c * step);
+        to += c * step;
+      }
+    }
+    const int pieces = count_pieces(from, to);
+    if (pieces > kFewPieces) {
+      if (lane == 0) {
+        const int k = atomicAdd(&longs, 1);
+        long_from[k] = from;
+        long_to[k] = to;
+      }
+      continue;
+    }
+    add_pieces(from, to, 0, pieces);
+    if (col_ok) store_row<VE>(a, r, col, acc[0]);
   }
-  if (!shared_work) return;
-  for (int w = 0; w < 8; ++w) {
-    const int to = last_run[w];
-    if (to < 0) continue;              // the same for the whole CTA
-    const int from = blockIdx.x * 8 + w;
+  __syncthreads();
+  for (int k = 0; k < longs; ++k) {          // in any order: each is a row of its own
+    const int from = long_from[k], to = long_to[k];
     const int pieces = count_pieces(from, to);
     const int share = (pieces + 7) / 8;
     add_pieces(from, to, min(pieces, warp * share), min(pieces, (warp + 1) * share));
@@ -1089,11 +1157,221 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
       for (int i = 0; i < VE; ++i) {
         sum[i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum[i] += part[k][lane * VE + i];
+        for (int w = 0; w < 8; ++w) sum[i] += part[w][lane * VE + i];
       }
-      store_row<VE>(a, pairs[from * kRun + kRun - 1].x, col, sum);
+      store_row<VE>(a, __ldg(&pairs[from * kRun + kRun - 1].x), col, sum);
     }
     __syncthreads();
+  }
+}
+
+// Up to kTiny lookups in one launch: every CTA sorts all of them for itself, a few microseconds that no other CTA has
+// to be waited for, and takes its share of the rows.  A warp sums a row of up to 32 lookups, the CTA's
+// warps together one of more; the rows that no lookup names are filled with zeros.  The kind of the call is
+// a branch here: instructions do not count at this size, launches do.
+template <int ITEMS>                // lookups a thread sorts
+struct TinyShared {
+  static constexpr int kMost = ITEMS * kSortThreads;
+  SmallSort<ITEMS> sort;
+  uint2 pairs[kMost];               // sorted
+  int begins[kMost + 1];            // of each row's lookups
+  int padding[kMost + 1];           // among the lookups before each
+  int count;                        // rows
+  int total;
+  int warps[kSortWarps];
+  unsigned named[kZeroRows / 32];
+};
+template <typename TG, int VE, int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) tiny_kernel(const BackArgs a, int kind) {
+  pdl_enter();
+  extern __shared__ uint4 dynamic[];
+  TinyShared<ITEMS>& s = *reinterpret_cast<TinyShared<ITEMS>*>(dynamic);
+  constexpr unsigned kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  sort_all<ITEMS>(a, s.sort, s.pairs, false);
+  // sums over the threads before this one; s.total: over all
+  auto scan = [&](int mine) {
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(kAll, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31) s.warps[warp] = sum;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+      if (w < warp) sum += s.warps[w];
+      all += s.warps[w];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s.total = all;
+    return sum - mine;
+  };
+  const int k0 = threadIdx.x * ITEMS;
+  const bool count_padding = a.mean && !a.mean_raw && a.padding_idx >= 0;
+  if (count_padding) {     // padding[j]: of the lookups before j
+    int mine = 0, is[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) mine += is[i] = k0 + i < a.n && index_at(a.indices, a.idx64, k0 + i) == a.padding_idx;
+    int at = scan(mine);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      if (k0 + i <= a.n) s.padding[k0 + i] = at;
+      at += is[i];
+    }
+    if (threadIdx.x == kSortThreads - 1) s.padding[ITEMS * kSortThreads] = at;
+    __syncthreads();
+  }
+  // the rows' first lookups, in order; those of no row (num_rows) sort last
+  {
+    int mine = 0, is[ITEMS], in = 0;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int k = k0 + i;
+      const bool row = k < a.n && s.pairs[k].x < a.num_rows;
+      in += row;
+      mine += is[i] = row && (k == 0 || s.pairs[k - 1].x != s.pairs[k].x);
+    }
+    scan(in);
+    __syncthreads();
+    const int behind = s.total;
+    __syncthreads();
+    int at = scan(mine);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      if (is[i]) s.begins[at++] = k0 + i;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      s.count = s.total;
+      s.begins[s.count] = behind;
+    }
+    __syncthreads();
+  }
+  const int rows = s.count, valid = s.begins[rows];
+  auto bag_of_lookup = [&](unsigned payload) {
+    if (a.by_bag) return (int)payload;
+    const int j = (int)payload;
+    if (a.fixed_len > 0) return j / a.fixed_len;
+    return max(0, upper_bound([&](int i) { return index_at(a.offsets, a.idx64, i); }, j, 0, a.num_bags) - 1);
+  };
+  const int column_tiles = (a.dim + 32 * VE - 1) / (32 * VE);
+  // the lookups [from, to) of one row into acc, columns `col` on
+  auto add = [&](int from, int to, int col, float (&acc)[VE]) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
+    for (int base = from; base < to; base += 32) {
+      const int most = min(32, to - base);
+      int bag = 0, pos = 0;      // a lane finds one lookup's bag, position in it and factor
+      float c = 1.0f;
+      if (lane < most) {
+        const unsigned payload = s.pairs[base + lane].y;
+        bag = bag_of_lookup(payload);
+        if (a.psw) c = a.psw[payload];
+        if (a.mean || kind == kMax) {
+          long long b, e;
+          bag_range(a, bag, b, e);
+          pos = (int)payload - (int)b;
+          if (a.mean) c = 1.0f / (float)((int)(e - b) - (count_padding ? s.padding[e] - s.padding[b] : 0));
+        }
+      }
+      constexpr int U = 4;
+      for (int e0 = 0; e0 < most; e0 += U) {
+        Pack<TG, VE> g[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int b = __shfl_sync(kAll, bag, e0 + u);
+          g[u].zero();
+          if (e0 + u < most && col < a.dim)
+            g[u].load_ro(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int b = __shfl_sync(kAll, bag, e0 + u), p = __shfl_sync(kAll, pos, e0 + u);
+          const float f = __shfl_sync(kAll, c, e0 + u);
+          if (e0 + u >= most || col >= a.dim) continue;
+          float x[VE];
+          g[u].get(x);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            if (kind == kMax) acc[i] += __ldg(&a.winners[(long long)b * a.win_stride + col + i].y) == p ? x[i] : 0.0f;
+            else acc[i] = fmaf(f, x[i], acc[i]);
+          }
+        }
+      }
+    }
+  };
+  // rows of up to 32 lookups, a warp each
+  for (int r = blockIdx.x * kSortWarps + warp; r < rows; r += gridDim.x * kSortWarps) {
+    const int from = s.begins[r], to = s.begins[r + 1];
+    if (to - from > kRun) continue;
+    for (int tile = 0; tile < column_tiles; ++tile) {
+      const int col = (tile * 32 + lane) * VE;
+      float acc[VE];
+      add(from, to, col, acc);
+      if (col < a.dim) store_row<VE>(a, s.pairs[from].x, col, acc);
+    }
+  }
+  // rows of more, a CTA each: a warp takes consecutive shares, which are added in order
+  float* part = reinterpret_cast<float*>(s.sort.in_warp);       // [16 warps][32 * VE]
+  static_assert(sizeof(s.sort.in_warp) >= kSortWarps * 32 * VE * sizeof(float), "the warps' sums fit");
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int from = s.begins[r], to = s.begins[r + 1];
+    if (to - from <= kRun) continue;
+    const int share = (to - from + kSortWarps - 1) / kSortWarps;
+    for (int tile = 0; tile < column_tiles; ++tile) {
+      const int col = (tile * 32 + lane) * VE;
+      float acc[VE];
+      add(min(to, from + warp * share), min(to, from + (warp + 1) * share), col, acc);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) part[warp * 32 * VE + lane * VE + i] = acc[i];
+      __syncthreads();
+      if (warp == 0 && col < a.dim) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          acc[i] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kSortWarps; ++w) acc[i] += part[w * 32 * VE + lane * VE + i];
+        }
+        store_row<VE>(a, s.pairs[from].x, col, acc);
+      }
+      __syncthreads();
+    }
+  }
+  if (a.grad_weights) {      // a warp a lookup; the payload is the lookup
+    for (int k = blockIdx.x * kSortWarps + warp; k < a.n; k += gridDim.x * kSortWarps) {
+      const uint2 p = s.pairs[k];
+      float dot = 0.0f;
+      if (k < valid) {
+        const char* g = a.grad_out + (long long)bag_of_lookup(p.y) * a.go_stride;
+        for (int col = lane * VE; col < a.dim; col += 32 * VE) {
+          Pack<TG, VE> r;
+          float fg[VE], fx[VE];
+          r.load_ro(reinterpret_cast<const TG*>(g) + col);
+          r.get(fg);
+          load_either<VE>(a.table + (long long)p.x * a.table_stride, a.table_f16, col, fx);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) dot = fmaf(fg[i], fx[i], dot);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(kAll, dot, o);
+      if (lane == 0) a.grad_weights[p.y] = dot;
+    }
+  }
+  for (int block = blockIdx.x; block < a.zero_blocks; block += gridDim.x) {
+    const long long first = (long long)block * a.zero_rows;
+    const int most = (int)min((long long)a.zero_rows, a.num_rows - first);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kZeroRows / 32; i += kSortThreads) s.named[i] = 0;
+    __syncthreads();
+    for (int k = threadIdx.x; k < valid; k += kSortThreads) {
+      const long long r = (long long)s.pairs[k].x - first;
+      if (r >= 0 && r < most) atomicOr(&s.named[r >> 5], 1u << (r & 31));
+    }
+    __syncthreads();
+    fill_zeros(a, s.named, first, most);
   }
 }
 
@@ -1135,6 +1413,7 @@ struct BackPlan {
   int ve;                    // columns a lane
   bool want_table;
   bool fused_weights;        // grad_weights comes out of the segment sum
+  bool tiny;                 // one launch does everything
   size_t bytes;              // workspace
 };
 
@@ -1242,7 +1521,21 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
     a.zero_blocks = (int)blocks;
   }
   a.by_bag = !a.winners && !a.psw && !pl->fused_weights;
+  // One launch for few lookups, although every CTA sorts them all and a popular row is the work of one CTA: 320 lookups
+  // of a 10000 x 64 fp32 table 7.2 us against 17.0 in three launches, 1024 lookups 9.3 against 18.8, all 1024 of one
+  // row of it 17.2 against 18.5 (of a table of that row alone 16.8 against 14.2).
+  pl->tiny = a.n <= kTiny && pl->want_table;
+  if (pl->tiny) {
+    a.by_bag = !a.winners && !a.psw && !a.grad_weights;
+    if (a.zero_blocks > 0) {      // a share of the zeros for every CTA
+      const long long rows = (f.num_rows + sm_count() - 1) / sm_count();
+      a.zero_rows = (int)(rows < 32 ? 32 : (rows < kZeroRows ? rows : kZeroRows));
+      a.zero_blocks = (int)((f.num_rows + a.zero_rows - 1) / a.zero_rows);
+    }
+  }
   const bool bags_apart = !a.by_bag || (a.grad_weights && !pl->fused_weights);
+
+  if (pl->tiny) return 0;     // no scratch
 
   // scratch, each part on a 256-byte border
   size_t at = 0;
@@ -1265,7 +1558,8 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
     a.partial = reinterpret_cast<float*>(ws + take((size_t)a.runs * 2 * a.pstride * 4));
     const int blocks = a.runs / kRun;
     const size_t super = take((size_t)blocks * a.pstride * 4);
-    a.super = blocks > 1 ? reinterpret_cast<float*>(ws + super) : nullptr;
+    // below that the rows' pieces are few enough to be added in one step (a launch less)
+    a.super = blocks >= kRun ? reinterpret_cast<float*>(ws + super) : nullptr;
     a.won = reinterpret_cast<unsigned char*>(ws + take(a.winners ? (size_t)a.num_bags * a.pstride : 0));
   } else {
     a.passes = 0;
@@ -1303,8 +1597,39 @@ cudaError_t launch_segments(const BackPlan& pl, const uint2* sorted, cudaStream_
     const dim3 blocks((unsigned)((a.runs / kRun + 7) / 8), tiles);
     FWD_EB_TRY(launch_pdl(segment_block_kernel<VE>, blocks, 256, 0, st, a, sorted));
   }
-  if (a.runs > 1) FWD_EB_TRY(launch_pdl(segment_join_kernel<VE>, grid, 256, 0, st, a, sorted));
+  if (a.runs > 1) {
+    const dim3 joins((unsigned)((a.runs + 8 * kJoinRuns - 1) / (8 * kJoinRuns)), tiles);
+    FWD_EB_TRY(launch_pdl(segment_join_kernel<VE>, joins, 256, 0, st, a, sorted));
+  }
   return cudaSuccess;
+}
+
+template <typename TG, int VE, int ITEMS>
+cudaError_t launch_tiny_items(const BackArgs& a, unsigned ctas, cudaStream_t st) {
+  constexpr int bytes = (int)sizeof(TinyShared<ITEMS>);
+  FWD_EB_TRY(allow_shared<tiny_kernel<TG, VE, ITEMS>, bytes>());
+  return launch_pdl(tiny_kernel<TG, VE, ITEMS>, dim3(ctas), kSortThreads, bytes, st, a, a.winners ? kMax : kPlain);
+}
+template <typename TG, int VE>
+cudaError_t launch_tiny(const BackPlan& pl, cudaStream_t st) {
+  const BackArgs& a = pl.a;
+  // a warp a row, and CTAs for the zeros, up to one an SM
+  const int want = (a.n + kSortWarps - 1) / kSortWarps, most = sm_count();
+  int ctas = want > a.zero_blocks ? want : a.zero_blocks;
+  if (ctas > most) ctas = most;
+  return a.n <= kSortThreads ? launch_tiny_items<TG, VE, 1>(a, (unsigned)ctas, st) : launch_tiny_items<TG, VE, 2>(a, (unsigned)ctas, st);
+}
+
+template <typename TG>
+cudaError_t launch_tiny_ve(const BackPlan& pl, cudaStream_t st) {
+  switch (pl.ve) {
+    case 8:
+      if constexpr (sizeof(TG) == 2) return launch_tiny<TG, 8>(pl, st);
+      return cudaErrorInvalidValue;
+    case 4: return launch_tiny<TG, 4>(pl, st);
+    case 2: return launch_tiny<TG, 2>(pl, st);
+    default: return launch_tiny<TG, 1>(pl, st);
+  }
 }
 
 template <typename TG>
@@ -1335,6 +1660,7 @@ cudaError_t launch_weights(const BackPlan& pl, cudaStream_t st) {
 cudaError_t launch_backward(const BackPlan& pl, const fwd_eb_backward_params* p, cudaStream_t st) {
   const BackArgs& a = pl.a;
   if (a.n == 0) return a.zero_blocks > 0 ? launch_pdl(zero_kernel, dim3((unsigned)a.zero_blocks), 256, 0, st, a) : cudaSuccess;
+  if (pl.tiny) return p->grad_out_dtype == FWD_EB_F16 ? launch_tiny_ve<__half>(pl, st) : launch_tiny_ve<float>(pl, st);
   if (a.counted && a.num_bags > 0)
     FWD_EB_TRY(launch_pdl(bag_length_kernel, dim3((unsigned)((a.num_bags + 255) / 256)), 256, 0, st, a));
   if (pl.want_table && a.winners) {

@@ -821,3 +821,23 @@ def test_a_training_step_of_a_table():
         plain.step()
         for got, leaf in zip((table, w, b), leaves):
             assert float((got.to(F64) - leaf.detach()).abs().max()) <= 1e-3
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("n,rows,dim", [(1, 3, 5), (33, 1, 64), (64, 2, 300), (700, 5, 128), (1023, 40, 16), (1024, 1, 8),
+                                        (1024, 3000, 1100), (1025, 50, 32), (1025, 1, 8)])
+def test_bag_gradient_small_calls(mode, n, rows, dim):
+    """Calls that run in one launch, and the first that do not; popular rows, empty bags, many columns."""
+    lengths = [n // 2, 0, n - n // 2 - n // 3, 0, n // 3]
+    for dtype, weighted in ((torch.float16, False), (torch.float32, mode == capi.MODE_SUM)):
+        s, go, bag, starts = make_bags(n + rows, rows, dim, lengths, mode=mode, dtype=dtype, pad=rows > 2, weighted=weighted,
+                                       hot=0.4)
+        check_bag(s, go, bag, starts)
+
+
+def test_bag_gradient_small_calls_with_more_bags_than_lookups():
+    """Thousands of empty bags around a few lookups, with and without a row that is only padding."""
+    lengths = [0] * 3000 + [2, 0, 5] + [0] * 2000 + [1]
+    for mode in MODES:
+        s, go, bag, starts = make_bags(6, 20, 12, lengths, mode=mode, dtype=torch.float32, pad=True)
+        check_bag(s, go, bag, starts)
