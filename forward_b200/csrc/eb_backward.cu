@@ -780,7 +780,9 @@ __global__ void __launch_bounds__(256) zero_kernel(const BackArgs a) {     // no
 // A warp per run of 32 sorted lookups and tile of 32 * VE columns.  The CTAs that fill with zeros are spread evenly
 // among those that add.  ACC: what grad_table holds is added.
 // A table row that is wanted is read with the loads of the row's first lookup, so that no load is waited for alone.
-template <typename TG, int VE, int KIND, bool ACC>
+// SAME: the table and grad_table have grad_out's type; branches on their types in every unrolled step would not fit the
+// instruction cache (4 M x 128 fp32, weighted and accumulated: SAME_A us against SAME_B).
+template <typename TG, int VE, int KIND, bool ACC, bool SAME>
 __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
   pdl_enter();
   int cta = blockIdx.x;
@@ -796,6 +798,7 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
   const int tile = cta / of_run;
   cta -= tile * of_run;
   constexpr bool kTable = KIND == kWeights || KIND == kSquare;
+  const int gt_f16 = SAME ? sizeof(TG) == 2 : a.gt_f16, table_f16 = SAME ? sizeof(TG) == 2 : a.table_f16;
   constexpr int U = kTable || VE == 8 ? 4 : 8;   // lookups whose loads are issued together
   constexpr unsigned kAll = 0xffffffffu;
   const int lane = threadIdx.x & 31;
@@ -838,8 +841,8 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
   if constexpr (kTable) {
     // the table rows of the run are asked for together: they come from DRAM, most of grad_out from the L2
     if (heads >> lane & 1u) {
-      const char* row = a.table + (long long)pair.x * a.table_stride + (long long)tile * 32 * VE * (a.table_f16 ? 2 : 4);
-      const int bytes = min(32 * VE, a.dim - tile * 32 * VE) * (a.table_f16 ? 2 : 4);
+      const char* row = a.table + (long long)pair.x * a.table_stride + (long long)tile * 32 * VE * (table_f16 ? 2 : 4);
+      const int bytes = min(32 * VE, a.dim - tile * 32 * VE) * (table_f16 ? 2 : 4);
       for (int b = 0; b < bytes; b += 128) asm volatile("prefetch.global.L2 [%0];" :: "l"(row + b));
     }
   }
@@ -858,8 +861,8 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
           for (int i = 0; i < VE; ++i) acc[i] *= 2.0f * x[i];
         }
         char* to = a.grad_table + (long long)row * a.gt_stride;
-        if constexpr (ACC) add_either<VE>(to, a.gt_f16, col, acc);
-        else store_either<VE>(to, a.gt_f16, col, acc);
+        if constexpr (ACC) add_either<VE>(to, gt_f16, col, acc);
+        else store_either<VE>(to, gt_f16, col, acc);
       } else {
         Pack<float, VE> r;
         r.set(acc);
@@ -886,7 +889,7 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
       }
       if constexpr (kTable) {
         const unsigned r = __shfl_sync(kAll, pair.x, e0 + u);
-        if (in && (heads >> (e0 + u) & 1u)) load_either<VE>(a.table + (long long)r * a.table_stride, a.table_f16, col, xs[u]);
+        if (in && (heads >> (e0 + u) & 1u)) load_either<VE>(a.table + (long long)r * a.table_stride, table_f16, col, xs[u]);
       }
     }
     [[maybe_unused]] float dot[KIND == kWeights ? U : 1];
@@ -970,43 +973,48 @@ __global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, cons
   put(valid - 1, __shfl_sync(kAll, pair.x, valid - 1) == next);
 }
 
-__device__ __forceinline__ unsigned first_row(const uint2* pairs, int run) { return pairs[run * kRun].x; }
+__device__ __forceinline__ unsigned first_row(const uint2* pairs, int run) { return __ldg(&pairs[run * kRun].x); }
 
-// super[s] = sum of the 32 runs of block s, where one row's lookups fill all the block's run starts.
+// super[s] = sum of the 32 runs of block s, where one row's lookups fill all the block's run starts.  A CTA a block.
 template <int VE>
 __global__ void __launch_bounds__(256) segment_block_kernel(const BackArgs a, const uint2* pairs) {
   pdl_enter();
-  const int block = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int col = (blockIdx.y * 32 + (threadIdx.x & 31)) * VE;
-  const int run0 = block * kRun;
-  if (run0 + kRun > a.runs || block == 0 || col >= a.dim) return;
-  const unsigned row = first_row(pairs, run0);
-  if (row >= a.num_rows || pairs[run0 * kRun - 1].x != row || first_row(pairs, run0 + kRun - 1) != row) return;
-  float acc[4][VE];
+  __shared__ float part[8][32 * VE];
+  const int run0 = blockIdx.x * kRun;
+  if (run0 + kRun > a.runs || blockIdx.x == 0) return;
+  const unsigned row = first_row(pairs, run0), before = __ldg(&pairs[run0 * kRun - 1].x), last = first_row(pairs, run0 + kRun - 1);
+  if (row >= a.num_rows || before != row || last != row) return;       // the same for the CTA
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = (blockIdx.y * 32 + lane) * VE;
+  Pack<float, VE> p[kRun / 8];
+  float sum[VE];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-#pragma unroll
-    for (int i = 0; i < VE; ++i) acc[k][i] = 0.0f;
-  }
-  constexpr int kTogether = VE == 8 ? 16 : 32;
-#pragma unroll
-  for (int r = 0; r < kRun; r += kTogether) {
-    Pack<float, VE> p[kTogether];
-#pragma unroll
-    for (int u = 0; u < kTogether; ++u) p[u].load(a.partial + (long long)(run0 + r + u) * 2 * a.pstride + col);
-#pragma unroll
-    for (int u = 0; u < kTogether; ++u) {
-      float f[VE];
-      p[u].get(f);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) acc[u & 3][i] += f[i];
-    }
+  for (int u = 0; u < kRun / 8; ++u) {
+    p[u].zero();
+    if (col < a.dim) p[u].load(a.partial + (long long)(run0 + warp * (kRun / 8) + u) * 2 * a.pstride + col);
   }
 #pragma unroll
-  for (int i = 0; i < VE; ++i) acc[0][i] = (acc[0][i] + acc[1][i]) + (acc[2][i] + acc[3][i]);
+  for (int i = 0; i < VE; ++i) sum[i] = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kRun / 8; ++u) {
+    float f[VE];
+    p[u].get(f);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) sum[i] += f[i];
+  }
+#pragma unroll
+  for (int i = 0; i < VE; ++i) part[warp][lane * VE + i] = sum[i];
+  __syncthreads();
+  if (warp != 0 || col >= a.dim) return;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    sum[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum[i] += part[w][lane * VE + i];
+  }
   Pack<float, VE> r;
-  r.set(acc[0]);
-  r.store(a.super + (long long)block * a.pstride + col);
+  r.set(sum);
+  r.store(a.super + (long long)blockIdx.x * a.pstride + col);
 }
 
 // Rows that cross runs.  A warp looks at 8 runs at once.  Most rows that start in one of them and go on end in the next:
@@ -1502,7 +1510,8 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
   while (bits < 32 && (a.num_rows >> bits) != 0) ++bits;     // num_rows itself is a key
   a.passes = (bits + 7) / 8;
   a.bits = (bits + a.passes - 1) / a.passes;
-  const long long per = ((long long)a.n + sm_count() - 1) / sm_count();
+  // two sort CTAs an SM: 1.3 M lookups 232 us a call against 264 with one of twice the lookups
+  const long long per = ((long long)a.n + 2 * sm_count() - 1) / (2 * sm_count());
   a.tile = (int)(per < 1024 ? 1024 : (per + 31) / 32 * 32);
   a.tiles = (int)(((long long)a.n + a.tile - 1) / a.tile);
   a.runs = (int)(((long long)a.n + kRun - 1) / kRun);
@@ -1574,14 +1583,14 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
     if (e_ != cudaSuccess) return e_;    \
   } while (0)
 
-template <typename TG, int VE, bool ACC>
+template <typename TG, int VE, bool ACC, bool SAME>
 cudaError_t launch_sums(const BackPlan& pl, dim3 grid, const uint2* sorted, cudaStream_t st) {
   const BackArgs& a = pl.a;
-  if (a.winners) return launch_pdl(segment_sum_kernel<TG, VE, kMax, ACC>, grid, 256, 0, st, a, sorted);
-  if (a.square) return launch_pdl(segment_sum_kernel<TG, VE, kSquare, ACC>, grid, 256, 0, st, a, sorted);
-  if (pl.fused_weights) return launch_pdl(segment_sum_kernel<TG, VE, kWeights, ACC>, grid, 256, 0, st, a, sorted);
-  if (a.psw || a.mean) return launch_pdl(segment_sum_kernel<TG, VE, kScaled, ACC>, grid, 256, 0, st, a, sorted);
-  return launch_pdl(segment_sum_kernel<TG, VE, kPlain, ACC>, grid, 256, 0, st, a, sorted);
+  if (a.winners) return launch_pdl(segment_sum_kernel<TG, VE, kMax, ACC, SAME>, grid, 256, 0, st, a, sorted);
+  if (a.square) return launch_pdl(segment_sum_kernel<TG, VE, kSquare, ACC, SAME>, grid, 256, 0, st, a, sorted);
+  if (pl.fused_weights) return launch_pdl(segment_sum_kernel<TG, VE, kWeights, ACC, SAME>, grid, 256, 0, st, a, sorted);
+  if (a.psw || a.mean) return launch_pdl(segment_sum_kernel<TG, VE, kScaled, ACC, SAME>, grid, 256, 0, st, a, sorted);
+  return launch_pdl(segment_sum_kernel<TG, VE, kPlain, ACC, SAME>, grid, 256, 0, st, a, sorted);
 }
 
 template <typename TG, int VE>
@@ -1592,9 +1601,11 @@ cudaError_t launch_segments(const BackPlan& pl, const uint2* sorted, cudaStream_
   const long long ctas = (long long)grid.x * tiles + a.zero_blocks;
   if (ctas > INT_MAX) return cudaErrorInvalidConfiguration;
   const dim3 sums((unsigned)ctas);
-  FWD_EB_TRY(a.accumulate ? launch_sums<TG, VE, true>(pl, sums, sorted, st) : launch_sums<TG, VE, false>(pl, sums, sorted, st));
+  const bool f16 = sizeof(TG) == 2, same = (a.gt_f16 != 0) == f16 && (a.table_f16 != 0) == f16;
+  if (a.accumulate) FWD_EB_TRY(same ? launch_sums<TG, VE, true, true>(pl, sums, sorted, st) : launch_sums<TG, VE, true, false>(pl, sums, sorted, st));
+  else FWD_EB_TRY(same ? launch_sums<TG, VE, false, true>(pl, sums, sorted, st) : launch_sums<TG, VE, false, false>(pl, sums, sorted, st));
   if (a.super) {
-    const dim3 blocks((unsigned)((a.runs / kRun + 7) / 8), tiles);
+    const dim3 blocks((unsigned)(a.runs / kRun), tiles);
     FWD_EB_TRY(launch_pdl(segment_block_kernel<VE>, blocks, 256, 0, st, a, sorted));
   }
   if (a.runs > 1) {
