@@ -8,8 +8,11 @@
 // as integers), and no value is read or written twice.
 //
 // States of 32 bits are bound by memory whatever the code does.  With states of 8 bits the bytes
-// shrink to a third and the instructions grow, so both count there: whole chunks run
-// a loop without bounds checks in which the next turn's loads are under way.
+// shrink to a third and the instructions grow, so both count there: a whole chunk's two turns are loaded
+// at once, without bounds checks, and all arithmetic is on pairs (sm_100's packed fp32).
+// Measured on B200, of the copy rate measured there: 128 M fp16 parameters with master copies and
+// states of 32 bits 524 us, 1.04; 100 M in 26 tensors with states of 8 bits 174 us, 0.89 (32 instructions
+// an element: latency and issue slots bound it together).
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -23,7 +26,7 @@ namespace {
 constexpr int kAdamThreads = 256;
 constexpr int kLane = 8;                                // elements a lane handles at a time
 constexpr int kTurn = kAdamThreads * kLane;              // elements a CTA handles at a time
-constexpr int kMostTurns = 8;                           // turns of a chunk, at most
+constexpr int kMostTurns = 2;                           // turns of a chunk, at most
 constexpr int kMost = 256;                              // tensors of a launch
 static_assert(32 * kLane == FWD_EB_ADAMW_BLOCK, "a warp's elements are one block of an 8-bit state");
 
@@ -217,37 +220,42 @@ __device__ __forceinline__ void square(float (&v)[kLane]) {   // of codes: exact
   }
 }
 
-// 8 elements of any type as they lie in memory: 16-bit types fill half of it.
+// 8 elements as they lie in memory: WIDE of 32 bits, else of 16.
+template <bool WIDE>
 struct Raw {
-  uint4 lo, hi;
-  __device__ __forceinline__ void load(const void* p, bool wide, int at) {
-    if (wide) {
-      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at);
-      lo = q[0];
-      hi = q[1];
-    } else {
-      lo = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(p) + at);
-    }
+  uint4 w[WIDE ? 2 : 1];
+  __device__ __forceinline__ void load(const void* p, int at) {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at * (WIDE ? 4 : 2));
+    w[0] = q[0];
+    if constexpr (WIDE) w[1] = q[1];
   }
   __device__ __forceinline__ void get(int dtype, float (&f)[kLane]) const {
-    if (dtype == FWD_EB_F32) {
-      memcpy(f, &lo, 16);
-      memcpy(f + 4, &hi, 16);
+    if constexpr (WIDE) {
+      memcpy(f, w, sizeof(f));
     } else if (dtype == FWD_EB_F16) {
       Pack<__half, kLane> r;
-      r.w[0] = lo;
+      r.w[0] = w[0];
       r.get(f);
     } else {
       Pack<__nv_bfloat16, kLane> r;
-      r.w[0] = lo;
+      r.w[0] = w[0];
       r.get(f);
     }
   }
 };
 
-template <int CAP, bool BITS8>
-__global__ void __launch_bounds__(kAdamThreads, BITS8 ? 3 : 4)
+// The tensors of a launch are of one kind: 0 has states of 32 bits; 1 to 4 have states of 8, and values of 16 or 32 bits
+// that the step works on and gradients of 16 or 32, so that loads under way hang on no branch.
+constexpr int kKinds = 5;
+inline int kind_of(const fwd_eb_adamw_tensor& t) {
+  if (t.state_bits == 32) return 0;
+  return 1 + (t.master || t.param_dtype == FWD_EB_F32 ? 2 : 0) + (t.grad_dtype == FWD_EB_F32 ? 1 : 0);
+}
+
+template <int CAP, int KIND>
+__global__ void __launch_bounds__(kAdamThreads, KIND < 2 ? 4 : 3)   // the others' loads would spill
 adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
+  constexpr bool BITS8 = KIND != 0, PWIDE = BITS8 && (KIND - 1) / 2 == 1, GWIDE = BITS8 && (KIND - 1) % 2 == 1;
   pdl_enter();
   if (a.s.d_skip && *a.s.d_skip != 0) return;
   int lo = 0, hi = a.count;   // the last tensor whose first chunk is not behind this one
@@ -283,33 +291,33 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   const void* from = t.master ? t.master : t.param;      // what the step works on, and its type
   const int ftype = t.master ? FWD_EB_F32 : t.ptype;
 
-  if (BITS8 && left == chunk && t.aligned && a.s.eps_normal) {
-    Raw p0, g0;
-    uint2 m0, v0;
-    float ms0, vs0;
-    auto fetch = [&](int at) {
-      p0.load(from, ftype == FWD_EB_F32, at);
-      g0.load(t.grad, gsize == 4, at);
-      m0 = *reinterpret_cast<const uint2*>(static_cast<const char*>(t.m) + at);
-      v0 = *reinterpret_cast<const uint2*>(static_cast<const char*>(t.v) + at);
-      ms0 = t.m_scale[at / FWD_EB_ADAMW_BLOCK];
-      vs0 = t.v_scale[at / FWD_EB_ADAMW_BLOCK];
+  if (BITS8 && left == chunk && t.aligned && a.s.eps_normal && a.turns == kMostTurns) {
+    struct Ahead {       // a turn's loads
+      Raw<PWIDE> p;
+      Raw<GWIDE> g;
+      uint2 m, v;
+      float ms, vs;
+    } ahead[2];
+    auto fetch = [&](Ahead& to, int at) {
+      to.p.load(from, at);
+      to.g.load(t.grad, at);
+      to.m = *reinterpret_cast<const uint2*>(static_cast<const char*>(t.m) + at);
+      to.v = *reinterpret_cast<const uint2*>(static_cast<const char*>(t.v) + at);
+      to.ms = t.m_scale[at / FWD_EB_ADAMW_BLOCK];
+      to.vs = t.v_scale[at / FWD_EB_ADAMW_BLOCK];
     };
-    int at = threadIdx.x * kLane;
-    fetch(at);
-    for (int turn = 0; turn < a.turns; ++turn, at += kTurn) {
+    auto turn = [&](const Ahead& now, int at) {
       float p[kLane], g[kLane], m[kLane], v[kLane], root[kLane];
-      p0.get(ftype, p);
-      g0.get(t.gtype, g);
-      decode(m0, m);
-      decode(v0, v);
-      const float keep1 = ms0 * r.beta1, keep2 = vs0 * vs0 * r.beta2;
-      if (turn + 1 < a.turns) fetch(at + kTurn);
+      now.p.get(ftype, p);
+      now.g.get(t.gtype, g);
+      decode(now.m, m);
+      decode(now.v, v);
+      const float keep1 = now.ms * r.beta1, keep2 = now.vs * now.vs * r.beta2;
       square(v);
       update<true>(r, keep1, keep2, p, g, m, v, root);
       float ms, vs;
       const uint2 cm = encode<false>(m, ms), cv = encode<true>(root, vs);
-      if (t.master) store_any<kLane>(t.master, FWD_EB_F32, at, p);
+      if (PWIDE && t.master) store_any<kLane>(t.master, FWD_EB_F32, at, p);
       store_any<kLane>(t.param, t.ptype, at, p);
       *reinterpret_cast<uint2*>(static_cast<char*>(t.m) + at) = cm;
       *reinterpret_cast<uint2*>(static_cast<char*>(t.v) + at) = cv;
@@ -317,7 +325,12 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
         t.m_scale[at / FWD_EB_ADAMW_BLOCK] = ms;
         t.v_scale[at / FWD_EB_ADAMW_BLOCK] = vs;
       }
-    }
+    };
+    const int at = threadIdx.x * kLane;
+    fetch(ahead[0], at);
+    fetch(ahead[1], at + kTurn);
+    turn(ahead[0], at);
+    turn(ahead[1], at + kTurn);
     return;
   }
 
@@ -448,8 +461,8 @@ AdamTensor tensor_of(const fwd_eb_adamw_tensor& t, unsigned first, double lr) {
   return r;
 }
 
-// Fills one launch with the tensors of one state width from *next on, moves *next behind them, launches.
-template <int CAP, bool BITS8>
+// Fills one launch with the tensors of one kind from *next on, moves *next behind them, launches.
+template <int CAP, int KIND>
 cudaError_t launch_some(const fwd_eb_adamw_tensor* ts, int count, int* next, const AdamScalars& s, double lr,
                         cudaStream_t st) {
   AdamArgs<CAP> a = {};
@@ -458,34 +471,34 @@ cudaError_t launch_some(const fwd_eb_adamw_tensor* ts, int count, int* next, con
   long long total = 0;     // turns, at one turn a chunk
   for (int found = 0; end < count && found < CAP; ++end) {
     const fwd_eb_adamw_tensor& t = ts[end];
-    if (t.n == 0 || (t.state_bits == 8) != BITS8) continue;
+    if (t.n == 0 || kind_of(t) != KIND) continue;
     total += (t.n + kTurn - 1) / kTurn;
     ++found;
   }
-  // 8-bit chunks: longer ones where a few waves of CTAs are left even so (100 M elements: 1 turn 293 us, 4 turns 273)
+  // 8-bit chunks of two turns, whose loads are under way together, where a few waves of CTAs are left even so: 100 M
+  // elements 174 us against 293 a turn at a time (202 and 220 with chunks of 4 and 8 turns)
   const long long wave = 3LL * sm_count();
-  a.turns = 1;
-  while (BITS8 && a.turns < kMostTurns && total / (2 * a.turns) >= 4 * wave) a.turns *= 2;
+  a.turns = KIND != 0 && total / kMostTurns >= 4 * wave ? kMostTurns : 1;
   long long chunks = 0;
   for (; *next < end; ++*next) {
     const fwd_eb_adamw_tensor& t = ts[*next];
-    if (t.n == 0 || (t.state_bits == 8) != BITS8) continue;
+    if (t.n == 0 || kind_of(t) != KIND) continue;
     const long long c = (t.n + (long long)a.turns * kTurn - 1) / ((long long)a.turns * kTurn);
     if (chunks + c > INT_MAX) break;     // the rest in a launch of its own
     a.t[a.count++] = tensor_of(t, (unsigned)chunks, lr);
     chunks += c;
   }
   if (chunks == 0) return cudaSuccess;
-  return launch_pdl(adamw_kernel<CAP, BITS8>, dim3((unsigned)chunks), kAdamThreads, 0, st, a);
+  return launch_pdl(adamw_kernel<CAP, KIND>, dim3((unsigned)chunks), kAdamThreads, 0, st, a);
 }
 
-template <bool BITS8>
+template <int KIND>
 cudaError_t launch_all(const fwd_eb_adamw_tensor* ts, int count, const AdamScalars& s, double lr, cudaStream_t st) {
   for (int next = 0; next < count;) {
     const int left = count - next;
-    cudaError_t e = left <= 8    ? launch_some<8, BITS8>(ts, count, &next, s, lr, st)
-                    : left <= 64 ? launch_some<64, BITS8>(ts, count, &next, s, lr, st)
-                                 : launch_some<kMost, BITS8>(ts, count, &next, s, lr, st);
+    cudaError_t e = left <= 8    ? launch_some<8, KIND>(ts, count, &next, s, lr, st)
+                    : left <= 64 ? launch_some<64, KIND>(ts, count, &next, s, lr, st)
+                                 : launch_some<kMost, KIND>(ts, count, &next, s, lr, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -506,10 +519,14 @@ extern "C" int fwd_eb_adamw_step(const fwd_eb_adamw_tensor* tensors, int32_t cou
   if (rc) return rc;
   clear_error();
   const AdamScalars s = scalars_of(cfg);
-  bool any8 = false, any32 = false;
-  for (int i = 0; i < count; ++i) (tensors[i].state_bits == 8 ? any8 : any32) = true;
+  bool any[kKinds] = {};
+  for (int i = 0; i < count; ++i) any[kind_of(tensors[i])] = true;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = any32 ? launch_all<false>(tensors, count, s, cfg->lr, st) : cudaSuccess;
-  if (e == cudaSuccess && any8) e = launch_all<true>(tensors, count, s, cfg->lr, st);
+  cudaError_t e = cudaSuccess;
+  if (any[0]) e = launch_all<0>(tensors, count, s, cfg->lr, st);
+  if (any[1] && e == cudaSuccess) e = launch_all<1>(tensors, count, s, cfg->lr, st);
+  if (any[2] && e == cudaSuccess) e = launch_all<2>(tensors, count, s, cfg->lr, st);
+  if (any[3] && e == cudaSuccess) e = launch_all<3>(tensors, count, s, cfg->lr, st);
+  if (any[4] && e == cudaSuccess) e = launch_all<4>(tensors, count, s, cfg->lr, st);
   return e == cudaSuccess ? 0 : cuda_fail(e, "kernel launch");
 }

@@ -188,7 +188,8 @@ size_t fwd_eb_adamw_config_size(void);
 
 /* One step over `count` tensors (a host array, read before the call returns; it needs not
  * outlive it).  No two tensors may overlap.  Everything is checked before the first launch;
- * one launch covers up to 256 tensors of one state width. */
+ * one launch covers up to 256 tensors of one kind (state width; with 8-bit states also the
+ * widths of values and gradients). */
 int fwd_eb_adamw_step(const fwd_eb_adamw_tensor* tensors, int32_t count,
                       const fwd_eb_adamw_config* cfg, void* stream);
 

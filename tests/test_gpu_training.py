@@ -841,3 +841,35 @@ def test_bag_gradient_small_calls_with_more_bags_than_lookups():
     for mode in MODES:
         s, go, bag, starts = make_bags(6, 20, 12, lengths, mode=mode, dtype=torch.float32, pad=True)
         check_bag(s, go, bag, starts)
+
+
+@pytest.mark.parametrize("param,grad,master", [
+    (torch.float16, torch.float16, False), (torch.bfloat16, torch.float32, False), (torch.float32, torch.bfloat16, False),
+    (torch.float16, torch.float32, True)])
+def test_adamw_8_bits_long_chunks(param, grad, master):
+    """Enough elements that a CTA takes several turns with its loads under way; ragged ends, a tensor at an odd address."""
+    c = adam_case(4, [9_000_001, 12_345_600, 257], param, grad, 8, master)
+    odd = adam_case(5, [4_000_003], param, grad, 8, master, 1)
+    for k in c:
+        if c[k] is not None:
+            c[k] = c[k] + odd[k]
+    check_adam(c, 8, step=2, grad_scale=0.5)
+
+
+def test_adamw_mixed_kinds_in_one_step():
+    """Parameters, gradients and master copies of every width side by side, more than one launch covers."""
+    cases = [adam_case(7 + i, [300 + 41 * i, 5], p, g, 8, m) for i, (p, g, m) in enumerate(
+        (p, g, m) for p in DTYPES for g in DTYPES for m in (False, True) if not (m and p == torch.float32))]
+    c = {k: [t for x in cases for t in (x[k] if x[k] is not None else [None] * 2)] for k in cases[0]}
+    solo = [T.AdamW(x["params"], state_bits=8, masters=x["masters"], exp_avg=[t.clone() for t in x["m"]],
+                    exp_avg_sq=[t.clone() for t in x["v"]], exp_avg_scale=[t.clone() for t in x["ms"]],
+                    exp_avg_sq_scale=[t.clone() for t in x["vs"]], **HYPER) for x in
+            [{k: [t.clone() if t is not None else None for t in v] if v is not None else None for k, v in x.items()} for x in cases]]
+    opt = T.AdamW(c["params"], state_bits=8, masters=c["masters"], exp_avg=c["m"], exp_avg_sq=c["v"], exp_avg_scale=c["ms"],
+                  exp_avg_sq_scale=c["vs"], **HYPER)
+    opt.step(c["grads"])
+    for o, x in zip(solo, cases):
+        o.step(x["grads"])
+    got = [t for o in solo for t in o.params]
+    assert all(same_bits(a, b) for a, b in zip(opt.params, got))
+    assert all(same_bits(a, b) for a, b in zip(opt.exp_avg_sq, [t for o in solo for t in o.exp_avg_sq]))
