@@ -257,7 +257,7 @@ PyObject* embedding_bag_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (table.dim() != 2 || (table.size(1) > 1 && table.size(0) > 0 && table.stride(1) != 1))
       value_error("table must be 2-D with unit column stride");
     const int64_t rows = table.size(0), dim = table.size(1);
-    if (dim > (1 << 24)) value_error("table has too many columns");
+    if (dim > INT32_MAX) value_error("table has too many columns");
     if (!indices.is_contiguous()) value_error("indices must be contiguous");
     const int64_t count = indices.numel();
     const bool gather = mode == FWD_EB_MODE_GATHER;

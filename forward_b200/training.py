@@ -240,7 +240,8 @@ class AdamW:
     exp_avg_sq_scale): the value of element i is float(code[i]) * scale[i // 256].  masters[i], fp32, is
     the copy that the step works on where parameter i is fp16 or bf16; the parameter is then
     its rounded image.  The state tensors may be given (to resume); otherwise they start at zero.
-    weight_decay is a number, or one per tensor.
+    weight_decay is a number, or one per tensor.  The optimizer addresses the tensors' memory: a tensor that
+    is given other memory (p.data = ...) needs a new one.
 
     capturable=True keeps the step count and lr on the device (step_tensor, lr_tensor): a step
     captured into a graph then counts on with every replay, and lr may be changed in between.
@@ -283,6 +284,9 @@ class AdamW:
             self._check(p, f"params[{i}]", p.numel())
             _dtype(p, f"params[{i}]")
         sizes = [p.numel() for p in self.params]
+        addresses = [p.data_ptr() for p in self.params if p.numel()]
+        if len(set(addresses)) < len(addresses):
+            raise ValueError("a parameter is in the list twice")
         self.masters = [None] * n if masters is None else list(masters)
         if len(self.masters) != n:
             raise ValueError("masters: one tensor (or None) per parameter")

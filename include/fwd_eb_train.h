@@ -56,7 +56,7 @@ enum {
  * FWD_EB_BACKWARD_ACCUMULATE every element of those rows is written (zeros where no lookup
  * falls); elements between rows (stride > dim) are left as they are.
  *
- * Limits: num_indices, num_bags < 2^31 - 65536 and dim <= 2^24 (FWD_EB_ETOOBIG); FWD_EB_FLAG_OFFSET_PAIRS
+ * Limits: num_indices, num_bags < 2^31 - 65536 and dim <= 2^20 (FWD_EB_ETOOBIG); FWD_EB_FLAG_OFFSET_PAIRS
  * is not supported (FWD_EB_EUNSUPPORTED).  Offsets must not decrease; offsets that do give
  * an unspecified gradient but never an access outside the buffers.
  */

@@ -4,8 +4,8 @@ Tolerances are bounds of the arithmetic, not fitted numbers.  U = 2^-24 is half 
 fp32 terms is off by at most k * U * (sum of magnitudes) whatever its order; a result is
 rounded once to its type, which moves it by at most half a step of that type (`half_step`).
 """
-import ctypes as C
 import math
+import os
 
 import pytest
 
@@ -136,13 +136,30 @@ def check_bag(s, grad_out, bag, starts, *, mean_raw=False, grad_dtype=None, need
 MODES = [capi.MODE_SUM, capi.MODE_MEAN, capi.MODE_MAX, capi.MODE_SQUARE_SUM, capi.MODE_GATHER]
 
 
+# calls of one launch, of a sort in one CTA, of a sort by tiles
+TIMES = [1, 10, 30]
+
+
+@pytest.mark.parametrize("times", TIMES)
 @pytest.mark.parametrize("dim", [1, 3, 8, 40, 64, 128, 200, 256, 520])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 @pytest.mark.parametrize("mode", MODES)
-def test_bag_gradient(mode, dtype, dim):
-    lengths = [0, 1, 7, 0, 33, 64, 31, 32, 2, 5, 0]
-    s, go, bag, starts = make_bags(dim, 37, dim, lengths, mode=mode, dtype=dtype, pad=dim % 2 == 0, hot=0.3)
+def test_bag_gradient(mode, dtype, dim, times):
+    lengths = [0, 1, 7, 0, 33, 64, 31, 32, 2, 5, 0] * times
+    s, go, bag, starts = make_bags(dim, 37 * times, dim, lengths, mode=mode, dtype=dtype, pad=dim % 2 == 0, hot=0.3)
     check_bag(s, go, bag, starts)
+
+
+@pytest.mark.parametrize("times", TIMES)
+@pytest.mark.parametrize("table,grad", [(torch.float32, torch.float16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("mode", MODES)
+def test_bag_gradient_types_apart(mode, table, grad, times):
+    """grad_out of another type than the table, the gradient of either's; weights where the mode has them."""
+    lengths = [3, 0, 50, 97, 25] * times
+    s, go, bag, starts = make_bags(times, 41 * times, 72, lengths, mode=mode, dtype=table, hot=0.2,
+                                   weighted=mode == capi.MODE_SUM)
+    for out in (table, grad):
+        check_bag(s, go.to(grad), bag, starts, grad_dtype=out)
 
 
 @pytest.mark.parametrize("n,rows,hot", [(1, 1, 0), (31, 1, 0), (32, 1, 0), (33, 2, 0), (64, 1, 0), (1024, 1, 0),
@@ -156,68 +173,80 @@ def test_bag_gradient_runs_and_sort_sizes(n, rows, hot):
     check_bag(s, go, bag, starts)
 
 
+@pytest.mark.parametrize("times", TIMES)
 @pytest.mark.parametrize("mode", MODES)
 @pytest.mark.parametrize("idx", [torch.int32, torch.int64])
-def test_bag_gradient_windows_and_forms(mode, idx):
+def test_bag_gradient_windows_and_forms(mode, idx, times):
     """A row window with indices on both sides of it, 64-bit indices, include_last_offset, fixed lengths."""
-    lengths = [5] * 40
+    lengths = [5] * 40 * times
     for window, last, fixed in ((1000, False, 0), (0, True, 0), (7, False, 5)):
         s, go, bag, starts = make_bags(window, 50, 20, lengths, mode=mode, dtype=torch.float16, idx=idx, pad=True,
                                        window=window, include_last=last and mode != capi.MODE_GATHER, fixed=fixed)
         check_bag(s, go, bag, starts, grad_dtype=torch.float32)
 
 
-def test_bag_gradient_lookups_outside_every_bag():
+@pytest.mark.parametrize("times", TIMES)
+def test_bag_gradient_lookups_outside_every_bag(times):
     """Lookups before the first offset and behind the last (include_last_offset) belong to no bag."""
     g = gen(5)
+    n = 100 * times + 1000 * (times > 1)
     table = torch.randn(11, 16, generator=g, device=DEV)
-    index = torch.randint(0, 11, (100,), generator=g, device=DEV, dtype=torch.int32)
-    offsets = torch.tensor([10, 10, 40, 90], device=DEV, dtype=torch.int32)
+    index = torch.randint(0, 11, (n,), generator=g, device=DEV, dtype=torch.int32)
+    edges = [n // 10, n // 10, n // 2, n - 10]
+    offsets = torch.tensor(edges, device=DEV, dtype=torch.int32)
     go = torch.randn(3, 16, generator=g, device=DEV)
-    w = torch.rand(100, generator=g, device=DEV)
+    w = torch.rand(n, generator=g, device=DEV)
     got, gw = T.embedding_bag_backward(go, table, index, offsets, include_last_offset=True, per_sample_weights=w,
                                        need_weights=True)
-    ref = torch.zeros(11, 16, dtype=F64, device=DEV)
-    for b, (s, e) in enumerate(((10, 10), (10, 40), (40, 90))):
+    ref, mag = (torch.zeros(11, 16, dtype=F64, device=DEV) for _ in range(2))
+    for b in range(3):
+        s, e = edges[b], edges[b + 1]
         ref.index_add_(0, index[s:e].long(), w[s:e, None].to(F64) * go[b].to(F64))
-    within(got, ref, 100 * U * ref.abs().max() * 10, "grad_table")
-    assert (gw[:10] == 0).all() and (gw[90:] == 0).all() and (gw[10:90] != 0).all()
+        mag.index_add_(0, index[s:e].long(), w[s:e, None].to(F64) * go[b].to(F64).abs())
+    within(got, ref, (n + 16) * U * mag, "grad_table")
+    assert (gw[:edges[0]] == 0).all() and (gw[edges[3]:] == 0).all() and (gw[edges[0]:edges[3]] != 0).all()
 
 
+@pytest.mark.parametrize("longest", [700, 2500, 9000])
 @pytest.mark.parametrize("mean_raw", [False, True])
-def test_bag_gradient_mean_counts(mean_raw):
-    lengths = [0, 3, 1, 700, 2, 2]
+def test_bag_gradient_mean_counts(mean_raw, longest):
+    lengths = [0, 3, 1, longest, 2, 2]
     s, go, bag, starts = make_bags(3, 9, 24, lengths, mode=capi.MODE_MEAN, dtype=torch.float32, pad=True)
     s["indices"][0:3] = s["padding_idx"]     # a bag of nothing but padding
     check_bag(s, go, bag, starts, mean_raw=mean_raw)
 
 
+@pytest.mark.parametrize("times", TIMES)
+@pytest.mark.parametrize("dim", [48, 7, 300])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
-@pytest.mark.parametrize("mode", [capi.MODE_SUM, capi.MODE_SQUARE_SUM, capi.MODE_MAX])
-def test_bag_gradient_accumulates(mode, dtype):
-    s, go, bag, starts = make_bags(8, 60, 48, [9, 0, 20, 1], mode=mode, dtype=dtype)
-    old = torch.randn(60, 48, generator=gen(9), device=DEV).to(dtype)
+@pytest.mark.parametrize("mode", [capi.MODE_SUM, capi.MODE_MEAN, capi.MODE_SQUARE_SUM, capi.MODE_MAX])
+def test_bag_gradient_accumulates(mode, dtype, dim, times):
+    rows = 6000
+    s, go, bag, starts = make_bags(8, rows, dim, [90, 0, 77, 1] * times, mode=mode, dtype=dtype, hot=0.3)
+    old = torch.randn(rows, dim, generator=gen(9), device=DEV).to(dtype)
     buf = old.clone()
     got, _, _ = check_bag(s, go, bag, starts, old=old, grad_table=buf)
     assert got is buf
-    untouched = torch.ones(60, dtype=torch.bool, device=DEV)
+    untouched = torch.ones(rows, dtype=torch.bool, device=DEV)
     untouched[s["indices"].long()] = False
     assert untouched.any() and same_bits(buf[untouched], old[untouched])
 
 
+@pytest.mark.parametrize("times", TIMES)
 @pytest.mark.parametrize("offset,stride", [(0, 40), (1, 40), (0, 41), (3, 57), (8, 48)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
-def test_bag_gradient_strides(dtype, offset, stride):
+def test_bag_gradient_strides(dtype, offset, stride, times):
     """Rows at odd addresses and strides; what lies between and around them stays."""
     def strided(rows, fill):
         flat = torch.full((rows * stride + offset + 64,), fill, dtype=dtype, device=DEV)
         return flat, flat[offset:offset + rows * stride].view(rows, stride)[:, :40]
-    s, go, bag, starts = make_bags(offset, 30, 40, [4, 0, 90, 2], mode=capi.MODE_SUM, dtype=dtype)
-    _, table = strided(30, 0.0)
+    rows = 30 if times == 1 else 5000
+    s, go, bag, starts = make_bags(offset, rows, 40, [4, 0, 190, 2] * times, mode=capi.MODE_SUM, dtype=dtype)
+    _, table = strided(rows, 0.0)
     table.copy_(s["table"])
-    _, grad_out = strided(4, 0.0)
+    _, grad_out = strided(4 * times, 0.0)
     grad_out.copy_(go)
-    flat, buf = strided(30, 7.0)
+    flat, buf = strided(rows, 7.0)
     s["table"] = table
     check_bag(s, grad_out, bag, starts, grad_table=buf)
     buf.fill_(7.0)
@@ -303,6 +332,34 @@ def test_bag_gradient_against_differences():
     scale = 24 * 26 * float(go.abs().max()) * 5 * 5
     assert abs(float(by_table - (got.to(F64) * d.to(F64)).sum())) <= 20 * U * scale
     assert abs(float(by_weight - (gw.to(F64) * dw.to(F64)).sum())) <= 20 * U * scale
+
+
+def test_bag_gradient_winners_of_long_bags():
+    """Positions past 255, which are compared whole, next to bags of 255 and 256 lookups and rows without a winner."""
+    for dim, dtype in ((24, torch.float16), (5, torch.float32), (64, torch.float32)):
+        s, go, bag, starts = make_bags(dim, 900, dim, [255, 256, 257, 1, 0, 4000, 254, 70_000], mode=capi.MODE_MAX, dtype=dtype,
+                                       pad=True)
+        check_bag(s, go, bag, starts)
+
+
+def test_bag_gradient_past_32_bits():
+    """A table of more than 2^31 elements: rows at both ends of it, zeros everywhere else."""
+    rows, dim = 17_000_000, 128
+    table = torch.empty(rows, dim, dtype=torch.float16, device=DEV)
+    index = torch.tensor([0, rows - 1, rows - 2, rows // 2, rows - 1] * 400, device=DEV)
+    go = torch.randn(2000, dim, generator=gen(1), device=DEV).half()
+    off = torch.arange(2000, device=DEV)
+    got, _ = T.embedding_bag_backward(go, table, index, off)
+    want = torch.zeros(5, dim, dtype=F64, device=DEV)
+    for k, slot in enumerate((0, 1, 2, 3, 1)):
+        want[slot] += go[k::5].to(F64).sum(0)
+    for slot, r in enumerate((0, rows - 1, rows - 2, rows // 2)):
+        within(got[r], want[slot], 900 * U * 900 * 5, f"row {r}")
+        got[r] = 0
+    assert not got.view(torch.int16).any()
+    acc = torch.zeros_like(got)
+    T.embedding_bag_backward(go, table, index, off, grad_table=acc, accumulate=True)
+    within(acc[rows - 1], want[1], 900 * U * 900 * 5, "accumulated")
 
 
 def test_bag_gradient_refusals():
@@ -527,6 +584,21 @@ def test_layer_norm_gradient_against_differences():
         diff = float(at(e) - at(-e)) / (2 * e)
         # the difference's own error: e^2 of the third derivative (rstd ~ 1, values of a few), 1e-16 / e of rounding
         assert abs(diff - float((grad.to(F64) * d).sum())) <= 100 * U * float((grad.to(F64) * d).abs().sum()) + 1e-5
+
+
+def test_layer_norm_past_32_bits():
+    x = torch.empty(70_000, 32_768, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = rows_of(3, 32_768, torch.bfloat16, 1)
+    x[:-3] = 1.0
+    y, mean, rstd = T.layer_norm(x, return_stats=True)
+    assert same_bits(y[-3:], T.layer_norm(x[-3:].clone())) and not y[:-3].any()
+    gy = torch.zeros_like(x)
+    gy[-3:] = rows_of(3, 32_768, torch.bfloat16, 2)
+    gx, gw, gb = T.layer_norm_backward(gy, x, mean, rstd, grad_x=gy)
+    check_ln_backward(rows_of(3, 32_768, torch.bfloat16, 2), x[-3:], mean[-3:], rstd[-3:], None)
+    three = rows_of(3, 32_768, torch.bfloat16, 2).to(F64)        # every other row adds zeros
+    within(gb, three.sum(0), 3 * U * three.abs().sum(0), "grad_bias")
+    assert not gx[:-3].any()
 
 
 def test_layer_norm_refusals():
@@ -755,8 +827,47 @@ def test_adamw_device_scalars(bits):
     assert all(same_bits(p, q) for p, q in zip(before, c2["params"] + c2["m"] + c2["v"]))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_past_32_bits(bits):
+    """A tensor of more than 2^31 elements steps at its end as a short one does."""
+    n, tail = 2**31 + 5000, 2048 + 136          # the last blocks: the tail starts on a block's border
+    assert (n - tail) % 256 == 0
+    p = torch.full((n,), 0.5, dtype=torch.bfloat16, device=DEV)
+    g = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    g[-tail:] = torch.randn(tail, generator=gen(1), device=DEV).bfloat16()
+    q, h = p[-tail:].clone(), g[-tail:].clone()
+    opt, short = (T.AdamW([t], state_bits=bits, **HYPER) for t in (p, q))
+    opt.step([g])
+    short.step([h])
+    assert same_bits(p[-tail:], q) and same_bits(opt.exp_avg_sq[0][-tail:], short.exp_avg_sq[0])
+    assert (p[:1000] == p[0]).all() and float(p[0]) == float(torch.tensor(0.5 * (1 - 0.01 * 0.1)).bfloat16())
+
+
+def test_the_first_call_may_be_captured():
+    """Nothing is set up on first use that a stream capture forbids: each operator's first call in a process."""
+    import subprocess
+    import sys
+    code = (
+        "import sys, torch; sys.path.insert(0, {root!r})\n"
+        "from forward_b200 import training as T\n"
+        "x = torch.randn(600, 2000, device='cuda'); w = torch.ones(2000, device='cuda'); s = torch.ones(600, device='cuda')\n"
+        "t = torch.randn(5000, 64, device='cuda'); i = torch.zeros(9000, dtype=torch.int32, device='cuda')\n"
+        "o = torch.arange(0, 9000, 9, dtype=torch.int32, device='cuda'); go = torch.randn(1000, 64, device='cuda')\n"
+        "opt = T.AdamW([t], state_bits=8); opt.bind([torch.ones_like(t)])\n"
+        "torch.cuda.synchronize(); g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    y = T.layer_norm(x, w); r = T.layer_norm_backward(x, x, s, s, w)\n"
+        "    b = T.embedding_bag_backward(go, t, i, o)[0]; c = T.embedding_bag_backward(go[:10], t, i[:90], o[:10])[0]; opt.step()\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "assert torch.equal(y, T.layer_norm(x, w)) and torch.equal(b, T.embedding_bag_backward(go, t, i, o)[0])\n"
+        "assert (b[0] != 0).any() and (c[0] != 0).any()\n"
+    ).format(root=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
 def test_adamw_refusals():
     p = torch.zeros(10, device=DEV)
+    pytest.raises(ValueError, T.AdamW, [p, p])
     bad = lambda exc, *a, **k: pytest.raises(exc, T.AdamW, *a, **k)  # noqa: E731
     bad(TypeError, [p.double()])
     bad(ValueError, [torch.zeros(4, 4, device=DEV).t()[1:]])
