@@ -31,8 +31,8 @@ namespace {
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kItems = 9;                          // pairs a thread ranks at a time
-constexpr int kSubTile = kSortThreads * kItems;
+// Pairs a thread of the sort ranks at a time: 5 where they cover a tile (2560 pairs), else 9.
+constexpr int kItemsFew = 5, kItemsMany = 9;
 constexpr int kSmallItems = 7;                     // ... in the kernel that sorts all of a small call
 constexpr int kSmall = kSortThreads * kSmallItems;
 constexpr int kTiny = 2 * kSortThreads;            // lookups of a call that one launch does
@@ -76,6 +76,7 @@ struct BackArgs {
   uint2* pairs[2];        // [n] {row, payload}
   int by_bag;             // the payload is the bag (-1 with a row of num_rows), else the lookup
   unsigned* hist;         // [tiles][kDigits]: pairs of a tile by digit
+  unsigned* hist16;       // [passes][(tiles + 15) / 16][kDigits]: of 16 tiles
   float* partial;         // [runs][2][pstride]: sums of a run's first row, when it began before the run,
                           // and of its last, when it began in the run and goes on
   float* super;           // [runs / 32][pstride]
@@ -237,8 +238,25 @@ __device__ __forceinline__ void uncount_padding(const BackArgs& a, long long idx
   if (pad && (threadIdx.x & 31) == __ffs(same) - 1) atomicSub(a.counted + bag, __popc(same));
 }
 
+// Zeros where the sums of 16 tiles will be counted.
+__global__ void __launch_bounds__(kSortThreads) clear_sums_kernel(unsigned* hist16, int words) {
+  pdl_enter();
+  const int i = blockIdx.x * kSortThreads + threadIdx.x;
+  if (i < words) hist16[i] = 0;
+}
+
+// A tile's histogram, and its share of the sums of 16 tiles.
+__device__ __forceinline__ void put_counts(const BackArgs& a, const unsigned* count, int pass) {
+  unsigned* sums = a.hist16 + (pass * ((a.tiles + 15) / 16) + blockIdx.x / 16) * kDigits;
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) {
+    a.hist[blockIdx.x * kDigits + d] = count[d];
+    if (count[d]) atomicAdd(sums + d, count[d]);
+  }
+}
+
 // Every lookup's pair (and bag, where it is wanted apart), and the histogram of the first digit.  A warp takes consecutive
 // lookups; all its indices are asked for at once (they may come from DRAM, a microsecond and a half a round).
+template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs a, uint2* to) {
   pdl_enter();
   __shared__ unsigned count[kDigits];
@@ -249,10 +267,10 @@ __global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int share = (a.tile / 32 + kSortWarps - 1) / kSortWarps * 32;
   const int first = begin + warp * share, last = min(end, first + share);
-  long long index[kItems];
+  long long index[ITEMS];
   auto fetch = [&](int base) {
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       const int j = base + i * 32 + lane;
       index[i] = j < last ? index_at(a.indices, a.idx64, j) : 0;
     }
@@ -262,9 +280,9 @@ __global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs
   __syncthreads();
   BagWalk walk = walk_from(a, first, t, starts);
   const unsigned mask = (1u << a.bits) - 1u;
-  for (int base = first; base < last; base += kItems * 32) {
+  for (int base = first; base < last; base += ITEMS * 32) {
     if (base != first) fetch(base);
-    walk_bags<kItems>(a, base, last, t, starts, walk, [&](int i, int bag) {
+    walk_bags<ITEMS>(a, base, last, t, starts, walk, [&](int i, int bag) {
       const int j = base + i * 32 + lane;
       if (j < last) {
         if (a.bag_of) a.bag_of[j] = bag;
@@ -278,12 +296,11 @@ __global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs
     });
   }
   __syncthreads();
-  if (to) {
-    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) a.hist[blockIdx.x * kDigits + d] = count[d];
-  }
+  if (to) put_counts(a, count, 0);
 }
 
 // The histogram of a later digit.
+template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const BackArgs a, const uint2* from, int pass) {
   pdl_enter();
   __shared__ unsigned count[kDigits];
@@ -292,20 +309,20 @@ __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const Back
   const int begin = blockIdx.x * a.tile;
   const int end = min(a.n, begin + a.tile);
   const unsigned mask = (1u << a.bits) - 1u;
-  for (int base = begin; base < end; base += kSubTile) {
-    unsigned key[kItems];
+  for (int base = begin; base < end; base += ITEMS * kSortThreads) {
+    unsigned key[ITEMS];
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       const int j = base + i * kSortThreads + threadIdx.x;
       key[i] = j < end ? __ldg(&from[j].x) : 0;
     }
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       if (base + i * kSortThreads + (int)threadIdx.x < end) atomicAdd(&count[(key[i] >> (pass * a.bits)) & mask], 1u);
     }
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) a.hist[blockIdx.x * kDigits + d] = count[d];
+  put_counts(a, count, pass);
 }
 
 // Ranks of a CTA's items among those of the same digit, in the order of (warp, item, lane): in the warp here, and
@@ -371,43 +388,51 @@ __device__ __forceinline__ unsigned digits_below(unsigned mine, unsigned* total)
 }
 
 // Moves a tile's pairs to their place in the order of digit `pass`, ties in the order they came.
+template <int ITEMS>
 struct DigitShared {
-  uint2 pairs[kSubTile];                   // in the digit's order
+  uint2 pairs[ITEMS * kSortThreads];                   // in the digit's order
   unsigned in_warp[kSortWarps][kDigits];
   unsigned place[kDigits];                 // next free place of a digit
   unsigned local[kDigits];                 // first place of a digit in `pairs`
   unsigned total[kDigits / 32];
 };
+template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_digit_kernel(const BackArgs a, const uint2* from, uint2* to, int pass) {
   pdl_enter();
   extern __shared__ uint4 dynamic[];
-  DigitShared& s = *reinterpret_cast<DigitShared*>(dynamic);
+  DigitShared<ITEMS>& s = *reinterpret_cast<DigitShared<ITEMS>*>(dynamic);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int begin = blockIdx.x * a.tile;
   const int end = min(a.n, begin + a.tile);
   const int shift = pass * a.bits;
   const unsigned mask = (1u << a.bits) - 1u;
-  uint2 pair[kItems];
+  uint2 pair[ITEMS];
   auto fetch = [&](int base) {
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int j = base + (warp * kItems + i) * 32 + lane;
+    for (int i = 0; i < ITEMS; ++i) {
+      const int j = base + (warp * ITEMS + i) * 32 + lane;
       pair[i] = j < end ? __ldg(from + j) : make_uint2(0, 0);
     }
   };
   fetch(begin);
   // place[d] = keys with a lower digit + keys with digit d in earlier tiles: 4 digits a thread, and the tiles
-  // shared among the threads of a digit, so that a thread's loads are few and all under way together
+  // shared among the threads of a digit, so that a thread's loads are few and all under way together.  Sums of 16
+  // tiles stand for all tiles but the 16 around this one (293 tiles: 3 us less a digit)
   {
     const int digits = (int)mask + 1, columns = digits < 4 ? 1 : digits / 4, groups = min(kSortThreads / columns, 32);
     const int column = threadIdx.x % columns, group = threadIdx.x / columns;
     uint4 all = make_uint4(0, 0, 0, 0), before = all;
     if (group < groups) {
-#pragma unroll 10
-      for (int t = group; t < a.tiles; t += groups) {
-        const uint4 c = reinterpret_cast<const uint4*>(a.hist + t * kDigits)[column];
-        const unsigned m = t < (int)blockIdx.x ? 0xffffffffu : 0u;
-        all.x += c.x, all.y += c.y, all.z += c.z, all.w += c.w;
+      const int sums = (a.tiles + 15) / 16, mine = (int)blockIdx.x / 16;
+      const unsigned* hist16 = a.hist16 + pass * sums * kDigits;
+      const unsigned* near = a.hist + mine * 16 * kDigits;           // the tiles that are looked at one by one
+      const int rows = sums + (int)blockIdx.x - mine * 16;
+#pragma unroll 6
+      for (int r = group; r < rows; r += groups) {
+        const uint4 c = reinterpret_cast<const uint4*>(r < sums ? hist16 + r * kDigits : near + (r - sums) * kDigits)[column];
+        const unsigned w = r < sums ? 0xffffffffu : 0u;                       // of the whole count
+        const unsigned m = r < mine || r >= sums ? 0xffffffffu : 0u;          // in earlier tiles
+        all.x += c.x & w, all.y += c.y & w, all.z += c.z & w, all.w += c.w & w;
         before.x += c.x & m, before.y += c.y & m, before.z += c.z & m, before.w += c.w & m;
       }
     }
@@ -431,18 +456,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_digit_kernel(const BackArgs
     if (threadIdx.x < kDigits) s.place[threadIdx.x] = lower + earlier;
     __syncthreads();
   }
-  for (int base = begin; base < end; base += kSubTile) {
+  for (int base = begin; base < end; base += (ITEMS * kSortThreads)) {
     if (base != begin) {
       __syncthreads();
       fetch(base);
     }
-    unsigned digit[kItems], rank[kItems];
+    unsigned digit[ITEMS], rank[ITEMS];
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      const int j = base + (warp * kItems + i) * 32 + lane;
+    for (int i = 0; i < ITEMS; ++i) {
+      const int j = base + (warp * ITEMS + i) * 32 + lane;
       digit[i] = j < end ? (pair[i].x >> shift) & mask : kNone;
     }
-    rank_items<kItems>(digit, rank, s.in_warp, a.bits);
+    rank_items<ITEMS>(digit, rank, s.in_warp, a.bits);
     unsigned sum = 0;
     if (threadIdx.x < kDigits) {
 #pragma unroll
@@ -462,13 +487,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_digit_kernel(const BackArgs
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       if (digit[i] != kNone) s.pairs[s.in_warp[warp][digit[i]] + rank[i]] = pair[i];
     }
     __syncthreads();
-    const int count = min(kSubTile, end - base);
+    const int count = min((ITEMS * kSortThreads), end - base);
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
+    for (int i = 0; i < ITEMS; ++i) {
       const int k = i * kSortThreads + threadIdx.x;
       if (k >= count) continue;
       const uint2 p = s.pairs[k];
@@ -1569,6 +1594,7 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
     a.pairs[0] = reinterpret_cast<uint2*>(ws + take(n * 8));
     a.pairs[1] = reinterpret_cast<uint2*>(ws + take(n * 8));
     a.hist = reinterpret_cast<unsigned*>(ws + take((size_t)a.tiles * kDigits * 4));
+    a.hist16 = reinterpret_cast<unsigned*>(ws + take((size_t)a.passes * ((a.tiles + 15) / 16) * kDigits * 4));
     a.partial = reinterpret_cast<float*>(ws + take((size_t)a.runs * 2 * a.pstride * 4));
     const int blocks = a.runs / kRun;
     const size_t super = take((size_t)blocks * a.pstride * 4);
@@ -1673,6 +1699,29 @@ cudaError_t launch_weights(const BackPlan& pl, cudaStream_t st) {
   }
 }
 
+// Pairs into pairs[1], then from one buffer to the other a digit at a time.
+template <int ITEMS>
+cudaError_t launch_sort(const BackPlan& pl, cudaStream_t st) {
+  const BackArgs& a = pl.a;
+  const dim3 tiles((unsigned)a.tiles);
+  uint2* first = pl.want_table ? a.pairs[1] : nullptr;
+  if (first) {
+    const int words = a.passes * ((a.tiles + 15) / 16) * kDigits;
+    FWD_EB_TRY(launch_pdl(clear_sums_kernel, dim3((unsigned)((words + kSortThreads - 1) / kSortThreads)), kSortThreads, 0, st,
+                          a.hist16, words));
+  }
+  FWD_EB_TRY(launch_pdl(make_pairs_kernel<ITEMS>, tiles, kSortThreads, 0, st, a, first));
+  int now = 1;
+  for (int pass = 0; pass < a.passes; ++pass, now ^= 1) {
+    const uint2* from = a.pairs[now];
+    if (pass > 0) FWD_EB_TRY(launch_pdl(sort_histogram_kernel<ITEMS>, tiles, kSortThreads, 0, st, a, from, pass));
+    constexpr int bytes = (int)sizeof(DigitShared<ITEMS>);
+    FWD_EB_TRY(allow_shared<sort_digit_kernel<ITEMS>, bytes>());
+    FWD_EB_TRY(launch_pdl(sort_digit_kernel<ITEMS>, tiles, kSortThreads, bytes, st, a, from, a.pairs[now ^ 1], pass));
+  }
+  return cudaSuccess;
+}
+
 cudaError_t launch_backward(const BackPlan& pl, const fwd_eb_backward_params* p, cudaStream_t st) {
   const BackArgs& a = pl.a;
   if (a.n == 0) return a.zero_blocks > 0 ? launch_pdl(zero_kernel, dim3((unsigned)a.zero_blocks), 256, 0, st, a) : cudaSuccess;
@@ -1688,16 +1737,8 @@ cudaError_t launch_backward(const BackPlan& pl, const fwd_eb_backward_params* p,
   if (a.n <= kSmall && pl.want_table) {
     FWD_EB_TRY(launch_pdl(sort_small_kernel, dim3(1), kSortThreads, 0, st, a, a.pairs[0]));
   } else {
-    const dim3 tiles((unsigned)a.tiles);
-    uint2* first = pl.want_table ? a.pairs[1] : nullptr;
-    FWD_EB_TRY(launch_pdl(make_pairs_kernel, tiles, kSortThreads, 0, st, a, first));
-    now = 1;
-    for (int pass = 0; pass < a.passes; ++pass, now ^= 1) {
-      const uint2* from = a.pairs[now];
-      if (pass > 0) FWD_EB_TRY(launch_pdl(sort_histogram_kernel, tiles, kSortThreads, 0, st, a, from, pass));
-      FWD_EB_TRY(allow_shared<sort_digit_kernel, (int)sizeof(DigitShared)>());
-      FWD_EB_TRY(launch_pdl(sort_digit_kernel, tiles, kSortThreads, sizeof(DigitShared), st, a, from, a.pairs[now ^ 1], pass));
-    }
+    FWD_EB_TRY(a.tile <= kItemsFew * kSortThreads ? launch_sort<kItemsFew>(pl, st) : launch_sort<kItemsMany>(pl, st));
+    now = (1 + a.passes) & 1;
   }
   if (a.grad_weights && !pl.fused_weights) {
     const bool g16 = p->grad_out_dtype == FWD_EB_F16;
