@@ -14,8 +14,8 @@
 // of runs are first added 32 at a time.  Every sum has one order, whatever the schedule.
 //
 // Measured on B200 (a call, of the copy rate measured there): 655 k Zipf lookups of a 1 M x 128 fp16 table, mean, dense gradient
-// 132 us, 0.30: sort 50, sums beside zeros 66, joins 12; 262 k of a 1 M x 256 fp16 table, max 160 us, 0.51; 1.3 M weighted
-// lookups of a 4 M x 128 fp32 table, both gradients, accumulated 219 us, 0.34: sort 60, sums 140, bound by the latency of rows
+// 119 us, 0.34: sort 38, sums beside zeros 66, joins 14; 262 k of a 1 M x 256 fp16 table, max 145 us, 0.56; 1.3 M weighted
+// lookups of a 4 M x 128 fp32 table, both gradients, accumulated 205 us, 0.37: sort 48, sums 136, bound by the latency of rows
 // from DRAM and by issue slots in like parts.
 //
 // The rows of a dense gradient that no lookup names are filled with zeros by other CTAs of the same launch, which
@@ -811,9 +811,10 @@ __global__ void __launch_bounds__(256) zero_kernel(const BackArgs a) {     // no
 // among those that add.  ACC: what grad_table holds is added.
 // A table row that is wanted is read with the loads of the row's first lookup, so that no load is waited for alone.
 // SAME: the table and grad_table have grad_out's type; branches on their types in every unrolled step would not fit the
-// instruction cache (4 M x 128 fp32, weighted and accumulated: 219 us a call against 232).
+// instruction cache (4 M x 128 fp32, weighted and accumulated: 219 us a call against 232).  kWeights is held to
+// 64 registers, four CTAs an SM: 205 us against 210.
 template <typename TG, int VE, int KIND, bool ACC, bool SAME>
-__global__ void __launch_bounds__(256) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
+__global__ void __launch_bounds__(256, KIND == kWeights ? 4 : 0) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
   pdl_enter();
   int cta = blockIdx.x;
   if (!ACC && a.zero_blocks > 0) {
