@@ -190,7 +190,7 @@ def build_training_ops(force: bool = False, verbose: bool = False) -> str | None
                f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", sysconfig.get_paths()["include"], "-I", tinc,
                "-I", os.path.join(tinc, "torch", "csrc", "api", "include"), "-I", "/usr/local/cuda/include",
                "-I", INCLUDE, "-o", target, src, "-L", tlib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
-               "-lc10_cuda", "-Wl,-rpath," + tlib]
+               "-lc10_cuda", "-L", "/usr/local/cuda/lib64", "-lcudart", "-Wl,-rpath," + tlib]
         _run(cmd, verbose)
     return target
 

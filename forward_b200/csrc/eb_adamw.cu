@@ -1,6 +1,6 @@
 // AdamW over many tensors at once (include/fwd_eb_train.h).
 //
-// One launch covers up to 256 tensors: their pointers travel as kernel parameters (80 bytes each),
+// One launch covers up to 256 tensors: their pointers travel as kernel parameters (88 bytes each),
 // so nothing is staged in device memory and the host array may go when the call returns.  A
 // CTA takes one chunk of a tensor, which it finds by bisection of the chunk counts.  A
 // lane handles 8 consecutive elements, so a warp's 256 are exactly one block of an 8-bit

@@ -22,7 +22,6 @@
 // find the named ones in the sorted pairs: every row is written once, and the sums, bound by
 // instructions and the L2, run beside the zeros, bound by DRAM.
 #include <climits>
-#include <cstddef>
 
 #include "eb_train.cuh"
 

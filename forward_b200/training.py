@@ -142,7 +142,7 @@ def _device_of(names, tensors) -> int:
 
 def _on(device: int, run, *args):
     """run(stream, *args) with the device current."""
-    stream = (_loaded_ops or _ops()).current_stream(device)
+    stream = (_loaded_ops or _ops()).current_stream(device, False)
     if device == torch.cuda.current_device():
         return run(stream, *args)
     with torch.cuda.device(device):
@@ -284,9 +284,6 @@ class AdamW:
             self._check(p, f"params[{i}]", p.numel())
             _dtype(p, f"params[{i}]")
         sizes = [p.numel() for p in self.params]
-        addresses = [p.data_ptr() for p in self.params if p.numel()]
-        if len(set(addresses)) < len(addresses):
-            raise ValueError("a parameter is in the list twice")
         self.masters = [None] * n if masters is None else list(masters)
         if len(self.masters) != n:
             raise ValueError("masters: one tensor (or None) per parameter")
@@ -301,6 +298,11 @@ class AdamW:
         if state_bits == 8:
             self.exp_avg_scale = states(exp_avg_scale, "exp_avg_scale", torch.float32, blocks)
             self.exp_avg_sq_scale = states(exp_avg_sq_scale, "exp_avg_sq_scale", torch.float32, blocks)
+        written = self.params + [t for t in self.masters if t is not None] + self.exp_avg + self.exp_avg_sq
+        written += (self.exp_avg_scale or []) + (self.exp_avg_sq_scale or [])
+        addresses = [t.data_ptr() for t in written if t.numel()]
+        if len(set(addresses)) < len(addresses):
+            raise ValueError("a parameter, master copy or state is there twice")
         self._table = (AdamWTensor * n)()
         for i, p in enumerate(self.params):
             t = self._table[i]
@@ -317,10 +319,11 @@ class AdamW:
             self.step_tensor = torch.full((1,), self.step_count, dtype=torch.int64, device=self.device)
             self.lr_tensor = torch.full((1,), lr, dtype=torch.float32, device=self.device)
             self._config.d_step, self._config.d_lr = self.step_tensor.data_ptr(), self.lr_tensor.data_ptr()
-            self._config.step = 1
         self._config_ref = C.byref(self._config)
         self._grads = None
         self._lib = _lib()
+        self._config.step = 1
+        capi.check(self._lib.fwd_eb_adamw_step(None, 0, self._config_ref, None))   # refuses what is out of range
 
     def _check(self, t, name, numel):
         if not t.is_cuda or t.device != self.device:
@@ -344,7 +347,8 @@ class AdamW:
     def step(self, grads=None, *, lr=None, grad_scale=1.0, skip=None) -> None:
         """One step with `grads` (bound first) or the bound gradients.  lr, where given, holds from this step
         on.  grad_scale: a number, or an fp32 device tensor of one element.  skip: an int32
-        device tensor of one element; where it is not 0 the step changes nothing (it still counts)."""
+        device tensor of one element; where it is not 0 the step changes nothing (it still counts).
+        A capture into a graph wants capturable=True: the numbers of any other step are the graph's for good."""
         if grads is not None:
             self.bind(grads)
         if self._grads is None:
@@ -355,16 +359,28 @@ class AdamW:
                 self._check(t, name, 1)
                 if t.dtype != dtype:
                     raise TypeError(f"{name} must be {dtype}")
+        if skip is not None and not isinstance(skip, torch.Tensor):
+            raise TypeError("skip must be an int32 device tensor")
         if isinstance(grad_scale, torch.Tensor):
             cfg.d_grad_scale = grad_scale.data_ptr()
         else:
             cfg.d_grad_scale, cfg.grad_scale = None, grad_scale
         cfg.d_skip = None if skip is None else skip.data_ptr()
+        before = cfg.lr
         if self.step_tensor is None:
             if lr is not None:
                 cfg.lr = lr
             cfg.step = self.step_count + 1
-        _on(self._ordinal, self._launch, lr)
+        try:
+            stream = (_loaded_ops or _ops()).current_stream(self._ordinal, self.step_tensor is None)
+            if self._ordinal == torch.cuda.current_device():
+                self._launch(stream, lr)
+            else:
+                with torch.cuda.device(self._ordinal):
+                    self._launch(stream, lr)
+        except Exception:
+            cfg.lr = before
+            raise
         self.step_count += 1
 
     def _launch(self, stream, lr):

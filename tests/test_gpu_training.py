@@ -853,7 +853,7 @@ def test_the_first_call_may_be_captured():
         "x = torch.randn(600, 2000, device='cuda'); w = torch.ones(2000, device='cuda'); s = torch.ones(600, device='cuda')\n"
         "t = torch.randn(5000, 64, device='cuda'); i = torch.zeros(9000, dtype=torch.int32, device='cuda')\n"
         "o = torch.arange(0, 9000, 9, dtype=torch.int32, device='cuda'); go = torch.randn(1000, 64, device='cuda')\n"
-        "opt = T.AdamW([t], state_bits=8); opt.bind([torch.ones_like(t)])\n"
+        "opt = T.AdamW([t], state_bits=8, capturable=True); opt.bind([torch.ones_like(t)])\n"
         "torch.cuda.synchronize(); g = torch.cuda.CUDAGraph()\n"
         "with torch.cuda.graph(g):\n"
         "    y = T.layer_norm(x, w); r = T.layer_norm_backward(x, x, s, s, w)\n"
@@ -868,6 +868,10 @@ def test_the_first_call_may_be_captured():
 def test_adamw_refusals():
     p = torch.zeros(10, device=DEV)
     pytest.raises(ValueError, T.AdamW, [p, p])
+    m = torch.zeros(10, device=DEV)
+    pytest.raises(ValueError, T.AdamW, [p], exp_avg=[m], exp_avg_sq=[m])
+    for kw in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=float("nan"))):
+        pytest.raises(capi.FwdEbError, T.AdamW, [p], **kw)
     bad = lambda exc, *a, **k: pytest.raises(exc, T.AdamW, *a, **k)  # noqa: E731
     bad(TypeError, [p.double()])
     bad(ValueError, [torch.zeros(4, 4, device=DEV).t()[1:]])
@@ -884,8 +888,16 @@ def test_adamw_refusals():
     pytest.raises(ValueError, opt.step, [p[:9]])
     pytest.raises(ValueError, opt.step, [p.cpu()])
     pytest.raises(TypeError, opt.step, [p.double()])
-    pytest.raises(capi.FwdEbError, opt.step, [p], lr=-1.0)
+    g = torch.ones(10, device=DEV)
+    pytest.raises(capi.FwdEbError, opt.step, [g], lr=-1.0)
+    assert opt.step_count == 0
+    opt.step()                                               # the refused lr is not kept
+    assert (p < 0).all() and opt.step_count == 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pytest.raises(RuntimeError, opt.step)
     pytest.raises(TypeError, opt.step, [p], lr=0.1, skip=torch.zeros(1, device=DEV))
+    pytest.raises(TypeError, opt.step, [p], lr=0.1, skip=1)
 
 
 # ---- together -----------------------------------------------------------------------------------
