@@ -88,6 +88,8 @@ struct BackArgs {
   int word;                     // bytes of a store: 16, 4 or 2
 };
 
+// Loads through the read-only path are for the lookups themselves: what an earlier kernel of the chain has written, this
+// one's CTAs may be resident before it is there, and plain loads are made.
 __device__ __forceinline__ long long index_at(const void* p, int idx64, long long i) {
   return idx64 ? __ldg(static_cast<const long long*>(p) + i) : (long long)__ldg(static_cast<const int*>(p) + i);
 }
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const Back
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int j = base + i * kSortThreads + threadIdx.x;
-      key[i] = j < end ? __ldg(&from[j].x) : 0;
+      key[i] = j < end ? from[j].x : 0;
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_digit_kernel(const BackArgs
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int j = base + (warp * ITEMS + i) * 32 + lane;
-      pair[i] = j < end ? __ldg(from + j) : make_uint2(0, 0);
+      pair[i] = j < end ? from[j] : make_uint2(0, 0);
     }
   };
   fetch(begin);
@@ -709,7 +711,7 @@ __device__ __forceinline__ int2 find_rows(const uint2* pairs, int n, unsigned ro
     const int step0 = (len0 + 31) / 32, step1 = (len1 + 31) / 32;
     const long long at0 = lo0 + (lane + 1LL) * step0 - 1, at1 = lo1 + (lane + 1LL) * step1 - 1;
     const bool in0 = step0 > 0 && at0 < lo0 + len0, in1 = step1 > 0 && at1 < lo1 + len1;
-    const unsigned v0 = in0 ? __ldg(&pairs[at0].x) : kNone, v1 = in1 ? __ldg(&pairs[at1].x) : kNone;
+    const unsigned v0 = in0 ? pairs[at0].x : kNone, v1 = in1 ? pairs[at1].x : kNone;
     const int c0 = __popc(__ballot_sync(kAll, in0 && v0 < row0)), c1 = __popc(__ballot_sync(kAll, in1 && v1 < row1));
     const int next0 = lo0 + c0 * step0, next1 = lo1 + c1 * step1;
     len0 = step0 > 0 ? min(step0 - 1, lo0 + len0 - next0) : 0;
@@ -776,8 +778,8 @@ __device__ __forceinline__ void zero_block(const BackArgs& a, const uint2* pairs
     unsigned row = kNone;
     bool mixed = false;
     if (from < to) {
-      row = __ldg(&pairs[from].x);
-      mixed = __ldg(&pairs[to - 1].x) != row;
+      row = pairs[from].x;
+      mixed = pairs[to - 1].x != row;
       if (!mixed) mark(row);
     }
     for (unsigned left = __ballot_sync(0xffffffffu, mixed); left != 0;) {
@@ -790,7 +792,7 @@ __device__ __forceinline__ void zero_block(const BackArgs& a, const uint2* pairs
         const int i = base + (__ffs(left) - 1) * 32 + lane;
         left &= left - 1;
         in[u] = i < span.y;
-        if (in[u]) rows4[u] = __ldg(&pairs[i].x);
+        if (in[u]) rows4[u] = pairs[i].x;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -912,10 +914,10 @@ __global__ void __launch_bounds__(256, KIND == kWeights ? 4 : 0) segment_sum_ker
       const int b = __shfl_sync(kAll, bag, e0 + u);
       const bool in = e0 + u < valid && col_ok;
       g[u].zero();
-      if (in) g[u].load_ro(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
+      if (in) g[u].load(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
       if constexpr (KIND == kMax) {
         won[u].zero();
-        if (in) won[u].load_ro(a.won + (long long)b * a.pstride + col);
+        if (in) won[u].load(a.won + (long long)b * a.pstride + col);
       }
       if constexpr (kTable) {
         const unsigned r = __shfl_sync(kAll, pair.x, e0 + u);
@@ -1003,7 +1005,7 @@ __global__ void __launch_bounds__(256, KIND == kWeights ? 4 : 0) segment_sum_ker
   put(valid - 1, __shfl_sync(kAll, pair.x, valid - 1) == next);
 }
 
-__device__ __forceinline__ unsigned first_row(const uint2* pairs, int run) { return __ldg(&pairs[run * kRun].x); }
+__device__ __forceinline__ unsigned first_row(const uint2* pairs, int run) { return pairs[run * kRun].x; }
 
 // super[s] = sum of the 32 runs of block s, where one row's lookups fill all the block's run starts.  A CTA a block.
 template <int VE>
@@ -1012,7 +1014,7 @@ __global__ void __launch_bounds__(256) segment_block_kernel(const BackArgs a, co
   __shared__ float part[8][32 * VE];
   const int run0 = blockIdx.x * kRun;
   if (run0 + kRun > a.runs || blockIdx.x == 0) return;
-  const unsigned row = first_row(pairs, run0), before = __ldg(&pairs[run0 * kRun - 1].x), last = first_row(pairs, run0 + kRun - 1);
+  const unsigned row = first_row(pairs, run0), before = pairs[run0 * kRun - 1].x, last = first_row(pairs, run0 + kRun - 1);
   if (row >= a.num_rows || before != row || last != row) return;       // the same for the CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int col = (blockIdx.y * 32 + lane) * VE;
@@ -1069,8 +1071,8 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
   bool crosses = false, two = false;
   if (lane < kJoinRuns && run0 + lane + 1 < a.runs) {
     const int run = run0 + lane;
-    row = __ldg(&pairs[run * kRun + kRun - 1].x);
-    const unsigned before = run > 0 ? __ldg(&pairs[run * kRun - 1].x) : kNone;
+    row = pairs[run * kRun + kRun - 1].x;
+    const unsigned before = run > 0 ? pairs[run * kRun - 1].x : kNone;
     const unsigned next = first_row(pairs, run + 1);
     const unsigned next2 = run + 2 < a.runs ? first_row(pairs, run + 2) : kNone;
     crosses = row < a.num_rows && before != row && next == row;
@@ -1197,7 +1199,7 @@ __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, con
 #pragma unroll
         for (int w = 0; w < 8; ++w) sum[i] += part[w][lane * VE + i];
       }
-      store_row<VE>(a, __ldg(&pairs[from * kRun + kRun - 1].x), col, sum);
+      store_row<VE>(a, pairs[from * kRun + kRun - 1].x, col, sum);
     }
     __syncthreads();
   }
@@ -1322,7 +1324,7 @@ __global__ void __launch_bounds__(kSortThreads) tiny_kernel(const BackArgs a, in
           const int b = __shfl_sync(kAll, bag, e0 + u);
           g[u].zero();
           if (e0 + u < most && col < a.dim)
-            g[u].load_ro(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
+            g[u].load(reinterpret_cast<const TG*>(a.grad_out + (long long)b * a.go_stride) + col);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -1386,7 +1388,7 @@ __global__ void __launch_bounds__(kSortThreads) tiny_kernel(const BackArgs a, in
         for (int col = lane * VE; col < a.dim; col += 32 * VE) {
           Pack<TG, VE> r;
           float fg[VE], fx[VE];
-          r.load_ro(reinterpret_cast<const TG*>(g) + col);
+          r.load(reinterpret_cast<const TG*>(g) + col);
           r.get(fg);
           load_either<VE>(a.table + (long long)p.x * a.table_stride, a.table_f16, col, fx);
 #pragma unroll
@@ -1430,8 +1432,8 @@ __global__ void __launch_bounds__(256) weight_gradient_kernel(const BackArgs a) 
         Pack<TG, VE> pg;
         Pack<TT, VE> px;
         float fg[VE], fx[VE];
-        pg.load_ro(g + col);
-        px.load_ro(x + col);
+        pg.load(g + col);
+        px.load(x + col);
         pg.get(fg);
         px.get(fx);
 #pragma unroll

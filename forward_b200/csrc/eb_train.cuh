@@ -134,10 +134,6 @@ struct Pack {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = static_cast<const W*>(p)[i];
   }
-  __device__ __forceinline__ void load_ro(const void* p) {   // nothing writes it while the kernel runs
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = __ldg(static_cast<const W*>(p) + i);
-  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = W{};

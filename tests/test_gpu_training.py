@@ -996,3 +996,41 @@ def test_adamw_mixed_kinds_in_one_step():
     got = [t for o in solo for t in o.params]
     assert all(same_bits(a, b) for a, b in zip(opt.params, got))
     assert all(same_bits(a, b) for a, b in zip(opt.exp_avg_sq, [t for o in solo for t in o.exp_avg_sq]))
+
+
+def test_calls_on_two_streams_at_once():
+    """Every operator on two streams in turn, nothing waited for in between: the results of one after the other."""
+    def work(seed):
+        s, go, bag, starts = make_bags(seed, 3000, 64, [30] * 800, mode=capi.MODE_MEAN, dtype=torch.float16, pad=True, hot=0.2)
+        small, go2, _, _ = make_bags(seed, 300, 64, [30] * 8, mode=capi.MODE_SUM, dtype=torch.float16)
+        x = rows_of(3000, 1000, torch.bfloat16, seed)
+        p, g = torch.randn(100_000, generator=gen(seed), device=DEV), torch.randn(100_000, generator=gen(seed + 1), device=DEV)
+        opt = T.AdamW([p], state_bits=8, **HYPER)
+
+        def once():
+            a = T.embedding_bag_backward(go, s["table"], s["indices"], s["offsets"], mode=s["mode"], padding_idx=s["padding_idx"])[0]
+            b = T.embedding_bag_backward(go2, small["table"], small["indices"], small["offsets"])[0]
+            y, mean, rstd = T.layer_norm(x, return_stats=True)
+            c = T.layer_norm_backward(y, x, mean, rstd)
+            opt.step([g])
+            return [a, b, y, *c, p.clone()]
+        return once
+
+    want = [work(seed)() for seed in (1, 2)]
+    calls = [work(1), work(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for k in (0, 1):
+        with torch.cuda.stream(streams[k]):
+            got[k] = calls[k]()
+    again = [[], []]
+    for turn in range(6):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                again[k].append(calls[k]())
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(same_bits(a, b) for a, b in zip(got[k], want[k]))
+        for r in again[k]:                                   # the parameter moves on, the rest stays
+            assert all(same_bits(a, b) for a, b in zip(r[:-1], want[k][:-1]))
