@@ -49,8 +49,8 @@ enum {
  *   GATHER      every index is a bag of its own
  *
  * Lookups of padding_idx, outside the row window or before the first bag contribute nothing,
- * and their grad_weights entry is 0.  A row's lookups are added in fp32, in lookup order
- * within runs of 32 and the runs in order, and rounded once to grad_table_dtype.
+ * and their grad_weights entry is 0.  A row's lookups are added in fp32, in an order that the
+ * call's sizes and indices alone determine, and rounded once to grad_table_dtype.
  *
  * grad_table covers the same row window as fwd.table: [num_rows, dim].  Without
  * FWD_EB_BACKWARD_ACCUMULATE every element of those rows is written (zeros where no lookup
