@@ -110,7 +110,9 @@ __device__ __forceinline__ void bag_range(const BackArgs& a, int bag, long long&
     start = index_at(a.offsets, a.idx64, bag);
     end = (a.include_last || bag + 1 < a.num_bags) ? index_at(a.offsets, a.idx64, bag + 1) : a.n;
   }
+  // what malformed offsets name stays within the lookups: both ends index shared memory in the tiny kernel
   if (start < 0) start = 0;
+  if (start > a.n) start = a.n;
   if (end > a.n) end = a.n;
   if (end < start) end = start;
 }
