@@ -52,7 +52,7 @@ struct AdamScalars {
   float step_size;     // lr / (1 - beta1^t)
   float root_scale;    // 1 / sqrt(1 - beta2^t)
   float log1, log2;    // log(beta), for a step that lies on the device
-  int eps_normal;      // eps is far enough from zero that a subnormal v may count as zero
+  int flush;           // a subnormal v may count as zero (see hides_subnormal)
   long long step;
   const float* d_lr;
   const float* d_grad_scale;
@@ -140,8 +140,7 @@ __device__ __forceinline__ void decode(uint2 r, float (&f)[kLane]) {
 
 // Root and reciprocal within an ulp or two, in one or a few instructions where the correctly rounded ones
 // take ten: the update is lr times smaller than the parameter it is added to, and a code or
-// scale of an 8-bit state is far coarser.  FTZ: a subnormal v counts as zero.  Without it the
-// reciprocal's argument is zero only where sqrt(v) + eps is.
+// scale of an 8-bit state is far coarser.  FTZ: a subnormal v counts as zero, where eps hides that.
 template <bool FTZ>
 __device__ __forceinline__ float quick_root(float x) {
   float y;
@@ -291,7 +290,7 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   const void* from = t.master ? t.master : t.param;      // what the step works on, and its type
   const int ftype = t.master ? FWD_EB_F32 : t.ptype;
 
-  if (BITS8 && left == chunk && t.aligned && a.s.eps_normal && a.turns == kMostTurns) {
+  if (BITS8 && left == chunk && t.aligned && a.s.flush && a.turns == kMostTurns) {
     struct Ahead {       // a turn's loads
       Raw<PWIDE> p;
       Raw<GWIDE> g;
@@ -417,6 +416,12 @@ int check_adamw(const fwd_eb_adamw_tensor* ts, int32_t count, const fwd_eb_adamw
   return 0;
 }
 
+// Whether eps hides what is lost where every v below 2^-126 counts as zero.  A step then loses less than
+// 2^-126 of v, steps 1 to t together less than 2^-126 (1 - beta2^t) / (1 - beta2), so sqrt(v / (1 - beta2^t)) is off by
+// less than 2^-63 / sqrt(1 - beta2).  That is half an ulp of a denominator of at least eps where eps is 2^24 times as
+// large, and 2^25 leaves room for what v loses when it is decoded: 1.6e-11 at beta2 = 0.95, 1.2e-10 at 0.999.
+bool hides_subnormal(double eps, double beta2) { return eps * std::sqrt(1.0 - beta2) >= 0x1p-38; }
+
 AdamScalars scalars_of(const fwd_eb_adamw_config* c) {
   AdamScalars s = {};
   s.beta1 = (float)c->beta1;
@@ -432,7 +437,7 @@ AdamScalars scalars_of(const fwd_eb_adamw_config* c) {
   s.log1 = (float)std::log(c->beta1);
   s.log2 = (float)std::log(c->beta2);
   s.step = c->step;
-  s.eps_normal = c->eps >= 1e-30;
+  s.flush = hides_subnormal(c->eps, c->beta2);
   s.d_lr = c->d_lr;
   s.d_grad_scale = c->d_grad_scale;
   s.d_step = reinterpret_cast<const long long*>(c->d_step);

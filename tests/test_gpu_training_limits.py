@@ -1,0 +1,64 @@
+"""The training operators at the edges of what their calls allow, on the GPU against plain 64-bit forms: values
+next to fp32's smallest, constant rows, chains of calls on one stream, refused and captured steps.
+
+Tolerances are bounds of the arithmetic, as in test_gpu_training.py, whose helpers are used.
+"""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from forward_b200 import training as T  # noqa: E402
+from test_gpu_training import DEV, F64, HYPER, U, from_codes, gen, within  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+LEAST = 2.0 ** -149       # the smallest fp32 value; a result below 2^-126 is off by at most half of it
+
+
+# ---- AdamW: gradients whose squares leave fp32's normal range -------------------------------
+
+
+def faint(n, seed):
+    """Magnitudes of 3e-20 to 3e-18, evenly over the logarithm: 0.05 g^2 lies on both sides of 2^-126."""
+    g = gen(seed)
+    size = 10.0 ** (torch.rand(n, generator=g, device=DEV, dtype=F64) * 2 - 19.5)
+    sign = torch.randint(0, 2, (n,), generator=g, device=DEV) * 2 - 1
+    return (size * sign).float()
+
+
+def check_faint_step(opt, g, step, hyper):
+    """One step of one fp32 tensor, against the update in 64 bits from the states as they are held before it."""
+    lr, (b1, b2), eps, wd = hyper["lr"], hyper["betas"], hyper["eps"], hyper["weight_decay"]
+    p = opt.params[0].to(F64)
+    if opt.state_bits == 8:
+        m, root = from_codes(opt.exp_avg[0], opt.exp_avg_scale[0]), from_codes(opt.exp_avg_sq[0], opt.exp_avg_sq_scale[0])
+        v = root.square()
+    else:
+        m, v = opt.exp_avg[0].to(F64), opt.exp_avg_sq[0].to(F64)
+    opt.step([g])
+    g = g.to(F64)
+    m1, v1 = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    root = v1.sqrt()
+    correct = 1 / math.sqrt(1 - b2 ** step)
+    den = root * correct + eps
+    upd = lr / (1 - b1 ** step) * m1 / den
+    # m: as for any gradient.  v: ten roundings, and at most six products and sums that may fall below 2^-126
+    dm = 8 * U * (b1 * m.abs() + (1 - b1) * g.abs()) + 4 * LEAST
+    dv = 10 * U * v1 + 3 * LEAST
+    # |sqrt(a) - sqrt(b)| <= |a - b| / sqrt(b); 2^-24 more where eps may hide a v below 2^-126
+    dden = dv / root * correct + U * eps
+    bound = upd.abs() * (16 * U + dden / (den - dden)) + lr / (1 - b1 ** step) * dm / (den - dden)
+    within(opt.params[0], p * (1 - lr * wd) - upd, bound + 4 * U * (p.abs() + upd.abs()), "param")
+
+
+@pytest.mark.parametrize("eps", [1e-25, 1e-20, 1e-17, 1e-13, 1.7e-11, 1e-8])
+@pytest.mark.parametrize("n", [5000, 9_000_001])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_first_step_from_faint_gradients(bits, n, eps):
+    """Short chunks and, with 8-bit states, the long ones whose loads are under way together: one formula for both, for
+    an eps below, among and above the roots of the smallest v."""
+    hyper = dict(HYPER, eps=eps)
+    opt = T.AdamW([torch.randn(n, generator=gen(n), device=DEV)], state_bits=bits, **hyper)
+    check_faint_step(opt, faint(n, 1), 1, hyper)
