@@ -218,6 +218,14 @@ __device__ __forceinline__ void square(float (&v)[kLane]) {   // of codes: exact
     v[i] = c2.x, v[i + 1] = c2.y;
   }
 }
+// v from codes of sqrt(v).  Their scale's own square leaves the normal range already where v is 2e5 times 2^-126.
+__device__ __forceinline__ void square_scaled(float (&v)[kLane], float scale) {
+#pragma unroll
+  for (int i = 0; i < kLane; i += 2) {
+    const float2 c = mul2(make_float2(v[i], v[i + 1]), both(scale)), c2 = mul2(c, c);
+    v[i] = c2.x, v[i + 1] = c2.y;
+  }
+}
 
 // 8 elements as they lie in memory: WIDE of 32 bits, else of 16.
 template <bool WIDE>
@@ -311,7 +319,7 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
       now.g.get(t.gtype, g);
       decode(now.m, m);
       decode(now.v, v);
-      const float keep1 = now.ms * r.beta1, keep2 = now.vs * now.vs * r.beta2;
+      const float keep1 = now.ms * r.beta1, keep2 = now.vs * now.vs * r.beta2;   // what vs^2 loses below 2^-126, eps hides too
       square(v);
       update<true>(r, keep1, keep2, p, g, m, v, root);
       float ms, vs;
@@ -342,20 +350,18 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
     load_lane(t.grad, t.gtype, at, n, whole, g);
     load_lane(from, ftype, at, n, whole, p);
     const int block = at / FWD_EB_ADAMW_BLOCK;
-    float keep1 = r.beta1, keep2 = r.beta2;
+    float keep1 = r.beta1;
     if (BITS8) {
       const uint2 cm = load_codes(t.m, at, n, whole), cv = load_codes(t.v, at, n, whole);
       keep1 *= t.m_scale[block];
-      const float vs = t.v_scale[block];
-      keep2 *= vs * vs;
       decode(cm, m);
       decode(cv, v);
-      square(v);
+      square_scaled(v, t.v_scale[block]);
     } else {
       load_lane(t.m, FWD_EB_F32, at, n, whole, m);
       load_lane(t.v, FWD_EB_F32, at, n, whole, v);
     }
-    update<false>(r, keep1, keep2, p, g, m, v, root);
+    update<false>(r, keep1, r.beta2, p, g, m, v, root);
     if (t.master) store_lane(t.master, FWD_EB_F32, at, n, whole, p);
     store_lane(t.param, t.ptype, at, n, whole, p);
     if (BITS8) {

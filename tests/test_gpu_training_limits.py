@@ -62,3 +62,15 @@ def test_adamw_first_step_from_faint_gradients(bits, n, eps):
     hyper = dict(HYPER, eps=eps)
     opt = T.AdamW([torch.randn(n, generator=gen(n), device=DEV)], state_bits=bits, **hyper)
     check_faint_step(opt, faint(n, 1), 1, hyper)
+
+
+@pytest.mark.parametrize("n,eps", [(5000, 1e-20), (5000, 1e-8), (9_000_001, 1e-20), (9_000_001, 1.7e-11)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_steps_from_faint_states(bits, n, eps):
+    """Later steps, from states that faint gradients left: what 8 bits hold is taken at its value, though its
+    scale's square is below 2^-126."""
+    hyper = dict(HYPER, eps=eps)
+    opt = T.AdamW([torch.randn(n, generator=gen(n), device=DEV)], state_bits=bits, **hyper)
+    opt.step([faint(n, 1)])
+    for step in (2, 3):
+        check_faint_step(opt, faint(n, step), step, hyper)
