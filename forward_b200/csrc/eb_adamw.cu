@@ -140,7 +140,8 @@ __device__ __forceinline__ void decode(uint2 r, float (&f)[kLane]) {
 
 // Root and reciprocal within an ulp or two, in one or a few instructions where the correctly rounded ones
 // take ten: the update is lr times smaller than the parameter it is added to, and a code or
-// scale of an 8-bit state is far coarser.  FTZ: a subnormal v counts as zero, where eps hides that.
+// scale of an 8-bit state is far coarser.  FTZ: a subnormal v counts as zero, where eps hides that.  The reciprocal's
+// argument sqrt(v) + eps is zero or normal: an eps above zero is normal, and the root of a subnormal v is.
 template <bool FTZ>
 __device__ __forceinline__ float quick_root(float x) {
   float y;
@@ -389,12 +390,15 @@ bool known(int dtype) { return dtype == FWD_EB_F32 || dtype == FWD_EB_F16 || dty
 int check_adamw(const fwd_eb_adamw_tensor* ts, int32_t count, const fwd_eb_adamw_config* c) {
   if (count < 0 || (count > 0 && !ts)) return fail(FWD_EB_EINVAL, "bad tensor list");
   if (!c) return fail(FWD_EB_EINVAL, "config is null");
-  auto good = [](double x) { return std::isfinite(x) && x >= 0.0; };
+  auto good = [](double x) { return x >= 0.0 && x <= FLT_MAX; };
   if (!c->d_lr && !good(c->lr)) return fail(FWD_EB_EINVAL, "lr must be finite and not negative");
   if (!good(c->eps)) return fail(FWD_EB_EINVAL, "eps must be finite and not negative");
+  // the least denominator, whose reciprocal has to be a normal fp32 value
+  if (c->eps != 0.0 && !(c->eps >= 0x1p-126 && c->eps <= 0x1p126))
+    return fail(FWD_EB_EINVAL, "eps is 0 or between 2^-126 and 2^126 (got %g)", c->eps);
   if (!(c->beta1 >= 0.0 && c->beta1 < 1.0) || !(c->beta2 >= 0.0 && c->beta2 < 1.0))
     return fail(FWD_EB_EINVAL, "beta1 and beta2 lie in [0, 1)");
-  if (!c->d_grad_scale && !std::isfinite(c->grad_scale)) return fail(FWD_EB_EINVAL, "grad_scale must be finite");
+  if (!c->d_grad_scale && !(std::fabs(c->grad_scale) <= FLT_MAX)) return fail(FWD_EB_EINVAL, "grad_scale must be finite");
   if (!c->d_step && c->step < 1) return fail(FWD_EB_EINVAL, "step counts from 1 (got %lld)", (long long)c->step);
   if (!aligned_to(c->d_lr, 4) || !aligned_to(c->d_grad_scale, 4) || !aligned_to(c->d_step, 8) || !aligned_to(c->d_skip, 4))
     return fail(FWD_EB_EALIGN, "a device scalar is not aligned to its type");

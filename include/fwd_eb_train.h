@@ -172,10 +172,10 @@ typedef struct fwd_eb_adamw_tensor {
  * host's is ignored.
  */
 typedef struct fwd_eb_adamw_config {
-  double lr;                  /* >= 0 */
+  double lr;                  /* >= 0, finite in fp32 */
   double beta1, beta2;        /* [0, 1) */
-  double eps;                 /* >= 0 */
-  double grad_scale;
+  double eps;                 /* 0, or 2^-126 .. 2^126 */
+  double grad_scale;          /* finite in fp32 */
   int64_t step;               /* t of this step, from 1 */
   const float* d_lr;
   const float* d_grad_scale;
