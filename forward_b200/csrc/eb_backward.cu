@@ -88,8 +88,9 @@ struct BackArgs {
   int word;                     // bytes of a store: 16, 4 or 2
 };
 
-// Loads through the read-only path are for the lookups themselves: what an earlier kernel of the chain has written, this
-// one's CTAs may be resident before it is there, and plain loads are made.
+// Loads through the read-only path are for the lookups themselves: what an earlier kernel of the chain has written, or the
+// forward call ahead of it (the winners: pooling kernels let their successors in at their start), this one's CTAs may be
+// resident before it is there, and plain loads are made.
 __device__ __forceinline__ long long index_at(const void* p, int idx64, long long i) {
   return idx64 ? __ldg(static_cast<const long long*>(p) + i) : (long long)__ldg(static_cast<const int*>(p) + i);
 }
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(256) winner_bytes_kernel(const BackArgs a) {
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long bag = i / a.dim;
     const int col = (int)(i - bag * a.dim);
-    a.won[bag * a.pstride + col] = (unsigned char)__ldg(&a.winners[bag * a.win_stride + col].y);
+    a.won[bag * a.pstride + col] = (unsigned char)a.winners[bag * a.win_stride + col].y;
   }
 }
 
@@ -948,7 +949,7 @@ __global__ void __launch_bounds__(256, KIND == kWeights ? 4 : 0) segment_sum_ker
           g[u].get(f);
           if (col_ok) {
             for (int i = 0; i < VE; ++i) {
-              if (__ldg(&a.winners[(long long)b * a.win_stride + col + i].y) == (at & INT_MAX)) acc[i] += f[i];
+              if (a.winners[(long long)b * a.win_stride + col + i].y == (at & INT_MAX)) acc[i] += f[i];
             }
           }
         }
@@ -1337,7 +1338,7 @@ __global__ void __launch_bounds__(kSortThreads) tiny_kernel(const BackArgs a, in
           g[u].get(x);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
-            if (kind == kMax) acc[i] += __ldg(&a.winners[(long long)b * a.win_stride + col + i].y) == p ? x[i] : 0.0f;
+            if (kind == kMax) acc[i] += a.winners[(long long)b * a.win_stride + col + i].y == p ? x[i] : 0.0f;
             else acc[i] = fmaf(f, x[i], acc[i]);
           }
         }

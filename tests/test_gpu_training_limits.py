@@ -9,8 +9,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from forward_b200 import training as T  # noqa: E402
-from test_gpu_training import DEV, F64, HYPER, U, from_codes, gen, within  # noqa: E402
+from forward_b200 import capi, training as T  # noqa: E402
+from test_gpu_training import DEV, F64, HYPER, U, from_codes, gen, make_bags, same_bits, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,30 @@ def test_adamw_steps_from_faint_states(bits, n, eps):
     opt.step([faint(n, 1)])
     for step in (2, 3):
         check_faint_step(opt, faint(n, step), step, hyper)
+
+
+# ---- calls one behind the other ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lengths", [[8] * 40, [40] * 2000, [300] * 60])
+def test_max_gradient_right_behind_its_forward_call(lengths):
+    """The winners are read while the launches of the call that wrote them may still be the ones ahead: every batch anew
+    into the same memory, the results of a run that waits after each call."""
+    batches = [make_bags(seed, 900, 64, lengths, mode=capi.MODE_MAX, dtype=torch.float32) for seed in range(6)]
+    pairs = torch.empty(len(lengths), 64, 2, device=DEV)
+
+    def run(wait):
+        got = []
+        for s, go, _, _ in batches * 3:
+            p = capi.make_params(s["table"], s["indices"], s["offsets"], out=pairs, mode=capi.MODE_MAX)
+            p.out_dtype, p.out_stride = capi.F32_POS, 0
+            capi.forward(p)
+            wait()
+            got.append(T.embedding_bag_backward(go, s["table"], s["indices"], s["offsets"], mode=capi.MODE_MAX, winners=pairs)[0])
+            wait()
+        return got
+
+    want = run(torch.cuda.synchronize)
+    got = run(lambda: None)
+    torch.cuda.synchronize()
+    assert all(same_bits(a, b) for a, b in zip(got, want))
