@@ -264,7 +264,7 @@ template <int CAP, int KIND>
 __global__ void __launch_bounds__(kAdamThreads, KIND < 2 ? 4 : 3)   // the others' loads would spill
 adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   constexpr bool BITS8 = KIND != 0, PWIDE = BITS8 && (KIND - 1) / 2 == 1, GWIDE = BITS8 && (KIND - 1) % 2 == 1;
-  pdl_enter();
+  pdl_enter(false);
   if (a.s.d_skip && *a.s.d_skip != 0) return;
   int lo = 0, hi = a.count;   // the last tensor whose first chunk is not behind this one
   while (hi - lo > 1) {

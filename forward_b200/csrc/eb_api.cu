@@ -515,7 +515,9 @@ static cudaError_t launch_pool(const Plan& pl, cudaStream_t st) {
     // Programmatic stream serialization: when the launch ahead of this one on the stream is
     // also a pooling grid, this grid's CTAs take their places while that grid's last CTAs
     // drain (they wait in griddepcontrol.wait before touching memory) — 1.6-2 us per call of
-    // back-to-back pooling.  After any other kind of work it is an ordinary launch.
+    // back-to-back pooling.  After any other kind of work it is an ordinary launch: the kernels that end
+    // a training call do not let their successors in early, so what they wrote (the table, weights) may be
+    // read through the read-only path here.
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)cta);

@@ -150,7 +150,7 @@ __device__ __forceinline__ int2 upper_bound_cta(const BackArgs& a, long long j0,
 
 // counted[b] = length of bag b; the kernel that makes the pairs takes the padding off.
 __global__ void __launch_bounds__(256) bag_length_kernel(const BackArgs a) {
-  pdl_enter();
+  pdl_enter(true);
   const int b = blockIdx.x * 256 + threadIdx.x;
   if (b >= a.num_bags) return;
   long long s, e;
@@ -244,7 +244,7 @@ __device__ __forceinline__ void uncount_padding(const BackArgs& a, long long idx
 
 // Zeros where the sums of 16 tiles will be counted.
 __global__ void __launch_bounds__(kSortThreads) clear_sums_kernel(unsigned* hist16, int words) {
-  pdl_enter();
+  pdl_enter(true);
   const int i = blockIdx.x * kSortThreads + threadIdx.x;
   if (i < words) hist16[i] = 0;
 }
@@ -262,7 +262,7 @@ __device__ __forceinline__ void put_counts(const BackArgs& a, const unsigned* co
 // lookups; all its indices are asked for at once (they may come from DRAM, a microsecond and a half a round).
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs a, uint2* to) {
-  pdl_enter();
+  pdl_enter(true);
   __shared__ unsigned count[kDigits];
   __shared__ int starts[kStarts];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kSortThreads) make_pairs_kernel(const BackArgs
 // The histogram of a later digit.
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_histogram_kernel(const BackArgs a, const uint2* from, int pass) {
-  pdl_enter();
+  pdl_enter(true);
   __shared__ unsigned count[kDigits];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) count[d] = 0;
   __syncthreads();
@@ -402,7 +402,7 @@ struct DigitShared {
 };
 template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_digit_kernel(const BackArgs a, const uint2* from, uint2* to, int pass) {
-  pdl_enter();
+  pdl_enter(true);
   extern __shared__ uint4 dynamic[];
   DigitShared<ITEMS>& s = *reinterpret_cast<DigitShared<ITEMS>*>(dynamic);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -580,7 +580,7 @@ __device__ __forceinline__ void sort_all(const BackArgs& a, SmallSort<ITEMS>& s,
 
 // Up to kSmall lookups: one CTA sorts them.
 __global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs a, uint2* to) {
-  pdl_enter();
+  pdl_enter(true);
   __shared__ SmallSort<kSmallItems> s;
   sort_all<kSmallItems>(a, s, to, a.bag_of != nullptr || a.counted != nullptr);
 }
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_small_kernel(const BackArgs
 // won[b][c] = the low byte of the position that won column c of bag b: what the sum below compares in bags of
 // fewer than 256 lookups, an eighth of the pairs' bytes.
 __global__ void __launch_bounds__(256) winner_bytes_kernel(const BackArgs a) {
-  pdl_enter();
+  pdl_enter(true);
   const long long total = (long long)a.num_bags * a.dim;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long bag = i / a.dim;
@@ -807,7 +807,7 @@ __device__ __forceinline__ void zero_block(const BackArgs& a, const uint2* pairs
   fill_zeros(a, named, first, rows);
 }
 __global__ void __launch_bounds__(256) zero_kernel(const BackArgs a) {     // no lookups at all
-  pdl_enter();
+  pdl_enter(false);
   zero_block(a, nullptr, blockIdx.x);
 }
 
@@ -819,7 +819,7 @@ __global__ void __launch_bounds__(256) zero_kernel(const BackArgs a) {     // no
 // 64 registers, four CTAs an SM: 205 us against 210.
 template <typename TG, int VE, int KIND, bool ACC, bool SAME>
 __global__ void __launch_bounds__(256, KIND == kWeights ? 4 : 0) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
-  pdl_enter();
+  pdl_enter(true);
   int cta = blockIdx.x;
   if (!ACC && a.zero_blocks > 0) {
     const int before = (int)((long long)cta * a.zero_blocks / gridDim.x);        // zero CTAs among the earlier ones
@@ -1013,7 +1013,7 @@ __device__ __forceinline__ unsigned first_row(const uint2* pairs, int run) { ret
 // super[s] = sum of the 32 runs of block s, where one row's lookups fill all the block's run starts.  A CTA a block.
 template <int VE>
 __global__ void __launch_bounds__(256) segment_block_kernel(const BackArgs a, const uint2* pairs) {
-  pdl_enter();
+  pdl_enter(true);
   __shared__ float part[8][32 * VE];
   const int run0 = blockIdx.x * kRun;
   if (run0 + kRun > a.runs || blockIdx.x == 0) return;
@@ -1059,7 +1059,7 @@ constexpr int kFewPieces = 24;
 constexpr int kJoinRuns = 8;       // of a warp
 template <int VE>
 __global__ void __launch_bounds__(256) segment_join_kernel(const BackArgs a, const uint2* pairs) {
-  pdl_enter();
+  pdl_enter(false);
   constexpr unsigned kAll = 0xffffffffu;
   __shared__ int long_from[8 * kJoinRuns], long_to[8 * kJoinRuns];
   __shared__ int longs;
@@ -1226,7 +1226,7 @@ struct TinyShared {
 };
 template <typename TG, int VE, int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) tiny_kernel(const BackArgs a, int kind) {
-  pdl_enter();
+  pdl_enter(false);
   extern __shared__ uint4 dynamic[];
   TinyShared<ITEMS>& s = *reinterpret_cast<TinyShared<ITEMS>*>(dynamic);
   constexpr unsigned kAll = 0xffffffffu;
@@ -1421,7 +1421,7 @@ __global__ void __launch_bounds__(kSortThreads) tiny_kernel(const BackArgs a, in
 // grad_weights[j] = <table[row j], grad_out[bag j]>, a warp per lookup.
 template <typename TG, typename TT, int VE>
 __global__ void __launch_bounds__(256) weight_gradient_kernel(const BackArgs a) {
-  pdl_enter();
+  pdl_enter(a.pairs[0] != nullptr);     // the sums follow where the table's gradient is wanted too
   const int lane = threadIdx.x & 31;
   const long long step = (long long)gridDim.x * 8;
   for (long long j = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); j < a.n; j += step) {
@@ -1645,6 +1645,7 @@ cudaError_t launch_segments(const BackPlan& pl, const uint2* sorted, cudaStream_
     FWD_EB_TRY(launch_pdl(segment_block_kernel<VE>, blocks, 256, 0, st, a, sorted));
   }
   if (a.runs > 1) {
+    // the last kernel of every call that sorts by tiles or in one CTA: those have more than one run
     const dim3 joins((unsigned)((a.runs + 8 * kJoinRuns - 1) / (8 * kJoinRuns)), tiles);
     FWD_EB_TRY(launch_pdl(segment_join_kernel<VE>, joins, 256, 0, st, a, sorted));
   }

@@ -172,7 +172,7 @@ struct Ahead {
 template <typename T, int VEC, int NV, int TPR>
 __global__ void __launch_bounds__(kThreads<TPR>, kForwardThreads / kThreads<TPR> < 1 ? 1 : kForwardThreads / kThreads<TPR>)
 layer_norm_forward_kernel(const NormArgs a) {
-  pdl_enter();
+  pdl_enter(false);
   constexpr int kRows = kThreads<TPR> / TPR;
   __shared__ float red[2][32][1];
   const int lane = threadIdx.x % TPR;
@@ -246,7 +246,7 @@ layer_norm_forward_kernel(const NormArgs a) {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(1024)
 layer_norm_forward_loop_kernel(const NormArgs a) {
-  pdl_enter();
+  pdl_enter(false);
   __shared__ float red[2][32][1];
   const int step = blockDim.x * VEC;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -294,7 +294,7 @@ layer_norm_forward_loop_kernel(const NormArgs a) {
 template <typename T, int VEC, int NV, int TPR>
 __global__ void __launch_bounds__(kThreads<TPR>, kBackwardThreads / kThreads<TPR> < 1 ? 1 : kBackwardThreads / kThreads<TPR>)
 layer_norm_backward_kernel(const NormArgs a) {
-  pdl_enter();
+  pdl_enter(a.partial != nullptr);
   constexpr int kRows = kThreads<TPR> / TPR;
   __shared__ float red[2][32][2];
   // the rows under way; at the end, with more than one row a CTA, [8 warps][2][cols] sums
@@ -447,7 +447,7 @@ layer_norm_backward_kernel(const NormArgs a) {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(1024)
 layer_norm_backward_loop_kernel(const NormArgs a) {
-  pdl_enter();
+  pdl_enter(a.partial != nullptr);
   __shared__ float red[2][32][1];
   const int step = blockDim.x * VEC;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -496,7 +496,7 @@ layer_norm_backward_loop_kernel(const NormArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 layer_norm_columns_kernel(const NormArgs a) {
-  pdl_enter();
+  pdl_enter(true);
   const long long col = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (col >= a.cols) return;
   float dw = 0.0f, db = 0.0f;
@@ -515,7 +515,7 @@ layer_norm_columns_kernel(const NormArgs a) {
 // take every 32nd part each, and their sums are added in order.
 __global__ void __launch_bounds__(1024)
 layer_norm_join_kernel(const float* partial, int parts, int cols, int wtype, void* gw, void* gb) {
-  pdl_enter();
+  pdl_enter(false);
   __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long col = (long long)blockIdx.x * 32 + lane;   // over both halves

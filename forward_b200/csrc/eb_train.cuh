@@ -15,11 +15,14 @@
 
 namespace fwd_eb {
 
-// Programmatic stream serialisation: the next grid of the stream may start its blocks as soon as
-// all of this one's are resident, and waits here until this one has finished.  Every kernel below
-// waits before its first access to memory, on every path.
-__device__ __forceinline__ void pdl_enter() {
-  asm volatile("griddepcontrol.launch_dependents;");
+// Programmatic stream serialisation: where a kernel releases its dependents at its start, the next grid of the stream may
+// start its blocks as soon as all of this one's are resident, and waits until this one has finished.  Every
+// kernel of these operators waits before its first access to memory, on every path.  It releases its successor
+// early only where that is the next kernel of the same call (`more`): what comes behind a call may read the call's
+// results through the read-only path, as the pooling kernels do with a table that AdamW has just written, and data on
+// that path may not change while the reader is resident.
+__device__ __forceinline__ void pdl_enter(bool more) {
+  if (more) asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 

@@ -101,3 +101,42 @@ def test_max_gradient_right_behind_its_forward_call(lengths):
     got = run(lambda: None)
     torch.cuda.synchronize()
     assert all(same_bits(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bags,rows", [(16, 200), (3000, 20_000)])
+def test_steps_and_lookups_right_behind_one_another(bags, rows, bits):
+    """The table that a step writes is pooled by the next call on the stream, its gradient taken, and so on, per-sample
+    weights among the parameters: the bits of a loop that waits after each call."""
+    batches = [make_bags(seed, rows, 64, [9] * bags, mode=capi.MODE_SUM, dtype=torch.float32) for seed in range(4)]
+
+    def run(wait):
+        table, w = torch.randn(rows, 64, generator=gen(1), device=DEV), torch.rand(9 * bags, generator=gen(2), device=DEV)
+        grad, gw = torch.empty_like(table), torch.empty_like(w)
+        opt = T.AdamW([table, w], state_bits=bits, **HYPER)
+        opt.bind([grad, gw])
+        kept = []
+        for s, go, _, _ in batches * 4:
+            pooled = capi.embedding_bag(table, s["indices"], s["offsets"], per_sample_weights=w)
+            wait()
+            y, mean, rstd = T.layer_norm(pooled, return_stats=True)
+            wait()
+            rows_again = capi.embedding_bag(y, s["indices"][:8] % bags, mode=capi.MODE_GATHER)     # the norm's rows as a table
+            wait()
+            gx, _, _ = T.layer_norm_backward(go, pooled, mean, rstd)
+            wait()
+            _, dw = T.embedding_bag_backward(gx, table, s["indices"], s["offsets"], per_sample_weights=w, grad_table=grad,
+                                             need_weights=True)
+            wait()
+            again = capi.embedding_bag(grad, s["indices"], s["offsets"], per_sample_weights=dw)      # gradients as inputs
+            wait()
+            gw.copy_(dw)
+            opt.step()
+            wait()
+            kept += [pooled, rows_again, again]
+        return kept + [table, w]
+
+    want = run(torch.cuda.synchronize)
+    got = run(lambda: None)
+    torch.cuda.synchronize()
+    assert all(same_bits(a, b) for a, b in zip(got, want))
