@@ -320,6 +320,7 @@ class AdamW:
             self.lr_tensor = torch.full((1,), lr, dtype=torch.float32, device=self.device)
             self._config.d_step, self._config.d_lr = self.step_tensor.data_ptr(), self.lr_tensor.data_ptr()
         self._config_ref = C.byref(self._config)
+        self._host = AdamWConfig(lr, betas[0], betas[1], eps, 1.0, 1, None, None, None, None)   # see step
         self._grads = None
         self._lib = _lib()
         self._config.step = 1
@@ -366,6 +367,14 @@ class AdamW:
         else:
             cfg.d_grad_scale, cfg.grad_scale = None, grad_scale
         cfg.d_skip = None if skip is None else skip.data_ptr()
+        if self.step_tensor is not None:      # what the call would refuse is refused before the device's numbers move
+            self._host.grad_scale = 1.0 if cfg.d_grad_scale else grad_scale
+            if lr is not None and not isinstance(lr, torch.Tensor):
+                self._host.lr = lr
+            try:
+                capi.check(self._lib.fwd_eb_adamw_step(None, 0, C.byref(self._host), None))
+            finally:
+                self._host.lr = cfg.lr
         before = cfg.lr
         if self.step_tensor is None:
             if lr is not None:

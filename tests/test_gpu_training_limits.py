@@ -140,3 +140,30 @@ def test_steps_and_lookups_right_behind_one_another(bags, rows, bits):
     got = run(lambda: None)
     torch.cuda.synchronize()
     assert all(same_bits(a, b) for a, b in zip(got, want))
+
+
+# ---- refused and captured steps --------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kw", [dict(grad_scale=float("inf")), dict(grad_scale=1e39), dict(lr=-1.0), dict(lr=float("nan")),
+                                dict(lr=0.5, grad_scale=float("nan"))])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_leaves_the_optimizer_as_it_was(capturable, kw):
+    p, g = torch.ones(300, device=DEV), torch.ones(300, device=DEV)
+    opt = T.AdamW([p], lr=0.25, capturable=capturable)
+    opt.step([g])
+    before = [t.clone() for t in (p, *opt.exp_avg, *opt.exp_avg_sq)]
+    for _ in range(2):
+        with pytest.raises(capi.FwdEbError):
+            opt.step([g], **kw)
+    assert all(same_bits(a, b) for a, b in zip(before, (p, *opt.exp_avg, *opt.exp_avg_sq)))
+    assert opt.step_count == 1
+    if capturable:
+        assert int(opt.step_tensor) == 1 and float(opt.lr_tensor) == 0.25
+    opt.step([g], lr=0.125)                                  # from the lr and the count of before
+    other = torch.ones(300, device=DEV)
+    plain = T.AdamW([other], lr=0.25, capturable=capturable)
+    plain.step([g])
+    plain.step([g], lr=0.125)
+    assert same_bits(p, other)
+    assert not capturable or (int(opt.step_tensor) == 2 and float(opt.lr_tensor) == 0.125)
