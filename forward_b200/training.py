@@ -322,6 +322,7 @@ class AdamW:
         self._config_ref = C.byref(self._config)
         self._host = AdamWConfig(lr, betas[0], betas[1], eps, 1.0, 1, None, None, None, None)   # see step
         self._grads = None
+        self._captured = []         # what captured steps read beside gradients and states
         self._lib = _lib()
         self._config.step = 1
         capi.check(self._lib.fwd_eb_adamw_step(None, 0, self._config_ref, None))   # refuses what is out of range
@@ -349,7 +350,9 @@ class AdamW:
         """One step with `grads` (bound first) or the bound gradients.  lr, where given, holds from this step
         on.  grad_scale: a number, or an fp32 device tensor of one element.  skip: an int32
         device tensor of one element; where it is not 0 the step changes nothing (it still counts).
-        A capture into a graph wants capturable=True: the numbers of any other step are the graph's for good."""
+        A capture into a graph wants capturable=True: the numbers of any other step are the graph's for good.  The
+        graph reads the tensors of the captured call: the optimizer keeps grad_scale and skip alive as long as it lives
+        itself; it and the gradients have to outlive the graph."""
         if grads is not None:
             self.bind(grads)
         if self._grads is None:
@@ -367,6 +370,7 @@ class AdamW:
         else:
             cfg.d_grad_scale, cfg.grad_scale = None, grad_scale
         cfg.d_skip = None if skip is None else skip.data_ptr()
+        scalars = [t for t in (grad_scale, skip) if isinstance(t, torch.Tensor)]
         if self.step_tensor is not None:      # what the call would refuse is refused before the device's numbers move
             self._host.grad_scale = 1.0 if cfg.d_grad_scale else grad_scale
             if lr is not None and not isinstance(lr, torch.Tensor):
@@ -383,17 +387,19 @@ class AdamW:
         try:
             stream = (_loaded_ops or _ops()).current_stream(self._ordinal, self.step_tensor is None)
             if self._ordinal == torch.cuda.current_device():
-                self._launch(stream, lr)
+                self._launch(stream, lr, scalars)
             else:
                 with torch.cuda.device(self._ordinal):
-                    self._launch(stream, lr)
+                    self._launch(stream, lr, scalars)
         except Exception:
             cfg.lr = before
             raise
         self.step_count += 1
 
-    def _launch(self, stream, lr):
+    def _launch(self, stream, lr, scalars):
         if self.step_tensor is not None:
+            if scalars and torch.cuda.is_current_stream_capturing():
+                self._captured += scalars
             if lr is not None:
                 self.lr_tensor.fill_(lr)
             self.step_tensor.add_(1)

@@ -3,7 +3,9 @@ next to fp32's smallest, constant rows, chains of calls on one stream, refused a
 
 Tolerances are bounds of the arithmetic, as in test_gpu_training.py, whose helpers are used.
 """
+import gc
 import math
+import weakref
 
 import pytest
 
@@ -167,3 +169,27 @@ def test_a_refused_step_leaves_the_optimizer_as_it_was(capturable, kw):
     plain.step([g], lr=0.125)
     assert same_bits(p, other)
     assert not capturable or (int(opt.step_tensor) == 2 and float(opt.lr_tensor) == 0.125)
+
+
+def test_a_captured_step_keeps_its_scale_and_skip_flag():
+    """Made for the call and dropped by the caller: their memory stays theirs, and each replay reads what they held."""
+    p, g = torch.zeros(300, device=DEV), torch.ones(300, device=DEV)
+    opt = T.AdamW([p], lr=0.25, betas=(0.0, 0.0), eps=1.0, weight_decay=0.0, capturable=True)
+    opt.bind([g])
+    scale, skip = torch.full((1,), 3.0, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    held = [weakref.ref(scale), weakref.ref(skip)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(grad_scale=scale, skip=skip)
+    del scale, skip
+    gc.collect()
+    assert all(r() is not None for r in held)
+    filler = [torch.full((1,), -7, dtype=torch.int32, device=DEV) for _ in range(200)]     # what freed memory would turn into
+    graph.replay()
+    # m = 3, v = 9: a step of lr * 3 / (3 + 1)
+    assert torch.equal(p, torch.full_like(p, -0.25 * 3 / 4)) and len(filler) == 200
+    eager = torch.full((1,), 3.0, device=DEV)
+    opt.step(grad_scale=eager)
+    held = weakref.ref(eager)
+    del eager
+    assert held() is None                                    # nobody replays an eager step
