@@ -109,6 +109,11 @@ void stats_of(const at::Tensor& t, const char* name, int64_t rows) {
 }
 void* pointer(Maybe t) { return t ? t->data_ptr() : nullptr; }
 
+// A given tensor was written: what autograd saved of it before counts as changed, as after torch's own in-place calls.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject* wrapped(const std::optional<at::Tensor>& t) {
   if (!t) Py_RETURN_NONE;
   return THPVariable_Wrap(*t);
@@ -167,6 +172,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.y = y.data_ptr();
     const int rc = g_norm_forward(&p, c10::cuda::getCurrentCUDAStream(device).stream());
     if (rc) return PyLong_FromLong(rc);
+    if (out) written(*out);
     PyObject* result = out ? Py_NewRef(a[4]) : THPVariable_Wrap(y);
     if (!stats) return result;
     return Py_BuildValue("(NNN)", result, wrapped(mean), wrapped(rstd));
@@ -232,6 +238,7 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const int rc = g_norm_backward(&p, c10::cuda::getCurrentCUDAStream(device).stream());
     if (rc) return PyLong_FromLong(rc);
+    if (given) written(*given);
     return Py_BuildValue("(NNN)", given ? Py_NewRef(a[5]) : wrapped(gx), wrapped(gw), wrapped(gb));
   } catch (const Refused& r) {
     PyErr_SetString(r.type, r.text.c_str());
@@ -351,6 +358,7 @@ PyObject* embedding_bag_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const int rc = g_backward(&p, c10::cuda::getCurrentCUDAStream(device).stream());
       if (rc) return PyLong_FromLong(rc);
     }
+    if (given) written(*given);
     return Py_BuildValue("(NN)", given ? Py_NewRef(a[12]) : wrapped(gt), wrapped(gw));
   } catch (const Refused& r) {
     PyErr_SetString(r.type, r.text.c_str());
@@ -371,6 +379,21 @@ PyObject* current_stream(PyObject*, PyObject* const* a, Py_ssize_t n) {
         throw Refused{PyExc_RuntimeError, "a step that is captured needs capturable=True"};
     }
     return PyLong_FromVoidPtr(stream);
+  } catch (const Refused& r) {
+    PyErr_SetString(r.type, r.text.c_str());
+    return nullptr;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// touched(list of tensors): each was written
+PyObject* touched(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  try {
+    want(1, n);
+    if (!PyList_Check(a[0])) type_error("touched takes a list");
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); ++i) written(tensor(PyList_GET_ITEM(a[0], i), "a tensor"));
+    Py_RETURN_NONE;
   } catch (const Refused& r) {
     PyErr_SetString(r.type, r.text.c_str());
     return nullptr;
@@ -403,7 +426,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FWD_EB_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {
     FWD_EB_METHOD(layer_norm), FWD_EB_METHOD(layer_norm_backward), FWD_EB_METHOD(embedding_bag_backward),
-    FWD_EB_METHOD(current_stream), FWD_EB_METHOD(bind), {nullptr, nullptr, 0, nullptr},
+    FWD_EB_METHOD(current_stream), FWD_EB_METHOD(touched), FWD_EB_METHOD(bind), {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_training_ops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

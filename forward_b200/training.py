@@ -4,6 +4,9 @@ EmbeddingBag call, layer norm with its gradients, and AdamW over many tensors at
 Like capi, the functions take torch CUDA tensors, launch on the current stream of the tensors'
 device and return without synchronising; outputs and scratch come from torch's allocator.
 Every result is deterministic.  There is no CPU path.
+
+They are the pieces of a hand-written step and stand outside autograd: results carry no graph, whatever
+their inputs require.  Tensors that a call is given to write into (not AdamW's states) count as changed in place.
 """
 from __future__ import annotations
 
@@ -303,6 +306,7 @@ class AdamW:
         addresses = [t.data_ptr() for t in written if t.numel()]
         if len(set(addresses)) < len(addresses):
             raise ValueError("a parameter, master copy or state is there twice")
+        self._valued = self.params + [t for t in self.masters if t is not None]     # what a loss may have been computed from
         self._table = (AdamWTensor * n)()
         for i, p in enumerate(self.params):
             t = self._table[i]
@@ -395,6 +399,7 @@ class AdamW:
             cfg.lr = before
             raise
         self.step_count += 1
+        _loaded_ops.touched(self._valued)
 
     def _launch(self, stream, lr, scalars):
         if self.step_tensor is not None:

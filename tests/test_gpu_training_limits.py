@@ -193,3 +193,61 @@ def test_a_captured_step_keeps_its_scale_and_skip_flag():
     held = weakref.ref(eager)
     del eager
     assert held() is None                                    # nobody replays an eager step
+
+
+# ---- autograd's bookkeeping ------------------------------------------------------------------------
+
+
+def test_tensors_written_in_place_count_as_changed():
+    """Autograd refuses to differentiate through a saved tensor that a call has overwritten; what was only read does not count."""
+    x, w = torch.randn(20, 16, device=DEV), torch.ones(16, device=DEV)
+    g, stats = torch.randn(20, 16, device=DEV), T.layer_norm(x, return_stats=True)[1:]
+    idx, off = torch.zeros(40, dtype=torch.int32, device=DEV), torch.arange(0, 40, 2, dtype=torch.int32, device=DEV)
+
+    def writes(out, call, *read):
+        before = out._version, [t._version for t in read]
+        leaf = torch.ones_like(out, requires_grad=True)
+        loss = (leaf * out).sum()
+        call()
+        assert out._version == before[0] + 1 and [t._version for t in read] == before[1]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+    for out in (torch.empty_like(x), x.clone()):
+        writes(out, lambda: T.layer_norm(x, w, out=out), x, w)
+        writes(out, lambda: T.layer_norm_backward(g, x, *stats, w, grad_x=out), g, x, w, *stats)
+    for rows in (30, 5000):
+        table, grad = torch.randn(rows, 16, device=DEV), torch.zeros(rows, 16, device=DEV)
+        for accumulate in (False, True):
+            writes(grad, lambda: T.embedding_bag_backward(g, table, idx, off, grad_table=grad, accumulate=accumulate), g, table, idx)
+    T.layer_norm(x, w)
+    assert x._version == 0
+    for bits in (32, 8):
+        p, master = torch.ones(300, device=DEV).half(), torch.ones(300, device=DEV)
+        opt = T.AdamW([p], masters=[master], state_bits=bits)
+        grad = torch.ones(300, device=DEV)
+        for t in (p, master):
+            before = t._version
+            opt.step([grad])
+            assert t._version == before + 1
+        assert grad._version == 0
+    p = torch.ones(300, device=DEV, requires_grad=True)
+    loss = (p * p).sum()
+    T.AdamW([p]).step([torch.ones(300, device=DEV)])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_tensors_of_inference_mode_are_taken():
+    with torch.inference_mode():
+        x, p = torch.randn(20, 16, device=DEV), torch.ones(300, device=DEV)
+        opt = T.AdamW([p])
+    T.layer_norm(x, out=x)
+    opt.step([torch.ones(300, device=DEV)])
+    assert (p < 1).all() and abs(float(x.mean())) < 1e-5
+
+
+def test_results_stand_outside_autograd():
+    x = torch.randn(20, 16, device=DEV, requires_grad=True)
+    y, mean, rstd = T.layer_norm(x, return_stats=True)
+    assert not y.requires_grad and not T.layer_norm_backward(y, x, mean, rstd)[0].requires_grad
