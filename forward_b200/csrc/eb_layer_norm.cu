@@ -74,6 +74,14 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[1]) {
   return one[0];
 }
 
+// sum / cols where a value is taken off that may be the mean itself (a row of one value): the product with 1 / cols, and what
+// it leaves of the sum shared out once more.  Two fused operations; a division in their place cost the
+// gradient of 32768 x 1000 bf16 5 % (50.6 us against 48.0).
+__device__ __forceinline__ float mean_of(float sum, float cols, float inv_cols) {
+  const float mean = sum * inv_cols, rest = fmaf(-mean, cols, sum);
+  return rest == rest ? fmaf(rest, inv_cols, mean) : mean;     // an infinite sum stays
+}
+
 template <int VEC>
 __device__ __forceinline__ void load_weight(const void* w, int dtype, int col, float unset, float (&f)[VEC]) {
   if (w) {
@@ -206,7 +214,7 @@ layer_norm_forward_kernel(const NormArgs a) {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
       each<VEC>([&](int i) { sum = add2(sum, at2(f[k], i)); }, [&](int i) { sum.x += f[k][i]; });
-    const float mean = row_sum<TPR>(sum.x + sum.y, red[0]) * inv_cols;
+    const float mean = mean_of(row_sum<TPR>(sum.x + sum.y, red[0]), (float)a.cols, inv_cols);
     float2 square = both(0.0f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -370,7 +378,7 @@ layer_norm_backward_kernel(const NormArgs a) {
     if (a.out) {
       float s[2] = {s1.x + s1.y, s2.x + s2.y};
       row_sum<TPR, 2>(s, red[turn]);
-      const float m1 = s[0] * inv_cols, m2 = s[1] * inv_cols;
+      const float m1 = mean_of(s[0], (float)a.cols, inv_cols), m2 = s[1] * inv_cols;
       T* gx = reinterpret_cast<T*>(a.out) + row * a.out_stride;
 #pragma unroll
       for (int k = 0; k < NV; ++k) {

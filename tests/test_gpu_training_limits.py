@@ -251,3 +251,31 @@ def test_results_stand_outside_autograd():
     x = torch.randn(20, 16, device=DEV, requires_grad=True)
     y, mean, rstd = T.layer_norm(x, return_stats=True)
     assert not y.requires_grad and not T.layer_norm_backward(y, x, mean, rstd)[0].requires_grad
+
+
+# ---- layer norm: rows of one value ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cols", [7, 41, 60, 63, 95, 100, 250, 777, 1000, 1023, 2000, 4095, 5000, 8000, 8191, 9000, 16000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_layer_norm_of_constant_rows_of_any_width(dtype, cols):
+    """x - mean is 0 in a row of one value, so y is the bias, and a constant grad_y has no gradient.  The values are small
+    integers: every sum of them is exact in fp32 (below 2^24), and so is the quotient."""
+    values = [1.0, 3.0, -7.0, 100.0, 1000.0]        # of 8 bits at most: bf16 holds them (1000 = 125 * 8)
+    x = torch.tensor(values, device=DEV).to(dtype)[:, None].expand(-1, cols).contiguous()
+    bias = torch.randn(cols, generator=gen(cols), device=DEV)
+    y, mean, rstd = T.layer_norm(x, None, bias, return_stats=True)
+    assert mean.tolist() == values
+    assert torch.equal(y, bias.to(dtype).expand(len(values), -1))
+    # h = 0 and g - mean(g) = 0
+    gx, gw, gb = T.layer_norm_backward(x, x, mean, rstd)
+    assert not gx.any() and not gw.any() and torch.equal(gb, torch.full_like(gb, sum(values)))
+
+
+@pytest.mark.parametrize("cols", [100, 1000, 20000])
+def test_layer_norm_mean_of_an_infinite_row(cols):
+    x = torch.ones(3, cols, device=DEV)
+    x[1, 5] = float("inf")
+    y, mean, _ = T.layer_norm(x, return_stats=True)
+    assert mean.tolist() == [1.0, float("inf"), 1.0]
+    assert torch.isnan(y[1, 5]) and not y[[0, 2]].any()
