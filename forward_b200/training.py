@@ -303,9 +303,9 @@ class AdamW:
             self.exp_avg_sq_scale = states(exp_avg_sq_scale, "exp_avg_sq_scale", torch.float32, blocks)
         written = self.params + [t for t in self.masters if t is not None] + self.exp_avg + self.exp_avg_sq
         written += (self.exp_avg_scale or []) + (self.exp_avg_sq_scale or [])
-        addresses = [t.data_ptr() for t in written if t.numel()]
-        if len(set(addresses)) < len(addresses):
-            raise ValueError("a parameter, master copy or state is there twice")
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in written if t.numel())
+        if any(end > begin for (_, end), (begin, _) in zip(spans, spans[1:])):
+            raise ValueError("a parameter, master copy or state is there twice, or two of them overlap")
         self._valued = self.params + [t for t in self.masters if t is not None]     # what a loss may have been computed from
         self._table = (AdamWTensor * n)()
         for i, p in enumerate(self.params):

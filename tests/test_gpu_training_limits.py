@@ -279,3 +279,22 @@ def test_layer_norm_mean_of_an_infinite_row(cols):
     y, mean, _ = T.layer_norm(x, return_stats=True)
     assert mean.tolist() == [1.0, float("inf"), 1.0]
     assert torch.isnan(y[1, 5]) and not y[[0, 2]].any()
+
+
+# ---- what AdamW is made from ----------------------------------------------------------------------
+
+
+def test_adamw_refuses_tensors_that_overlap():
+    """Every tensor of a step is a thread's own to read and write: views that share a part are as wrong as the same one twice."""
+    flat, state = torch.zeros(1000, device=DEV), torch.zeros(1000, device=DEV)
+    for a, b in ((flat[:600], flat[599:]), (flat[100:200], flat), (flat[600:], flat[:601])):
+        with pytest.raises(ValueError, match="overlap"):
+            T.AdamW([a, b])
+    with pytest.raises(ValueError, match="overlap"):
+        T.AdamW([flat[:500]], exp_avg=[state[:500]], exp_avg_sq=[state[499:999]])
+    with pytest.raises(ValueError, match="overlap"):
+        T.AdamW([flat[:500].view(torch.float16)], masters=[torch.zeros(1000, device=DEV)], exp_avg=[flat[499:1000].new_zeros(1000)],
+                exp_avg_sq=[flat])
+    halves = T.AdamW([flat[:500], flat[500:], flat[3:3]], exp_avg=[state[500:], state[:500], state[:0]])
+    halves.step([torch.ones(500, device=DEV), torch.ones(500, device=DEV), torch.zeros(0, device=DEV)])
+    assert (flat < 0).all() and same_bits(flat[:500], flat[500:])
