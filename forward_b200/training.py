@@ -262,6 +262,8 @@ class AdamW:
         self.device = self.params[0].device
         self.state_bits = state_bits
         self.step_count = int(step)
+        if self.step_count < 0:
+            raise ValueError(f"step counts the steps that were made (got {step})")
         n = len(self.params)
         decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(d) for d in weight_decay]
         if len(decay) != n:

@@ -298,3 +298,10 @@ def test_adamw_refuses_tensors_that_overlap():
     halves = T.AdamW([flat[:500], flat[500:], flat[3:3]], exp_avg=[state[500:], state[:500], state[:0]])
     halves.step([torch.ones(500, device=DEV), torch.ones(500, device=DEV), torch.zeros(0, device=DEV)])
     assert (flat < 0).all() and same_bits(flat[:500], flat[500:])
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_adamw_refuses_a_negative_step_count(capturable):
+    """From the device a count of 0 and less would divide by the zero that 1 - beta^0 is."""
+    with pytest.raises(ValueError, match="step"):
+        T.AdamW([torch.zeros(10, device=DEV)], step=-1, capturable=capturable)
