@@ -3,6 +3,7 @@ next to fp32's smallest, constant rows, chains of calls on one stream, refused a
 
 Tolerances are bounds of the arithmetic, as in test_gpu_training.py, whose helpers are used.
 """
+import ctypes as C
 import gc
 import math
 import weakref
@@ -305,3 +306,67 @@ def test_adamw_refuses_a_negative_step_count(capturable):
     """From the device a count of 0 and less would divide by the zero that 1 - beta^0 is."""
     with pytest.raises(ValueError, match="step"):
         T.AdamW([torch.zeros(10, device=DEV)], step=-1, capturable=capturable)
+
+
+# ---- malformed offsets ------------------------------------------------------------------------------
+
+
+def _back_params(s, go, grad, gw, winners, workspace=None, workspace_bytes=0):
+    out = torch.empty(0, device=DEV)
+    p = T.BackwardParams()
+    p.fwd = capi.make_params(s["table"], s["indices"], s["offsets"], out=out, mode=s["mode"], padding_idx=s["padding_idx"],
+                             include_last_offset=s["include_last_offset"])
+    p.grad_out, p.grad_out_dtype, p.grad_table_dtype = go.data_ptr(), capi.F32, capi.F32
+    p.grad_table = grad.data_ptr()
+    p.grad_weights = None if gw is None else gw.data_ptr()
+    p.winners = None if winners is None else winners.data_ptr()
+    p.workspace = None if workspace is None else workspace.data_ptr()
+    p.workspace_bytes = workspace_bytes
+    return p
+
+
+@pytest.mark.parametrize("idx", [torch.int32, torch.int64])
+@pytest.mark.parametrize("last", [False, True])
+@pytest.mark.parametrize("mode", [capi.MODE_SUM, capi.MODE_MEAN, capi.MODE_MAX, capi.MODE_SQUARE_SUM])
+@pytest.mark.parametrize("n,bags", [(300, 40), (1024, 1), (3000, 300), (20_000, 7), (20_000, 3000)])
+def test_malformed_offsets_stay_inside_the_buffers(n, bags, mode, last, idx):
+    """Offsets that decrease, or lie before the first lookup or far behind the last, give some gradient: the memory around the
+    results and the scratch stays as it was, inputs too, and the next well-formed call gives what it gave before."""
+    s, go, _, _ = make_bags(n, 900, 24, [n // bags] * (bags - 1) + [n - n // bags * (bags - 1)], mode=mode, dtype=torch.float32,
+                            idx=idx, pad=True, include_last=last)
+    go = go.contiguous()
+    lib, pad = T._lib(), 4096
+    winners = None
+    if mode == capi.MODE_MAX:
+        winners = T.embedding_bag_winners(s["table"], s["indices"], s["offsets"], padding_idx=s["padding_idx"], include_last_offset=last)
+    buf = torch.full((pad + 900 * 24 + pad,), 7.0, device=DEV)
+    wbuf = torch.full((pad + n + pad,), 7.0, device=DEV)
+    grad, gw = buf[pad:-pad], wbuf[pad:-pad] if mode == capi.MODE_SUM else None
+    need = lib.fwd_eb_backward_workspace_size(C.byref(_back_params(s, go, grad, gw, winners)))
+    scratch = torch.full((pad + (need + 255) // 256 * 256 + pad,), 5, dtype=torch.uint8, device=DEV)
+
+    def call(offsets):
+        t = dict(s, offsets=offsets)
+        p = _back_params(t, go, grad, gw, winners, scratch[pad:], need)
+        capi.check(lib.fwd_eb_backward(C.byref(p), capi.current_stream_ptr()))
+        torch.cuda.synchronize()
+        return grad.clone(), None if gw is None else gw.clone()
+
+    good, inputs = call(s["offsets"]), [t.clone() for t in (s["indices"], go, s["table"])]
+    far = torch.iinfo(idx)
+    g = gen(n + bags)
+    anywhere = torch.randint(-2 * n, 3 * n, s["offsets"].shape, generator=g, device=DEV).to(idx)
+    extremes = torch.tensor([far.min, far.max, -1, 0, n, n + 1], device=DEV, dtype=idx)[
+        torch.randint(0, 6, s["offsets"].shape, generator=g, device=DEV)]
+    dented = s["offsets"].clone()
+    dented[bags // 2] = 3 * n
+    dented[-1] = -5
+    for offsets in (s["offsets"].flip(0), anywhere, extremes, dented, torch.full_like(dented, far.max), torch.full_like(dented, far.min)):
+        kept = offsets.clone()
+        call(offsets)
+        for b in (buf, wbuf):
+            assert (b[:pad] == 7).all() and (b[-pad:] == 7).all()
+        assert (scratch[:pad] == 5).all() and (scratch[-pad:] == 5).all()
+        assert torch.equal(offsets, kept) and all(same_bits(a, b) for a, b in zip(inputs, (s["indices"], go, s["table"])))
+    again = call(s["offsets"])
+    assert same_bits(good[0], again[0]) and (gw is None or same_bits(good[1], again[1]))
