@@ -370,3 +370,51 @@ def test_malformed_offsets_stay_inside_the_buffers(n, bags, mode, last, idx):
         assert torch.equal(offsets, kept) and all(same_bits(a, b) for a, b in zip(inputs, (s["indices"], go, s["table"])))
     again = call(s["offsets"])
     assert same_bits(good[0], again[0]) and (gw is None or same_bits(good[1], again[1]))
+
+
+# ---- the weights' gradient by itself -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [1, 3, 4, 33, 1030, 2370, 9475, 40_003, 80_001])
+@pytest.mark.parametrize("dim", [1, 5, 64, 132, 260, 1100])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_weights_gradient_by_itself(dtype, dim, n):
+    """Numbers of lookups around those that a warp takes at a time; rows of one load a lane and of more; lookups of the padding row,
+    outside the table and before the first bag."""
+    g = gen(n + dim)
+    rows = 500
+    table = torch.randn(rows, dim, generator=g, device=DEV).to(dtype)
+    idx = torch.randint(-3, rows + 3, (n,), generator=g, device=DEV, dtype=torch.int32)
+    off = torch.arange(min(2, n - 1), n, 7, device=DEV, dtype=torch.int32)
+    go = torch.randn(off.numel(), dim, generator=g, device=DEV).to(dtype)
+    _, gw = T.embedding_bag_backward(go, table, idx, off, padding_idx=7, need_table=False, need_weights=True)
+    bag = (torch.arange(n, device=DEV) - off[0]).div(7, rounding_mode="floor")
+    keep = (bag >= 0) & (idx >= 0) & (idx < rows) & (idx != 7)
+    prod = go.to(F64)[bag.clamp(min=0)] * table.to(F64)[idx.long().clamp(0, rows - 1)] * keep[:, None]
+    within(gw, prod.sum(1), (dim + 2) * U * prod.abs().sum(1), "grad_weights")
+    assert not gw[~keep].any()
+
+
+def test_gather_gradient_right_behind_a_compaction():
+    """The indices that a window's compaction keeps are read by the next call's first kernel."""
+    batches = [make_bags(seed, 900, 64, [40] * 100, mode=capi.MODE_SUM, dtype=torch.float32) for seed in range(6)]
+    kept = torch.empty(4000, dtype=torch.int32, device=DEV)
+    bounds, pooled = torch.empty(100, 2, dtype=torch.int32, device=DEV), torch.empty(100, 64, device=DEV)
+    go = torch.randn(4000, 64, generator=gen(1), device=DEV)
+
+    def run(wait):
+        got = []
+        for s, _, _, _ in batches * 3:
+            window = s["table"][:500]
+            kept.fill_(-1)                                   # names no row
+            wait()
+            capi.compact_window(capi.make_params(window, s["indices"], s["offsets"], out=pooled), kept, bounds)
+            wait()
+            got.append(T.embedding_bag_backward(go, window, kept, mode=capi.MODE_GATHER)[0])
+            wait()
+        return got
+
+    want = run(torch.cuda.synchronize)
+    got = run(lambda: None)
+    torch.cuda.synchronize()
+    assert all(same_bits(a, b) for a, b in zip(got, want)) and want[0].any()
