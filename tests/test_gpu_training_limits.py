@@ -418,3 +418,50 @@ def test_gather_gradient_right_behind_a_compaction():
     got = run(lambda: None)
     torch.cuda.synchronize()
     assert all(same_bits(a, b) for a, b in zip(got, want)) and want[0].any()
+
+
+@pytest.mark.parametrize("mode", [capi.MODE_MEAN, capi.MODE_MAX])
+@pytest.mark.parametrize("bags,rows", [(16, 200), (3000, 20_000)])
+def test_a_captured_chain_of_calls_replays(bags, rows, mode):
+    """Lookup (with its winners), norm, both gradients and the step, two batches in one graph: three replays leave the bits of
+    six steps with a wait after each call."""
+    batches = [make_bags(seed, rows, 64, [9] * bags, mode=mode, dtype=torch.float32) for seed in range(2)]
+
+    def made():
+        table, w, b = torch.randn(rows, 64, generator=gen(1), device=DEV), torch.ones(64, device=DEV), torch.zeros(64, device=DEV)
+        grads = [torch.empty_like(t) for t in (table, w, b)]
+        opt = T.AdamW([table, w, b], state_bits=8, capturable=True, **HYPER)
+        opt.bind(grads)
+        return table, w, b, grads, opt
+
+    def steps(table, w, b, grads, opt, wait):
+        for s, go, _, _ in batches:
+            winners = None
+            if mode == capi.MODE_MAX:
+                winners = T.embedding_bag_winners(table, s["indices"], s["offsets"])
+                pooled = winners[..., 0].contiguous()
+            else:
+                pooled = capi.embedding_bag(table, s["indices"], s["offsets"], mode=mode)
+            wait()
+            y, mean, rstd = T.layer_norm(pooled, w, b, return_stats=True)
+            wait()
+            gx, gw, gb = T.layer_norm_backward(go, pooled, mean, rstd, w)
+            wait()
+            T.embedding_bag_backward(gx, table, s["indices"], s["offsets"], mode=mode, winners=winners, grad_table=grads[0])
+            wait()
+            grads[1].copy_(gw)
+            grads[2].copy_(gb)
+            opt.step()
+            wait()
+
+    eager, captured = made(), made()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps(*captured, lambda: None)
+    for _ in range(3):
+        steps(*eager, torch.cuda.synchronize)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert int(captured[4].step_tensor) == int(eager[4].step_tensor) == 6
+    assert all(same_bits(a, b) for a, b in zip(captured[:3], eager[:3]))
+    assert all(same_bits(a, b) for a, b in zip(captured[4].exp_avg_sq, eager[4].exp_avg_sq))
