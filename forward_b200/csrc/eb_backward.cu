@@ -819,7 +819,7 @@ __global__ void __launch_bounds__(256) zero_kernel(const BackArgs a) {     // no
 // 64 registers, four CTAs an SM: 205 us against 210.
 template <typename TG, int VE, int KIND, bool ACC, bool SAME>
 __global__ void __launch_bounds__(256, KIND == kWeights ? 4 : 0) segment_sum_kernel(const BackArgs a, const uint2* pairs) {
-  pdl_enter(true);
+  pdl_enter(a.runs > 1);
   int cta = blockIdx.x;
   if (!ACC && a.zero_blocks > 0) {
     const int before = (int)((long long)cta * a.zero_blocks / gridDim.x);        // zero CTAs among the earlier ones
@@ -1607,8 +1607,11 @@ int make_back_plan(const fwd_eb_backward_params* p, BackPlan* pl) {
   a.by_bag = !a.winners && !a.psw && !pl->fused_weights;
   // One launch for few lookups, although every CTA sorts them all and a popular row is the work of one CTA: 320 lookups
   // of a 10000 x 64 fp32 table 7.2 us against 17.0 in three launches, 1024 lookups 9.3 against 18.8, all 1024 of one
-  // row of it 17.2 against 18.5 (of a table of that row alone 16.8 against 14.2).
-  pl->tiny = a.n <= kTiny && pl->want_table;
+  // row of it 17.2 against 18.5 (of a table of that row alone 16.8 against 14.2).  The zeros of large tables are faster from
+  // the CTAs of the other form: 32 and 1024 lookups of 1 M x 128 fp16 (256 MB) 47 and 52 us against 51 and 56, of
+  // 1 M x 128 fp32 (512 MB) 89 and 93 against 85 and 90, of 4 M x 128 fp32 328 and 330 against 289 and 294.
+  const bool many_zeros = a.zero_blocks > 0 && f.num_rows * f.dim * (int64_t)te > 384LL << 20;
+  pl->tiny = a.n <= kTiny && pl->want_table && !many_zeros;
   if (pl->tiny) {
     a.by_bag = !a.winners && !a.psw && !a.grad_weights;
     if (a.zero_blocks > 0) {      // a share of the zeros for every CTA
@@ -1685,7 +1688,6 @@ cudaError_t launch_segments(const BackPlan& pl, const uint2* sorted, cudaStream_
     FWD_EB_TRY(launch_pdl(segment_block_kernel<VE>, blocks, 256, 0, st, a, sorted));
   }
   if (a.runs > 1) {
-    // the last kernel of every call that sorts by tiles or in one CTA: those have more than one run
     const dim3 joins((unsigned)((a.runs + 8 * kJoinRuns - 1) / (8 * kJoinRuns)), tiles);
     FWD_EB_TRY(launch_pdl(segment_join_kernel<VE>, joins, 256, 0, st, a, sorted));
   }

@@ -465,3 +465,40 @@ def test_a_captured_chain_of_calls_replays(bags, rows, mode):
     assert int(captured[4].step_tensor) == int(eager[4].step_tensor) == 6
     assert all(same_bits(a, b) for a, b in zip(captured[:3], eager[:3]))
     assert all(same_bits(a, b) for a, b in zip(captured[4].exp_avg_sq, eager[4].exp_avg_sq))
+
+
+# ---- few lookups of a large table ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [0, 1, 31, 32, 33, 64, 1024])
+@pytest.mark.parametrize("mode", [capi.MODE_SUM, capi.MODE_MEAN, capi.MODE_MAX, capi.MODE_SQUARE_SUM, capi.MODE_GATHER])
+def test_few_lookups_of_a_large_table(mode, n):
+    """Dense gradients of half a gigabyte, whose zeros want the launches of a large call: one run of sorted lookups and more."""
+    rows, dim = 4_100_000, 32
+    g = gen(n + mode)
+    table = torch.zeros(rows, dim, device=DEV)
+    named = torch.randint(0, rows, (max(n // 3, 1),), generator=g, device=DEV)
+    idx = named[torch.randint(0, named.numel(), (n,), generator=g, device=DEV)]
+    table[named] = torch.randn(named.numel(), dim, generator=g, device=DEV)
+    lengths = [n // 2, 0, n - n // 2]
+    off = torch.tensor([0, n // 2, n // 2], device=DEV, dtype=torch.int32)
+    go = torch.randn(n if mode == capi.MODE_GATHER else 3, dim, generator=g, device=DEV)
+    winners = T.embedding_bag_winners(table, idx.int(), off) if mode == capi.MODE_MAX and n else None
+    if mode == capi.MODE_MAX and not n:
+        winners = torch.zeros(3, dim, 2, device=DEV)
+    weights = mode == capi.MODE_SUM
+    out = torch.full((rows, dim), 7.0, device=DEV)
+    _, gw = T.embedding_bag_backward(go, table, idx.int(), None if mode == capi.MODE_GATHER else off, mode=mode, winners=winners,
+                                     grad_table=out, need_weights=weights)
+    small, to = torch.unique(idx, return_inverse=True)        # the same lookups of a table of the named rows alone
+    want, gw_want = T.embedding_bag_backward(go, table[small].contiguous(), to.int(), None if mode == capi.MODE_GATHER else off,
+                                             mode=mode, winners=winners, need_weights=weights)
+    bag = torch.arange(n, device=DEV) if mode == capi.MODE_GATHER else torch.repeat_interleave(
+        torch.arange(3, device=DEV), torch.tensor(lengths, device=DEV))
+    # both sums pass at most n additions, each lookup's product as in the formula
+    mag = torch.zeros(small.numel(), dim, device=DEV, dtype=F64).index_add_(0, to, go[bag].abs().to(F64))
+    if mode == capi.MODE_SQUARE_SUM:
+        mag = mag * 2 * table[small].abs().to(F64)
+    assert ((out[small].to(F64) - want.to(F64)).abs() <= 2 * (n + 16) * U * mag).all()
+    assert int((out != 0).any(1).sum()) == int((want != 0).any(1).sum())
+    assert not weights or ((gw - gw_want).abs().to(F64) <= 2 * (dim + 2) * U * (go[bag].abs() * table[idx].abs()).sum(1).to(F64)).all()
