@@ -11,8 +11,8 @@
 // shrink to a third and the instructions grow, so both count there: a whole chunk's two turns are loaded
 // at once, without bounds checks, and all arithmetic is on pairs (sm_100's packed fp32).
 // Measured on B200, of the copy rate measured there: 128 M fp16 parameters with master copies and
-// states of 32 bits 524 us, 1.04; 100 M in 26 tensors with states of 8 bits 174 us, 0.89 (32 instructions
-// an element: latency and issue slots bound it together).
+// states of 32 bits 531-534 us, 1.03; 100 M in 26 tensors with states of 8 bits 178-180 us, 0.86-0.87 (32 instructions
+// an element, 59 % of the issue slots: latency and issue slots bound it together).
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -491,7 +491,7 @@ cudaError_t launch_some(const fwd_eb_adamw_tensor* ts, int count, int* next, con
     ++found;
   }
   // 8-bit chunks of two turns, whose loads are under way together, where a few waves of CTAs are left even so: 100 M
-  // elements 174 us against 293 a turn at a time (202 and 220 with chunks of 4 and 8 turns)
+  // elements 178 us against 293 a turn at a time (202 and 220 with chunks of 4 and 8 turns)
   const long long wave = 3LL * sm_count();
   a.turns = KIND != 0 && total / kMostTurns >= 4 * wave ? kMostTurns : 1;
   long long chunks = 0;

@@ -14,9 +14,10 @@
 // of runs are first added 32 at a time.  Every sum has one order, whatever the schedule.
 //
 // Measured on B200 (a call, of the copy rate measured there): 655 k Zipf lookups of a 1 M x 128 fp16 table, mean, dense gradient
-// 119 us, 0.34: sort 38, sums beside zeros 66, joins 14; 262 k of a 1 M x 256 fp16 table, max 145 us, 0.56; 1.3 M weighted
-// lookups of a 4 M x 128 fp32 table, both gradients, accumulated 205 us, 0.37: sort 48, sums 136, bound by the latency of rows
-// from DRAM and by issue slots in like parts.
+// 113 us, 0.36: sort 38, sums beside zeros 66, joins 14; 262 k of a 1 M x 256 fp16 table, max 144 us, 0.57; 1.3 M weighted
+// lookups of a 4 M x 128 fp32 table, both gradients, accumulated 203 us, 0.37: sort 48, sums 136, bound by the latency of rows
+// from DRAM and by issue slots in like parts; 655 k uniform lookups of a 1 M x 128 fp16 table, square sum 144 us, 0.46 (65 % of
+// the issue slots in the sums), gather 115.
 //
 // The rows of a dense gradient that no lookup names are filled with zeros by other CTAs of the same launch, which
 // find the named ones in the sorted pairs: every row is written once, and the sums, bound by

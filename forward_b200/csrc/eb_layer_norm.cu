@@ -8,8 +8,8 @@
 // once and stay in registers as fp32; the mean is taken first, then the squared distances from it (no
 // cancellation).  Arithmetic is done on pairs (sm_100's packed fp32).
 //
-// Measured on B200 (a call, of the copy rate measured there): forward of 32768 x 4096 bf16 91-95 us, 0.87-0.90;
-// backward of 16383 x 2000 bf16 51 us, 0.59: a row's chain of loads, two sums and one barrier, with 125 registers
+// Measured on B200 (a call, of the copy rate measured there): forward of 32768 x 4096 bf16 94-96 us, 0.86-0.87;
+// backward of 16383 x 2000 bf16 50.5 us, 0.59: a row's chain of loads, two sums and one barrier, with 125 registers
 // a thread leaving 16 warps an SM to hide it (8 elements a thread and twice the warps measured 59).
 //
 // Rows that do not fit the registers of a CTA take the *_loop kernels, which read them again for

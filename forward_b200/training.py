@@ -3,7 +3,8 @@ EmbeddingBag call, layer norm with its gradients, and AdamW over many tensors at
 
 Like capi, the functions take torch CUDA tensors, launch on the current stream of the tensors'
 device and return without synchronising; outputs and scratch come from torch's allocator.
-Every result is deterministic.  There is no CPU path.
+Every result is deterministic; calls that accumulate into one gradient go one behind the other.
+There is no CPU path.
 
 They are the pieces of a hand-written step and stand outside autograd: results carry no graph, whatever
 their inputs require.  Tensors that a call is given to write into (not AdamW's states) count as changed in place.

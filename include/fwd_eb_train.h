@@ -9,7 +9,8 @@
  * Conventions are those of fwd_eb.h: device pointers of the current CUDA device, launches
  * on `stream` only, no allocation, no synchronisation, 0 / FWD_EB_E* / cudaError_t as
  * status.  Every result is deterministic: the same call on the same inputs gives the same
- * bits (no floating-point atomics anywhere).  All launches can be captured into a graph.
+ * bits.  Calls that write the same buffer (two gradients accumulated into one) go one behind the
+ * other; at the same time they have no defined result.  All launches can be captured into a graph.
  */
 #ifndef FWD_EB_TRAIN_H_
 #define FWD_EB_TRAIN_H_
@@ -30,7 +31,8 @@ enum { FWD_EB_BF16 = 3 };
 enum {
   /* add to what grad_table holds instead of overwriting it: rows that no lookup names are
    * neither read nor written, so the cost goes by the lookups and not by the table.  In fp32 the
-   * memory system adds, which takes subnormal values for zero */
+   * memory system adds, one atomic addition an element and call (so its order does not matter), which
+   * takes subnormal values for zero; in fp16 the row is read, added to in fp32 and rounded */
   FWD_EB_BACKWARD_ACCUMULATE = 1
 };
 
@@ -160,8 +162,10 @@ typedef struct fwd_eb_adamw_tensor {
  *       - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * in fp32.  8-bit states: each block of FWD_EB_ADAMW_BLOCK elements holds x as
  * scale * e4m3(x / scale), scale = max|x| / 448, rounded to nearest, for x = m and
- * x = sqrt(v); a sqrt(v) of 2^-63 and more never rounds to zero.  The update itself uses the
- * unrounded m and v.  An 8-bit v only follows changes larger than half a code (about 6 %
+ * x = sqrt(v); a sqrt(v) of 2^-63 and more never rounds to zero, and a block whose scale
+ * would be below 2^-126 holds zeros.  The update itself uses the
+ * unrounded m and v; a v below 2^-126 may count as zero where eps * sqrt(1 - beta2) >= 2^-38, which
+ * moves no update by more than half an ulp.  An 8-bit v only follows changes larger than half a code (about 6 %
  * of sqrt(v)) within a step relative to its block's largest: it suits beta2 of 0.95 or so.
  * A gradient that is not finite makes the states of its element NaN or infinite, and the
  * parameter from then on; in 8 bits an infinity does that to its whole block.  d_skip is there to
