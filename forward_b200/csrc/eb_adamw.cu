@@ -11,8 +11,8 @@
 // shrink to a third and the instructions grow, so both count there: a whole chunk's two turns are loaded
 // at once, without bounds checks, and all arithmetic is on pairs (sm_100's packed fp32).
 // Measured on B200, of the copy rate measured there: 128 M fp16 parameters with master copies and
-// states of 32 bits 531-534 us, 1.03; 100 M in 26 tensors with states of 8 bits 178-180 us, 0.86-0.87 (32 instructions
-// an element, 59 % of the issue slots: latency and issue slots bound it together).
+// states of 32 bits 531-534 us, 1.03; 100 M in 26 tensors with states of 8 bits 197 us, 0.79 (38 instructions
+// an element, 65 % of the issue slots: latency and issue slots bound it together).
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -52,7 +52,8 @@ struct AdamScalars {
   float step_size;     // lr / (1 - beta1^t)
   float root_scale;    // 1 / sqrt(1 - beta2^t)
   float log1, log2;    // log(beta), for a step that lies on the device
-  int flush;           // a subnormal v may count as zero (see hides_subnormal)
+  float none;          // -0, which the compiler does not know
+  int flush;           // a v near 2^-126 and below may count as less than it is (see hides_subnormal)
   long long step;
   const float* d_lr;
   const float* d_grad_scale;
@@ -139,14 +140,11 @@ __device__ __forceinline__ void decode(uint2 r, float (&f)[kLane]) {
 }
 
 // Root and reciprocal within an ulp or two, in one or a few instructions where the correctly rounded ones
-// take ten: the update is lr times smaller than the parameter it is added to, and a code or
-// scale of an 8-bit state is far coarser.  FTZ: a subnormal v counts as zero, where eps hides that.  The reciprocal's
-// argument sqrt(v) + eps is zero or normal: an eps above zero is normal, and the root of a subnormal v is.
-template <bool FTZ>
+// take ten: the update is lr times smaller than the parameter it is added to.  The reciprocal's argument
+// sqrt(v) + eps is zero or normal: an eps above zero is normal, and the root of a subnormal v is.
 __device__ __forceinline__ float quick_root(float x) {
   float y;
-  if (FTZ) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  else asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float quick_reciprocal(float x) {
@@ -154,34 +152,64 @@ __device__ __forceinline__ float quick_reciprocal(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
-// Codes of a block's values and its scale, the same in every lane: x ~ scale * e4m3(x / scale) with
-// scale = max|x| / 448.  Every lane of the warp calls it.  UP: x >= 0, and a value above zero
-// gets the smallest code at least.  A scale below the normal range counts as zero: its reciprocal
-// would not be finite.  A NaN gets the code of a NaN and does not touch the scale; an infinity makes
-// the scale infinite, and the whole block reads back as NaN.
-template <bool UP>
-__device__ __forceinline__ uint2 encode(const float (&x)[kLane], float& scale) {
+// What a code of 8 bits is made from is rounded as the formula is written, an operation at a time, so that the states are those of
+// plain fp32, whichever path a chunk takes: an ulp more or less makes another code of a value at a code's border, which is
+// a tenth of the state from then on.  Root and reciprocal by one step of Newton's iteration from the hardware's
+// approximation, with the residual exact in a fused operation (Markstein, 1990); they are the correctly rounded
+// ones but for a few in a million.  Of 200 M codes and 1 M scales none differs from torch's elementary operations (with fused
+// sums and the approximations by themselves 167 and a third), for 197 us in place of 178 (100 M elements in 26 tensors).
+__device__ __forceinline__ float reciprocal(float x) {      // normal, and so is 1 / x
+  const float y = quick_reciprocal(x);
+  return fmaf(fmaf(-x, y, 1.0f), y, y);
+}
+// Roots of two values, all with their signs turned (no negation is left to be done); NaN where a value is 0 (unless FTZ), infinite or
+// NaN.  FTZ: one below 2^-126 gives some value up to its root, which eps hides.
+template <bool FTZ>
+__device__ __forceinline__ float2 turned_roots(float2 x) {      // of -x
+  float2 s;
+  if (FTZ) {
+    const float2 w = fma2(x, both(-1.0f), both(FLT_MIN));     // no infinite reciprocal; far above it no change
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(w.x));
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(w.y));
+  } else {
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(s.x) : "f"(-x.x));
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(s.y) : "f"(-x.y));
+  }
+  const float2 y = mul2(x, s), over = fma2(y, y, x);
+  return fma2(over, mul2(s, both(0.5f)), y);
+}
+__device__ __forceinline__ float top_of(const float (&x)[kLane]) {      // the largest magnitude, NaN aside
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kLane; ++i) top = fmaxf(top, UP ? x[i] : fabsf(x[i]));
+  for (int i = 0; i < kLane; ++i) top = fmaxf(top, fabsf(x[i]));
+  return top;
+}
+
+// Codes of a block's values and its scale, the same in every lane: x ~ scale * e4m3(x / scale) with
+// scale = max|x| / 448, `top` being the lane's largest.  Every lane of the warp calls it.  TURNED: x <= 0 stands for -x, and a
+// value above zero gets the smallest code at least.  A scale below the normal range counts as zero: its reciprocal
+// would not be finite.  A NaN gets the code of a NaN and does not touch the scale; an infinity makes
+// the scale infinite, and the whole block reads back as NaN.
+template <bool TURNED>
+__device__ __forceinline__ uint2 encode(const float (&x)[kLane], float top, float& scale) {
   // floats that are not negative order as integers
   scale = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top))) * (float)(1.0 / 448.0);
   if (scale < FLT_MIN) scale = 0.0f;
-  const float inverse = scale > 0.0f ? quick_reciprocal(scale) : 0.0f;
+  float inverse = scale > 0.0f ? reciprocal(scale) : 0.0f;
+  if (TURNED) inverse = -inverse;
   unsigned w[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 t = mul2(make_float2(x[2 * i], x[2 * i + 1]), both(inverse));
     w[i / 2] |= (unsigned)__nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
   }
-  if (UP) {
+  if (TURNED) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       if (((w[k] - 0x01010101u) & ~w[k] & 0x80808080u) == 0) continue;   // no byte of it is zero
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (x[4 * k + i] > 0.0f && (w[k] & (0xffu << (8 * i))) == 0) w[k] |= 1u << (8 * i);
+        if (x[4 * k + i] < 0.0f && (w[k] & (0xffu << (8 * i))) == 0) w[k] |= 1u << (8 * i);
       }
     }
   }
@@ -190,41 +218,62 @@ __device__ __forceinline__ uint2 encode(const float (&x)[kLane], float& scale) {
 
 // What a step multiplies by, once device scalars are read.
 struct Rates {
-  float beta1, rest1, beta2, rest2, eps, grad_scale, step_size, root_scale, keep;
+  float beta1, rest1, beta2, rest2, eps, grad_scale, step_size, root_scale, keep, none;
 };
 
-// One lane's 8 elements: m and v come as loaded, to be multiplied by keep1 and keep2.
-template <bool FTZ>
-__device__ __forceinline__ void update(const Rates& r, float keep1, float keep2, float (&p)[kLane], const float (&g)[kLane],
-                                       float (&m)[kLane], float (&v)[kLane], float (&root)[kLane]) {
+// One lane's 8 elements.  BITS8: the states' roundings are those of the formula (see above); v comes out as -sqrt(v), and root_top is
+// the largest of its magnitudes.
+template <bool BITS8, bool FTZ>
+__device__ __forceinline__ void update(const Rates& r, float (&p)[kLane], const float (&g)[kLane], float (&m)[kLane],
+                                       float (&v)[kLane], float& root_top) {
+  float root[kLane];
+  root_top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kLane; i += 2) {
-    const float2 gi = mul2(make_float2(g[i], g[i + 1]), both(r.grad_scale));
-    const float2 mi = fma2(make_float2(m[i], m[i + 1]), both(keep1), mul2(gi, both(r.rest1)));
-    const float2 vi = fma2(make_float2(v[i], v[i + 1]), both(keep2), mul2(mul2(gi, gi), both(r.rest2)));
-    const float2 ri = make_float2(quick_root<FTZ>(vi.x), quick_root<FTZ>(vi.y));
-    const float2 den = fma2(ri, both(r.root_scale), both(r.eps));
-    const float2 upd = mul2(mi, make_float2(quick_reciprocal(den.x), quick_reciprocal(den.y)));
-    const float2 pi = fma2(make_float2(p[i], p[i + 1]), both(r.keep), mul2(upd, both(-r.step_size)));
+    const float2 gi = mul2(make_float2(g[i], g[i + 1]), both(r.grad_scale)), gg = mul2(gi, gi);
+    float2 mi = make_float2(m[i], m[i + 1]), vi = make_float2(v[i], v[i + 1]), ri;
+    if constexpr (BITS8) {
+      // products with -0 added: a product and a sum by themselves are made one operation by the compiler
+      const float2 none = both(r.none);
+      mi = add2(fma2(mi, both(r.beta1), none), fma2(gi, both(r.rest1), none));
+      vi = add2(fma2(vi, both(-r.beta2), none), fma2(gg, both(-r.rest2), none));
+      ri = turned_roots<FTZ>(vi);
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(root_top) : "f"(root_top), "f"(fabsf(ri.x)));
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(root_top) : "f"(root_top), "f"(fabsf(ri.y)));
+    } else {
+      mi = fma2(mi, both(r.beta1), mul2(gi, both(r.rest1)));
+      vi = fma2(vi, both(r.beta2), mul2(gg, both(r.rest2)));
+      ri = make_float2(quick_root(vi.x), quick_root(vi.y));
+    }
     m[i] = mi.x, m[i + 1] = mi.y;
     v[i] = vi.x, v[i + 1] = vi.y;
     root[i] = ri.x, root[i + 1] = ri.y;
+  }
+  if (BITS8) {
+    if (root_top != root_top) {
+#pragma unroll
+      for (int i = 0; i < kLane; ++i) root[i] = root[i] == root[i] ? root[i] : v[i];      // 0, infinity and NaN are their own roots
+      root_top = top_of(root);
+    }
+#pragma unroll
+    for (int i = 0; i < kLane; ++i) v[i] = root[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kLane; i += 2) {
+    const float2 den = fma2(make_float2(root[i], root[i + 1]), both(BITS8 ? -r.root_scale : r.root_scale), both(r.eps));
+    const float2 upd = mul2(make_float2(m[i], m[i + 1]), make_float2(quick_reciprocal(den.x), quick_reciprocal(den.y)));
+    const float2 pi = fma2(make_float2(p[i], p[i + 1]), both(r.keep), mul2(upd, both(-r.step_size)));
     p[i] = pi.x, p[i + 1] = pi.y;
   }
 }
-__device__ __forceinline__ void square(float (&v)[kLane]) {   // of codes: exact
+// m and v from their codes, sqrt(v)'s scale before the square: its own leaves the normal range already where v is 2e5 times 2^-126.
+__device__ __forceinline__ void scaled(float (&m)[kLane], float m_scale, float (&v)[kLane], float v_scale) {
 #pragma unroll
   for (int i = 0; i < kLane; i += 2) {
-    const float2 c = make_float2(v[i], v[i + 1]), c2 = mul2(c, c);
-    v[i] = c2.x, v[i + 1] = c2.y;
-  }
-}
-// v from codes of sqrt(v).  Their scale's own square leaves the normal range already where v is 2e5 times 2^-126.
-__device__ __forceinline__ void square_scaled(float (&v)[kLane], float scale) {
-#pragma unroll
-  for (int i = 0; i < kLane; i += 2) {
-    const float2 c = mul2(make_float2(v[i], v[i + 1]), both(scale)), c2 = mul2(c, c);
-    v[i] = c2.x, v[i + 1] = c2.y;
+    const float2 a = mul2(make_float2(m[i], m[i + 1]), both(m_scale)), b = mul2(make_float2(v[i], v[i + 1]), both(v_scale));
+    const float2 c = mul2(b, b);
+    m[i] = a.x, m[i + 1] = a.y;
+    v[i] = c.x, v[i + 1] = c.y;
   }
 }
 
@@ -272,7 +321,7 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
     if (a.t[mid].first <= blockIdx.x) lo = mid; else hi = mid;
   }
   AdamTensor t = a.t[lo];
-  Rates r = {a.s.beta1, a.s.rest1, a.s.beta2, a.s.rest2, a.s.eps, a.s.grad_scale, a.s.step_size, a.s.root_scale, t.keep};
+  Rates r = {a.s.beta1, a.s.rest1, a.s.beta2, a.s.rest2, a.s.eps, a.s.grad_scale, a.s.step_size, a.s.root_scale, t.keep, a.s.none};
   if (a.s.d_grad_scale) r.grad_scale = *a.s.d_grad_scale;
   if (a.s.d_lr || a.s.d_step) {
     // 1 - beta^t = -expm1(t log beta): no cancellation, in fp32
@@ -315,16 +364,15 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
       to.vs = t.v_scale[at / FWD_EB_ADAMW_BLOCK];
     };
     auto turn = [&](const Ahead& now, int at) {
-      float p[kLane], g[kLane], m[kLane], v[kLane], root[kLane];
+      float p[kLane], g[kLane], m[kLane], v[kLane], root_top;
       now.p.get(ftype, p);
       now.g.get(t.gtype, g);
       decode(now.m, m);
       decode(now.v, v);
-      const float keep1 = now.ms * r.beta1, keep2 = now.vs * now.vs * r.beta2;   // what vs^2 loses below 2^-126, eps hides too
-      square(v);
-      update<true>(r, keep1, keep2, p, g, m, v, root);
+      scaled(m, now.ms, v, now.vs);
+      update<true, true>(r, p, g, m, v, root_top);
       float ms, vs;
-      const uint2 cm = encode<false>(m, ms), cv = encode<true>(root, vs);
+      const uint2 cm = encode<false>(m, top_of(m), ms), cv = encode<true>(v, root_top, vs);
       if (PWIDE && t.master) store_any<kLane>(t.master, FWD_EB_F32, at, p);
       store_any<kLane>(t.param, t.ptype, at, p);
       *reinterpret_cast<uint2*>(static_cast<char*>(t.m) + at) = cm;
@@ -347,31 +395,30 @@ adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
     if (left <= at - (int)(threadIdx.x & 31) * kLane) return;   // the warp's first element: all its lanes go on together
     const int n = left - at < 0 ? 0 : (left - at < kLane ? left - at : kLane);
     const bool whole = n == kLane && t.aligned;
-    float p[kLane], g[kLane], m[kLane], v[kLane], root[kLane];
+    float p[kLane], g[kLane], m[kLane], v[kLane], root_top;
     load_lane(t.grad, t.gtype, at, n, whole, g);
     load_lane(from, ftype, at, n, whole, p);
     const int block = at / FWD_EB_ADAMW_BLOCK;
-    float keep1 = r.beta1;
     if (BITS8) {
       const uint2 cm = load_codes(t.m, at, n, whole), cv = load_codes(t.v, at, n, whole);
-      keep1 *= t.m_scale[block];
       decode(cm, m);
       decode(cv, v);
-      square_scaled(v, t.v_scale[block]);
+      scaled(m, t.m_scale[block], v, t.v_scale[block]);
     } else {
       load_lane(t.m, FWD_EB_F32, at, n, whole, m);
       load_lane(t.v, FWD_EB_F32, at, n, whole, v);
     }
-    update<false>(r, keep1, r.beta2, p, g, m, v, root);
+    update<BITS8, false>(r, p, g, m, v, root_top);
     if (t.master) store_lane(t.master, FWD_EB_F32, at, n, whole, p);
     store_lane(t.param, t.ptype, at, n, whole, p);
     if (BITS8) {
 #pragma unroll
       for (int i = 0; i < kLane; ++i) {   // what lies behind the tensor's end takes no part in its last scale
-        if (i >= n) m[i] = root[i] = 0.0f;
+        if (i >= n) m[i] = v[i] = 0.0f;
       }
+      root_top = top_of(v);
       float ms, vs;
-      const uint2 cm = encode<false>(m, ms), cv = encode<true>(root, vs);
+      const uint2 cm = encode<false>(m, top_of(m), ms), cv = encode<true>(v, root_top, vs);
       store_codes(t.m, at, n, whole, cm);
       store_codes(t.v, at, n, whole, cv);
       if ((threadIdx.x & 31) == 0) {
@@ -426,7 +473,7 @@ int check_adamw(const fwd_eb_adamw_tensor* ts, int32_t count, const fwd_eb_adamw
   return 0;
 }
 
-// Whether eps hides what is lost where every v below 2^-126 counts as zero.  A step then loses less than
+// Whether eps hides what is lost where a v near 2^-126 and below counts as less than it is.  A step then loses less than
 // 2^-126 of v, steps 1 to t together less than 2^-126 (1 - beta2^t) / (1 - beta2), so sqrt(v / (1 - beta2^t)) is off by
 // less than 2^-63 / sqrt(1 - beta2).  That is half an ulp of a denominator of at least eps where eps is 2^24 times as
 // large, and 2^25 leaves room for what v loses when it is decoded: 1.6e-11 at beta2 = 0.95, 1.2e-10 at 0.999.
@@ -447,6 +494,7 @@ AdamScalars scalars_of(const fwd_eb_adamw_config* c) {
   s.log1 = (float)std::log(c->beta1);
   s.log2 = (float)std::log(c->beta2);
   s.step = c->step;
+  s.none = -0.0f;
   s.flush = hides_subnormal(c->eps, c->beta2);
   s.d_lr = c->d_lr;
   s.d_grad_scale = c->d_grad_scale;
@@ -491,7 +539,8 @@ cudaError_t launch_some(const fwd_eb_adamw_tensor* ts, int count, int* next, con
     ++found;
   }
   // 8-bit chunks of two turns, whose loads are under way together, where a few waves of CTAs are left even so: 100 M
-  // elements 178 us against 293 a turn at a time (202 and 220 with chunks of 4 and 8 turns)
+  // elements 174 us against 293 a turn at a time (202 and 220 with chunks of 4 and 8 turns; before the states' roundings
+  // were the formula's, 197 us now)
   const long long wave = 3LL * sm_count();
   a.turns = KIND != 0 && total / kMostTurns >= 4 * wave ? kMostTurns : 1;
   long long chunks = 0;

@@ -163,9 +163,11 @@ typedef struct fwd_eb_adamw_tensor {
  * in fp32.  8-bit states: each block of FWD_EB_ADAMW_BLOCK elements holds x as
  * scale * e4m3(x / scale), scale = max|x| / 448, rounded to nearest, for x = m and
  * x = sqrt(v); a sqrt(v) of 2^-63 and more never rounds to zero, and a block whose scale
- * would be below 2^-126 holds zeros.  The update itself uses the
- * unrounded m and v; a v below 2^-126 may count as zero where eps * sqrt(1 - beta2) >= 2^-38, which
- * moves no update by more than half an ulp.  An 8-bit v only follows changes larger than half a code (about 6 %
+ * would be below 2^-126 holds zeros.  m, v, sqrt(v), the scale and x * (1 / scale) are rounded an operation at a
+ * time, so that the codes are those of the formulas in plain fp32 (root and reciprocal: but for a few in a
+ * million).  The update itself uses the
+ * unrounded m and v; a v near 2^-126 and below may count as less than it is where
+ * eps * sqrt(1 - beta2) >= 2^-38, which moves no update by more than half an ulp.  An 8-bit v only follows changes larger than half a code (about 6 %
  * of sqrt(v)) within a step relative to its block's largest: it suits beta2 of 0.95 or so.
  * A gradient that is not finite makes the states of its element NaN or infinite, and the
  * parameter from then on; in 8 bits an infinity does that to its whole block.  d_skip is there to

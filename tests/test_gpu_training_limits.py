@@ -13,7 +13,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from forward_b200 import capi, training as T  # noqa: E402
-from test_gpu_training import DEV, F64, HYPER, U, from_codes, gen, make_bags, same_bits, within  # noqa: E402
+from test_gpu_training import DEV, F64, HYPER, U, adam_case, from_codes, gen, make_bags, same_bits, within  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -502,3 +502,44 @@ def test_few_lookups_of_a_large_table(mode, n):
     assert ((out[small].to(F64) - want.to(F64)).abs() <= 2 * (n + 16) * U * mag).all()
     assert int((out != 0).any(1).sum()) == int((want != 0).any(1).sum())
     assert not weights or ((gw - gw_want).abs().to(F64) <= 2 * (dim + 2) * U * (go[bag].abs() * table[idx].abs()).sum(1).to(F64)).all()
+
+
+# ---- AdamW: states of 8 bits as plain fp32 gives them ---------------------------------------------------
+
+
+@pytest.mark.parametrize("param,grad,master", [
+    (torch.float32, torch.float32, False), (torch.float16, torch.float16, False), (torch.bfloat16, torch.float32, True)])
+def test_adamw_states_of_8_bits_are_those_of_plain_fp32(param, grad, master):
+    """Three steps over long chunks, short ones, ragged ends and an odd address, against the formulas in torch's elementary
+    operations.  One of those more or less fused moves a few codes in a million, by up to an eighth each.  A root or a
+    reciprocal is off by an ulp once in 2^18: 110000 blocks have two scales with one of each, and a code follows only
+    where its value is next to a border besides."""
+    sizes = [9_000_001, 3000, 257, 70_000]
+    c = adam_case(11, sizes, param, grad, 8, master, 1)
+    c["params"][0], c["grads"][0] = c["params"][0].clone(), c["grads"][0].clone()       # the long one at an even address
+    for k in ("m", "v") + (("masters",) if master else ()):
+        c[k][0] = c[k][0].clone()
+    (b1, b2), least = HYPER["betas"], 2.0 ** -9
+    opt = T.AdamW(c["params"], state_bits=8, masters=c["masters"], exp_avg=c["m"], exp_avg_sq=c["v"], exp_avg_scale=c["ms"],
+                  exp_avg_sq_scale=c["vs"], **HYPER)
+    odd_scales = 0
+    for step in range(3):
+        held = [[t.clone() for t in c[k]] for k in ("m", "v", "ms", "vs")]
+        opt.step(c["grads"], grad_scale=0.7 + step)
+        for i, n in enumerate(sizes):
+            m8, v8, ms, vs = (h[i] for h in held)
+            wide = lambda s: s.repeat_interleave(256)[:n]  # noqa: E731
+            g = c["grads"][i].float() * (0.7 + step)
+            m = (m8.float() * wide(ms)) * b1 + g * (1 - b1)
+            v = (v8.float() * wide(vs)).square() * b2 + (g * g) * (1 - b2)
+            for x, code, scale, up in ((m, c["m"][i], c["ms"][i], False), (v.sqrt(), c["v"][i], c["vs"][i], True)):
+                pad = torch.zeros(scale.numel() * 256, device=DEV)
+                pad[:n] = x
+                want = pad.view(-1, 256).abs().amax(1) * (1.0 / 448.0)
+                ulps = (want.view(torch.int32) - scale.view(torch.int32)).abs()
+                assert int(ulps.max()) <= 1
+                odd_scales += int((ulps > 0).sum())
+                t = x * wide(torch.where(scale > 0, 1 / scale, torch.zeros_like(scale)))
+                t = torch.where(x > 0, t.clamp(min=least), t) if up else t
+                assert same_bits(t.clamp(-448, 448).to(torch.float8_e4m3fn), code), (i, step, up)
+    assert odd_scales <= 8
