@@ -206,6 +206,7 @@ __device__ __forceinline__ uint2 encode(const float (&x)[kLane], float top, floa
   if (TURNED) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
+      w[k] &= 0x7f7f7f7fu;                                               // a zero has no sign
       if (((w[k] - 0x01010101u) & ~w[k] & 0x80808080u) == 0) continue;   // no byte of it is zero
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -543,3 +543,18 @@ def test_adamw_states_of_8_bits_are_those_of_plain_fp32(param, grad, master):
                 t = torch.where(x > 0, t.clamp(min=least), t) if up else t
                 assert same_bits(t.clamp(-448, 448).to(torch.float8_e4m3fn), code), (i, step, up)
     assert odd_scales <= 8
+
+
+@pytest.mark.parametrize("n", [5000, 9_000_001])
+def test_adamw_zeros_of_8_bits_are_code_0(n):
+    """Elements that never had a gradient: no sign, no smallest code, whichever path their chunk takes; whole blocks of them too."""
+    p, g = torch.ones(n, device=DEV), torch.zeros(n, device=DEV)
+    g[::600] = 0.5
+    g[4::600] = -0.5
+    opt = T.AdamW([p], state_bits=8, **dict(HYPER, weight_decay=0.0))
+    for _ in range(2):
+        opt.step([g])
+        for t in (opt.exp_avg[0], opt.exp_avg_sq[0]):
+            assert torch.equal(t.view(torch.uint8) != 0, g != 0)
+        assert not (opt.exp_avg_sq[0].view(torch.uint8) & 0x80).any()
+        assert (p[g == 0] == 1).all() and (p[g != 0] != 1).all()
